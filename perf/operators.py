@@ -1,0 +1,317 @@
+"""The operators of a gated feed-forward block as measured work: their plain forms, the framework's calls, and their definition in 64 bits.
+
+  rms_norm            y = h / sqrt(mean(h^2) + eps) * w with h = x + r, forward and backward (points of a field, tokens of a batch)
+  rms_norm_quantized  the same y as 8-bit codes with one scale a row, for serving
+  int8_linear         8-bit activations times 8-bit weights with a scale for each row and each channel; in two of the forms the
+                      activations arrive as floats and are quantised by quantize_rows in the same pass
+  int8_gated_linear   gate and up projections of the block in 8 bits, their activation and product
+  gated_mlp           act(x Wg^T) * (x Wu^T) Wd^T, forward for serving, forward and backward for training
+"""
+import math
+
+import torch
+
+own = False
+
+EPS = 1e-6
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+BYTES = {"fp32": 4, "bf16": 2, "fp16": 2}
+ACTS = ("silu", "gelu")  # smooth ones: a gradient at a kink is decided by the last bit of a sum
+
+
+def listed():
+    return [
+        # a training step's norm between two blocks over one batch of a surface model: 4096 rays of 128 samples, 256 features
+        dict(name="norm_train_points", op="rms_norm", rows=4096 * 128, dim=256, dtype="bf16", residual=True),
+        # the first norm of a stack: no residual yet, full precision, a row count and a width that fit no tile
+        dict(name="norm_train_odd", op="rms_norm", rows=4099, dim=1001, dtype="fp32", residual=False),
+        # one token of a serving loop
+        dict(name="norm_quant_one", op="rms_norm_quantized", rows=1, dim=4096, dtype="bf16", residual=True),
+        # a prompt, or a large batch of them
+        dict(name="norm_quant_batch", op="rms_norm_quantized", rows=16384, dim=4096, dtype="fp16", residual=True),
+        # one token through a square projection: the weights are read once
+        dict(name="int8_one", op="int8_linear", rows=1, dim=4096, out=4096, dtype="bf16", bias=True, floats=False),
+        # a ragged chunk of points into an odd number of channels, quantised on the way
+        dict(name="int8_odd", op="int8_linear", rows=4099, dim=1000, out=1111, dtype="fp32", bias=True, floats=True),
+        # a prompt through a wide projection
+        dict(name="int8_prompt", op="int8_linear", rows=16384, dim=4096, out=8192, dtype="bf16", bias=False, floats=False),
+        # a small batch of single tokens through the gate and up projections
+        dict(name="int8_gated_few", op="int8_gated_linear", rows=24, dim=4096, hidden=8192, dtype="bf16", act="silu", floats=False),
+        # an evaluation chunk of 4096 rays x 128 samples through a field's block, quantised on the way
+        dict(name="int8_gated_points", op="int8_gated_linear", rows=4096 * 128, dim=256, hidden=512, dtype="fp16", act="gelu", floats=True),
+        # one token of a serving loop through the whole block
+        dict(name="gated_one", op="gated_mlp", rows=1, dim=4096, hidden=16384, dtype="bf16", act="silu", train=False),
+        # a training step of a field's block in full precision on one batch of points
+        dict(name="gated_train_points", op="gated_mlp", rows=4096 * 128, dim=256, hidden=512, dtype="fp32", act="gelu", train=True),
+        # a training step of a wide block on a batch of tokens
+        dict(name="gated_train_tokens", op="gated_mlp", rows=8192, dim=4096, hidden=16384, dtype="bf16", act="silu", train=True),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["rms_norm", "rms_norm_quantized", "int8_linear", "int8_gated_linear", "gated_mlp", "gated_mlp"])
+    dtype = rng.choice(["fp32", "bf16", "fp16"])
+    odd = rng.random() < 0.4  # widths that fit nothing; the others are multiples of 64, as most networks have
+
+    def width(lo, hi):
+        n = _log(rng, lo, hi)
+        return n if odd else max(64, n // 64 * 64)
+
+    if op in ("rms_norm", "rms_norm_quantized"):
+        dim = width(17, 8192)
+        return dict(op=op, rows=_log(rng, 1, min(4096 * 128, (1 << 26) // dim)), dim=dim, dtype=dtype, residual=rng.random() < 0.6)
+    if op == "int8_linear":
+        dim, out = width(33, 8192), width(33, 8192)
+        return dict(op=op, rows=_log(rng, 1, min(4096 * 128, (1 << 38) // (dim * out))), dim=dim, out=out, dtype=dtype,
+                    bias=rng.random() < 0.5, floats=rng.random() < 0.5)
+    dim, hidden = width(33, 4096), width(33, 8192)
+    act = rng.choice(ACTS)
+    if op == "int8_gated_linear":
+        return dict(op=op, rows=_log(rng, 1, min(4096 * 64, (1 << 37) // (dim * hidden))), dim=dim, hidden=hidden, dtype=dtype, act=act,
+                    floats=rng.random() < 0.5)
+    train = rng.random() < 0.6
+    return dict(op=op, rows=_log(rng, 1, min(4096 * 64, (1 << 37) // (dim * hidden))), dim=dim, hidden=hidden, dtype=dtype, act=act, train=train)
+
+
+def _codes(x):
+    """Symmetric 8-bit codes of each row and their scales, as weights are stored."""
+    x = x.float()
+    top = x.abs().amax(dim=-1, keepdim=True)
+    return torch.round(x * (127.0 / top)).to(torch.int8), (top / 127.0).squeeze(-1)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed * 1000003 + 17)
+    t = TYPES[case["dtype"]]
+    rows, dim = case["rows"], case["dim"]
+
+    def normal(*shape, std=1.0):
+        return torch.randn(*shape, generator=g, device="cuda") * std
+
+    s = {"case": case}
+    # features of unequal size, as networks have them
+    spread = torch.exp(0.5 * normal(dim))
+    if case["op"] in ("rms_norm", "rms_norm_quantized"):
+        s["x"] = (normal(rows, dim) * spread).to(t)
+        s["r"] = normal(rows, dim).to(t) if case["residual"] else None
+        s["w"] = (1.0 + normal(dim, std=0.2)).to(t)
+        if case["op"] == "rms_norm":
+            s["dy"] = normal(rows, dim).to(t)
+            s["dh"] = normal(rows, dim).to(t) if case["residual"] else None
+            if own:
+                for k in ("x", "r", "w"):
+                    if s[k] is not None:
+                        s[k].requires_grad_(True)
+        return s
+    x = (normal(rows, dim) * spread).to(t)
+    if case["op"] == "gated_mlp":
+        hidden = case["hidden"]
+        s["x"] = x
+        s["wg"] = normal(hidden, dim, std=dim ** -0.5).to(t)
+        s["wu"] = normal(hidden, dim, std=dim ** -0.5).to(t)
+        s["wd"] = normal(dim, hidden, std=hidden ** -0.5).to(t)
+        if case["train"]:
+            s["dy"] = normal(rows, dim).to(t)
+            if own:
+                for k in ("x", "wg", "wu", "wd"):
+                    s[k].requires_grad_(True)
+        return s
+    if case["floats"]:
+        s["x"] = x
+    else:
+        s["q"], s["sx"] = _codes(x)
+    if case["op"] == "int8_linear":
+        s["wq"], s["sw"] = _codes(normal(case["out"], dim, std=dim ** -0.5))
+        s["b"] = normal(case["out"], std=0.1) if case["bias"] else None
+    else:
+        s["gq"], s["sg"] = _codes(normal(case["hidden"], dim, std=dim ** -0.5))
+        s["uq"], s["su"] = _codes(normal(case["hidden"], dim, std=dim ** -0.5))
+    return s
+
+
+# ------------------------------------------------------------------------------------------------ plain forms, 32 bits
+def _act(name, z):
+    if name == "silu":
+        return z / (1.0 + torch.exp(-z))
+    return 0.5 * z * (1.0 + torch.erf(z * math.sqrt(0.5)))
+
+
+def _plain_norm(x, r, w):
+    h = x if r is None else x + r
+    inv = 1.0 / torch.sqrt((h * h).mean(dim=-1, keepdim=True) + EPS)
+    return h, inv, h * inv * w
+
+
+def _plain_codes(v):
+    """In 64 bits: a value next to the border of two codes would go to either of them by the last bit of 32."""
+    step = v.abs().amax(dim=-1, keepdim=True) / 127.0
+    return torch.where(step > 0, torch.round(v / step), torch.zeros_like(v)).float(), step
+
+
+def _plain(s):
+    case = s["case"]
+    t = TYPES[case["dtype"]]
+    op = case["op"]
+    if op == "rms_norm":
+        x = s["x"].float().requires_grad_(True)
+        r = None if s["r"] is None else s["r"].float().requires_grad_(True)
+        w = s["w"].float().requires_grad_(True)
+        h, _, y = _plain_norm(x, r, w)
+        if r is None:
+            dx, dw = torch.autograd.grad(y, (x, w), s["dy"].float())
+            return [y.detach().to(t), dx.to(t), dw.to(t)]
+        dx, dr, dw = torch.autograd.grad((y, h), (x, r, w), (s["dy"].float(), s["dh"].float()))
+        return [y.detach().to(t), h.detach().to(t), dx.to(t), dr.to(t), dw.to(t)]
+    if op == "rms_norm_quantized":
+        h, inv, _ = _plain_norm(s["x"].double(), None if s["r"] is None else s["r"].double(), s["w"].double())
+        q, step = _plain_codes(h * s["w"].double())  # the codes do not depend on the row's norm
+        out = [q * (step * inv).float()]
+        return out if s["r"] is None else out + [h.to(t)]
+    if op == "gated_mlp":
+        names = ("x", "wg", "wu", "wd")
+        x, wg, wu, wd = (s[k].float().requires_grad_(case["train"]) for k in names)
+        y = (_act(case["act"], x @ wg.t()) * (x @ wu.t())) @ wd.t()
+        if not case["train"]:
+            return y.to(t)
+        return [y.detach().to(t)] + [d.to(t) for d in torch.autograd.grad(y, (x, wg, wu, wd), s["dy"].float())]
+    out = []
+    if case["floats"]:
+        q, sx = _plain_codes(s["x"].double())
+        sx = sx.float()
+        out.append(q * sx)
+    else:
+        q, sx = s["q"].float(), s["sx"][:, None]
+    if op == "int8_linear":
+        y = q @ s["wq"].float().t() * sx * s["sw"]
+        out.append((y if s["b"] is None else y + s["b"]).to(t))
+    else:
+        gate = q @ s["gq"].float().t() * sx * s["sg"]
+        up = q @ s["uq"].float().t() * sx * s["su"]
+        out.append((_act(case["act"], gate) * up).to(t))
+    return out
+
+
+# ------------------------------------------------------------------------------------------------ the framework's calls
+def _framework(s):
+    from sdfstudio_amd.field_components.mlp import gated_mlp
+    from sdfstudio_amd.field_components.normalization import rms_norm, rms_norm_quantized
+    from sdfstudio_amd.field_components.quantization import int8_gated_linear, int8_linear, quantize_rows
+
+    case = s["case"]
+    op = case["op"]
+    t = TYPES[case["dtype"]]
+    if op == "rms_norm":
+        if s["r"] is None:
+            y = rms_norm(s["x"], s["w"], eps=EPS)
+            return [y.detach(), *torch.autograd.grad(y, (s["x"], s["w"]), s["dy"])]
+        y, h = rms_norm(s["x"], s["w"], residual=s["r"], eps=EPS)
+        return [y.detach(), h.detach(), *torch.autograd.grad((y, h), (s["x"], s["r"], s["w"]), (s["dy"], s["dh"]))]
+    if op == "rms_norm_quantized":
+        if s["r"] is None:
+            q, scale = rms_norm_quantized(s["x"], s["w"], eps=EPS)
+            return [q * scale[:, None]]
+        q, scale, h = rms_norm_quantized(s["x"], s["w"], residual=s["r"], eps=EPS)
+        return [q * scale[:, None], h]
+    if op == "gated_mlp":
+        y = gated_mlp(s["x"], s["wg"], s["wu"], s["wd"], activation=case["act"])
+        if not case["train"]:
+            return y
+        return [y.detach(), *torch.autograd.grad(y, (s["x"], s["wg"], s["wu"], s["wd"]), s["dy"])]
+    out = []
+    if case["floats"]:
+        q, sx = quantize_rows(s["x"])
+        out.append(q * sx[:, None])
+    else:
+        q, sx = s["q"], s["sx"]
+    if op == "int8_linear":
+        out.append(int8_linear(q, sx, s["wq"], s["sw"], bias=s["b"], out_dtype=t))
+    else:
+        out.append(int8_gated_linear(q, sx, s["gq"], s["sg"], s["uq"], s["su"], activation=case["act"], out_dtype=t))
+    return out
+
+
+def run(state):
+    return _framework(state) if own else _plain(state)
+
+
+# ------------------------------------------------------------------------------------------------ the definition in 64 bits
+def _exact_act(name, z):
+    """The activation and its derivative."""
+    if name == "silu":
+        p = torch.sigmoid(z)
+        return z * p, p * (1 + z * (1 - p))
+    phi = 0.5 * torch.erfc(-z / math.sqrt(2))
+    return z * phi, phi + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+
+
+def _exact_codes(v):
+    step = v.abs().amax(dim=-1, keepdim=True) / 127
+    return torch.where(step > 0, torch.round(v / step), torch.zeros_like(v)), step
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    d = {k: v.detach().double() for k, v in s.items() if isinstance(v, torch.Tensor)}
+    op = case["op"]
+    with torch.no_grad():
+        if op in ("rms_norm", "rms_norm_quantized"):
+            h = d["x"] + d["r"] if case["residual"] else d["x"]
+            inv = torch.rsqrt(h.square().sum(-1, keepdim=True) / h.shape[-1] + EPS)
+            if op == "rms_norm_quantized":
+                q, step = _exact_codes(h * d["w"])  # inv divides out of the codes, and its rounding would break their ties
+                return [q * step * inv, h] if case["residual"] else [q * step * inv]
+            n = h * inv
+            u = d["dy"] * d["w"]
+            dx = inv * (u - n * (u * n).mean(-1, keepdim=True))
+            dw = (d["dy"] * n).sum(0)
+            if not case["residual"]:
+                return [n * d["w"], dx, dw]
+            return [n * d["w"], h, dx + d["dh"], dx + d["dh"], dw]
+        if op == "gated_mlp":
+            gate, up = d["x"] @ d["wg"].t(), d["x"] @ d["wu"].t()
+            a, slope = _exact_act(case["act"], gate)
+            y = (a * up) @ d["wd"].t()
+            if not case["train"]:
+                return y
+            dwd = d["dy"].t().contiguous() @ (a * up)
+            dhid = d["dy"] @ d["wd"]
+            dgate, dup = dhid * up * slope, dhid * a
+            del dhid, a, slope, up, gate
+            return [y, dgate @ d["wg"] + dup @ d["wu"], dgate.t().contiguous() @ d["x"], dup.t().contiguous() @ d["x"], dwd]
+        out = []
+        if case["floats"]:
+            q, sx = _exact_codes(d["x"])
+            out.append(q * sx)
+        else:
+            q, sx = d["q"], d["sx"][:, None]
+        if op == "int8_linear":
+            y = (q * sx) @ (d["wq"] * d["sw"][:, None]).t()
+            out.append(y + d["b"] if case["bias"] else y)
+        else:
+            gate, up = (q * sx) @ (d["gq"] * d["sg"][:, None]).t(), (q * sx) @ (d["uq"] * d["su"][:, None]).t()
+            out.append(_exact_act(case["act"], gate)[0] * up)
+        return out
+
+
+def work(case):
+    b, m, k = BYTES[case["dtype"]], case["rows"], case["dim"]
+    op = case["op"]
+    if op == "rms_norm":  # forward x (r) -> y (h); backward x (r) dy (dh) -> one gradient that serves both inputs
+        tensors = 9 if case["residual"] else 5
+        return {"bytes": tensors * m * k * b + 2 * k * b, "flops": 12 * m * k}
+    if op == "rms_norm_quantized":
+        tensors = 3 if case["residual"] else 1
+        return {"bytes": tensors * m * k * b + m * k + 4 * m + k * b, "flops": 6 * m * k}
+    if op == "gated_mlp":
+        f = case["hidden"]
+        if not case["train"]:
+            return {"bytes": b * (2 * m * k + 3 * k * f), "flops": 6 * m * k * f}
+        return {"bytes": b * (4 * m * k + 6 * k * f), "flops": 18 * m * k * f}
+    n = case["out"] if op == "int8_linear" else case["hidden"]
+    both = 1 if op == "int8_linear" else 2
+    read = m * k * b if case["floats"] else m * k + 4 * m
+    return {"bytes": read + both * (n * k + 4 * n) + m * n * b, "flops": 2 * both * m * n * k}
