@@ -147,9 +147,10 @@ def _plain_norm(x, r, w):
 
 
 def _plain_codes(v):
-    """In 64 bits: a value next to the border of two codes would go to either of them by the last bit of 32."""
-    step = v.abs().amax(dim=-1, keepdim=True) / 127.0
-    return torch.where(step > 0, torch.round(v / step), torch.zeros_like(v)).float(), step
+    """In 64 bits: a value next to the border of two codes would go to either of them by the last bit of 32.  One division, of exact
+    numbers: half the largest value lies ON a border, and goes to the even code."""
+    top = v.abs().amax(dim=-1, keepdim=True)
+    return torch.where(top > 0, torch.round(v * 127.0 / top), torch.zeros_like(v)).float(), top / 127.0
 
 
 def _plain(s):
@@ -249,8 +250,8 @@ def _exact_act(name, z):
 
 
 def _exact_codes(v):
-    step = v.abs().amax(dim=-1, keepdim=True) / 127
-    return torch.where(step > 0, torch.round(v / step), torch.zeros_like(v)), step
+    top = v.abs().amax(dim=-1, keepdim=True)
+    return torch.where(top > 0, torch.round(127 * v / top), torch.zeros_like(v)), top / 127
 
 
 def exact(case, seed):
