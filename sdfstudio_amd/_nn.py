@@ -1,0 +1,127 @@
+"""ctypes binding of libsdfnn.so (the C ABI declared in include/sdfnn.h): the gated feed-forward block's operators.
+
+No fallback, as _lib.py: a missing library or a failing call raises.  PyTorch provides device memory and the stream.
+"""
+import ctypes
+import os
+from typing import Optional, Tuple
+
+import torch
+
+_HERE = os.path.dirname(os.path.abspath(__file__))
+LIB_PATH = os.environ.get("SDFNN_LIB", os.path.join(_HERE, "libsdfnn.so"))
+
+_p, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+_SIGNATURES = {
+    "sdfnn_version": (ctypes.c_int, []),
+    "sdfnn_last_error": (ctypes.c_char_p, []),
+    "sdfnn_rms_norm_forward": (ctypes.c_int, [_p, _i64, _p, _i64, _p, _i32, _i64, _i64, _f32, _p, _p, _p, _p]),
+    "sdfnn_rms_norm_backward_workspace_size": (_i64, [_i64, _i64]),
+    "sdfnn_rms_norm_backward": (ctypes.c_int, [_p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _i64, _i32, _i64, _i64, _p, _p, _p, _i64, _p]),
+    "sdfnn_rms_norm_quantize": (ctypes.c_int, [_p, _i64, _p, _i64, _p, _i32, _i64, _i64, _f32, _p, _p, _p, _p]),
+    "sdfnn_int8_linear_workspace_size": (_i64, [_i64, _i64, _i64, _i32]),
+    "sdfnn_int8_linear": (ctypes.c_int, [_p, _i64, _p, _p, _i64, _p, _p, _i32, _i64, _i64, _i64, _p, _p, _i64, _p]),
+    "sdfnn_int8_gated_linear": (ctypes.c_int, [_p, _i64, _p, _p, _i64, _p, _p, _i64, _p, _i32, _i32, _i64, _i64, _i64, _p, _p, _i64, _p]),
+    "sdfnn_gated_saved_size": (_i64, [_i32, _i64, _i64]),
+    "sdfnn_gated_workspace_size": (_i64, [_i32, _i64, _i64, _i64, _i64, _i32]),
+    "sdfnn_gated_forward": (ctypes.c_int, [_p, _i64, _p, _p, _p, _i32, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p]),
+    "sdfnn_gated_backward": (ctypes.c_int, [_p, _i64, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p]),
+}
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
+_lib: Optional[ctypes.CDLL] = None
+
+
+class SdfNnError(RuntimeError):
+    pass
+
+
+def load() -> ctypes.CDLL:
+    """Load libsdfnn.so; raises if it has not been built (python -m sdfstudio_amd.build / __graft_entry__.build())."""
+    global _lib
+    if _lib is not None:
+        return _lib
+    if not os.path.exists(LIB_PATH):
+        raise SdfNnError(f"{LIB_PATH} is missing: build the HIP extensions first (python -m sdfstudio_amd.build). "
+                         "There is no CPU fallback for the gated block.")
+    lib = ctypes.CDLL(LIB_PATH)
+    for name, (restype, argtypes) in _SIGNATURES.items():
+        fn = getattr(lib, name)  # AttributeError if the symbol is not exported
+        fn.restype = restype
+        fn.argtypes = argtypes
+    _lib = lib
+    return lib
+
+
+def last_error() -> str:
+    return (load().sdfnn_last_error() or b"").decode(errors="replace")
+
+
+def check(rc: int, what: str):
+    if rc != 0:
+        raise SdfNnError(f"{what} failed ({rc}): {last_error()}")
+
+
+def dtype_code(t: torch.Tensor, what: str) -> int:
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what}: {t.dtype} is not supported (float32, bfloat16, float16)")
+    return code
+
+
+def activation_code(name: str, what: str) -> int:
+    if name not in ACTIVATIONS:
+        raise ValueError(f"{what}: activation {name!r}: one of {sorted(ACTIVATIONS)}")
+    return ACTIVATIONS[name]
+
+
+def on_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
+    """The one HIP device that every tensor of a call lives on."""
+    if not first.is_cuda:
+        raise SdfNnError(f"{what} runs on the sdfnn kernels: HIP device tensors required (no CPU fallback)")
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+    return first.device
+
+
+def rows_of(t: torch.Tensor, align: bool = False) -> Tuple[torch.Tensor, int]:
+    """t [..., dim] as rows: ([rows, dim] whose rows the kernels can walk, row stride in elements).  A view wherever that is possible; a
+    copy for rows that are not adjacent in memory, overlap, or - with `align` - do not start at 16-byte boundaries although their width
+    would allow it."""
+    dim = t.shape[-1]
+    rows = 1
+    for s in t.shape[:-1]:
+        rows *= s
+    t2 = t.reshape(rows, dim)
+    stride = t2.stride(0) if rows > 1 else dim
+    es = t2.element_size()
+    bad = (dim > 1 and t2.stride(1) != 1) or (dim == 1 and rows > 1 and stride < 1) or stride < dim
+    if align and dim * es % 16 == 0:
+        bad = bad or t2.data_ptr() % 16 != 0 or stride * es % 16 != 0
+    if bad:
+        t2 = t2.clone(memory_format=torch.contiguous_format)
+        stride = dim
+    return t2, stride
+
+
+def aligned(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor that starts at a 16-byte boundary (weights: a slice of a flat parameter buffer may not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+    """Scratch memory of one call, from the caching allocator: it goes back when the call has been issued, in stream order, and inside a
+    graph capture it belongs to that graph's pool - no two calls or graphs share one."""
+    if nbytes < 0:
+        raise SdfNnError("sizes refused by the library")
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+
+def stream():
+    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)

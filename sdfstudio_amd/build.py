@@ -122,8 +122,43 @@ def build_mesh(verbose: bool = True) -> str:
     return MESH_LIB
 
 
+# ---- libsdfnn.so: the gated feed-forward block's operators (include/sdfnn.h), a separate library for the same reason.
+NN_CSRC = os.path.join(HERE, "csrc_nn")
+NN_LIB = os.path.join(HERE, "libsdfnn.so")
+# -packed-fp32-ops: scalar fp32 instructions only (their packed forms save no time beside matrix instructions or HBM-bound loops)
+NN_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-slp-vectorize", "-Xclang", "-target-feature", "-Xclang",
+            "-packed-fp32-ops", "-Wno-unused-result", "-Wno-unused-function"]
+
+
+def nn_source_digest() -> str:
+    h = hashlib.sha256()
+    h.update(" ".join(NN_FLAGS).encode())
+    for path in [os.path.join(NN_CSRC, n) for n in sorted(os.listdir(NN_CSRC)) if n.endswith((".h", ".hip"))] + \
+            [os.path.join(HERE, "..", "include", "sdfnn.h")]:
+        with open(path, "rb") as fh:
+            h.update(fh.read())
+    return h.hexdigest()[:16]
+
+
+def build_nn(verbose: bool = True) -> str:
+    digest = nn_source_digest()
+    stamp = NN_LIB + ".digest"
+    prev = open(stamp).read().strip() if os.path.exists(stamp) else ""
+    if prev != digest or not os.path.exists(NN_LIB):
+        cmd = [_hipcc(), *NN_FLAGS, "-shared", "-I", NN_CSRC, os.path.join(NN_CSRC, "nn_api.hip"), "-o", NN_LIB]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"hipcc failed for nn_api.hip:\n{r.stdout}\n{r.stderr}")
+        with open(stamp, "w") as fh:
+            fh.write(digest)
+    if verbose:
+        print(f"[sdfhip] built {NN_LIB} ({os.path.getsize(NN_LIB) / 1e6:.1f} MB)")
+    return NN_LIB
+
+
 def build(verbose: bool = True) -> str:
     build_mesh(verbose)
+    build_nn(verbose)
     os.makedirs(BUILD, exist_ok=True)
     with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, min(len(SOURCES), os.cpu_count() or 1))) as ex:
         objs = list(ex.map(_compile, SOURCES))

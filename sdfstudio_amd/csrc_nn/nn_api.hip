@@ -1,0 +1,411 @@
+// libsdfnn.so: the gated feed-forward block's operators (include/sdfnn.h).  gfx950 only.
+#include <math.h>
+#include <stdarg.h>
+#include <stdio.h>
+
+#include "nn_launch.h"
+#include "norm_kernels.h"
+
+namespace {
+thread_local char g_err[512] = "";
+}
+void sdfnn_set_error(const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+}
+
+#define NN_TRY(expr)                \
+  do {                              \
+    if (const int rc_ = (expr)) return rc_; \
+  } while (0)
+
+namespace {
+
+constexpr int64_t kMaxRows = 0x7fffffff, kMaxDim = (int64_t)1 << 24;
+
+bool aligned16(const void* p, const int64_t ld_bytes) { return ((uintptr_t)p & 15) == 0 && (ld_bytes & 15) == 0; }
+
+// ---------------------------------------------------------------------------------------------- norm
+// f(IC<TPR>, IC<NV>, IC<RPB>) for the row width: how many threads and registers hold a row (norm_kernels.h)
+template <int N> using IC = std::integral_constant<int, N>;
+template <class F>
+void pick_row(const int64_t dim, F&& f) {
+  if (dim <= 512) f(IC<64>{}, IC<1>{}, IC<4>{});
+  else if (dim <= 1024) f(IC<64>{}, IC<2>{}, IC<4>{});
+  else if (dim <= 2048) f(IC<64>{}, IC<4>{}, IC<4>{});
+  else if (dim <= 4096) f(IC<256>{}, IC<2>{}, IC<1>{});
+  else if (dim <= 8192) f(IC<256>{}, IC<4>{}, IC<1>{});
+  else if (dim <= 32768) f(IC<1024>{}, IC<4>{}, IC<1>{});
+  else f(IC<1024>{}, IC<0>{}, IC<1>{});
+}
+
+int check_norm(const char* what, const void* x, const int64_t ldx, const void* residual, const int64_t ldr, const int32_t dtype,
+               const int64_t rows, const int64_t dim) {
+  NN_REQUIRE(dtype >= SDFNN_F32 && dtype <= SDFNN_F16, "%s: dtype %d", what, dtype);
+  NN_REQUIRE(rows >= 0 && rows <= kMaxRows, "%s: %lld rows", what, (long long)rows);
+  NN_REQUIRE(dim >= 1 && dim <= kMaxDim, "%s: rows of %lld elements (1 .. 2^24)", what, (long long)dim);
+  NN_REQUIRE(x, "%s: null tensor", what);
+  NN_REQUIRE(ldx >= dim && (!residual || ldr >= dim), "%s: a row stride is smaller than the row", what);
+  return 0;
+}
+
+template <int DT>
+int norm_forward(const NormArgs& a, hipStream_t s) {
+  pick_row(a.dim, [&](auto tpr, auto nv, auto rpb) {
+    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, RPB = decltype(rpb)::value;
+    hipLaunchKernelGGL((rms_norm_fwd_kernel<DT, TPR, NV, RPB>), dim3((unsigned)ceil_div(a.rows, RPB)), dim3(TPR * RPB), 0, s, a);
+  });
+  NN_LAUNCHED("rms_norm_forward");
+  return 0;
+}
+template <int DT>
+int norm_quantize(const NormArgs& a, hipStream_t s) {
+  pick_row(a.dim, [&](auto tpr, auto nv, auto rpb) {
+    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, RPB = decltype(rpb)::value;
+    hipLaunchKernelGGL((rms_norm_quant_kernel<DT, TPR, NV, RPB>), dim3((unsigned)ceil_div(a.rows, RPB)), dim3(TPR * RPB), 0, s, a);
+  });
+  NN_LAUNCHED("rms_norm_quantize");
+  return 0;
+}
+
+// workgroups of the backward pass (= partial sums of dweight): enough to fill the chip, few enough that their sums are small beside the tensors
+int64_t bwd_groups(const int64_t rows, const int64_t dim) {
+  const int64_t per = dim <= 2048 ? 4 : 1;
+  const int64_t most = dim <= 2048 ? 1024 : dim <= 8192 ? 1024 : 256;
+  return std::max<int64_t>(1, std::min(most, ceil_div(rows, per)));
+}
+template <int DT>
+int norm_backward(NormArgs a, elem_t<DT>* dw, hipStream_t s) {
+  const int64_t groups = bwd_groups(a.rows, a.dim);
+  bool wide = false;
+  if (a.rows > 0)
+    pick_row(a.dim, [&](auto tpr, auto nv, auto rpb) {
+      constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, RPB = decltype(rpb)::value;
+      wide = NV == 0;
+      if (dw && NV > 0) hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, TPR, NV, RPB, true>), dim3((unsigned)groups), dim3(TPR * RPB), 0, s, a);
+      else if (a.dx) hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, TPR, NV, RPB, false>), dim3((unsigned)groups), dim3(TPR * RPB), 0, s, a);
+    });
+  NN_LAUNCHED("rms_norm_backward");
+  if (!dw) return 0;
+  if (wide) hipLaunchKernelGGL((rms_norm_dw_wide_kernel<DT>), dim3((unsigned)ceil_div(a.dim, 256), (unsigned)groups), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((rms_norm_dw_reduce_kernel<DT>), dim3((unsigned)ceil_div(a.dim, 64)), dim3(1024), 0, s, a.partial,
+                     a.rows > 0 ? (int)groups : 0, a.dim, dw);
+  NN_LAUNCHED("rms_norm_backward (weight)");
+  return 0;
+}
+
+// ---------------------------------------------------------------------------------------------- 8-bit products
+// an operand that the tiles read where it lies, or its copy with rows of whole steps
+int int8_operand(Call& c, const int8_t* p, const int64_t ld, const int64_t rows, const int64_t k, const bool direct, Operand& o) {
+  if (direct) {
+    o = {(const char*)p, ld, 0};
+    return 0;
+  }
+  return pack_rows<1>(c, p, ld, rows, k, round_up(k, 128), o);
+}
+
+template <int DT, bool DUAL>
+int int8_products(Call& c, const int8_t* q, const int64_t ldq, const int8_t* w0, const int64_t ld0, const int8_t* w1, const int64_t ld1,
+                  const int64_t rows, const int64_t n, const int64_t k, const Int8Epi<DT>& epi) {
+  if (rows <= kSkinnyRows) {
+    const Operand a{(const char*)q, ldq, 0}, b0{(const char*)w0, ld0, 0}, b1{(const char*)w1, ld1, 0};
+    return skinny<2, DUAL>(c, a, b0, b1, rows, n, k, n, epi);
+  }
+  const bool direct = k % 16 == 0;
+  Operand a{}, b0{}, b1{};
+  NN_TRY(int8_operand(c, q, ldq, rows, k, direct, a));
+  NN_TRY(int8_operand(c, w0, ld0, n, k, direct, b0));
+  if (DUAL) NN_TRY(int8_operand(c, w1, ld1, n, k, direct, b1));
+  return product<2, 1, DUAL>(c, a, b0, b1, rows, n, direct ? k : round_up(k, 128), epi);
+}
+
+int check_int8(const char* what, const int8_t* q, const int64_t ldq, const int8_t* w0, const int64_t ld0, const int8_t* w1, const int64_t ld1,
+               const int32_t dtype, const int64_t rows, const int64_t n, const int64_t k) {
+  NN_REQUIRE(dtype >= SDFNN_F32 && dtype <= SDFNN_F16, "%s: dtype %d", what, dtype);
+  NN_REQUIRE(rows >= 0 && rows <= kMaxRows, "%s: %lld rows", what, (long long)rows);
+  NN_REQUIRE(n >= 1 && n <= kMaxDim, "%s: %lld channels (1 .. 2^24)", what, (long long)n);
+  NN_REQUIRE(k >= 1 && k <= 131072, "%s: k = %lld: the 32-bit sum is exact for 1 .. 131072", what, (long long)k);
+  NN_REQUIRE(q && w0 && w1, "%s: null tensor", what);
+  NN_REQUIRE(ldq >= k && ld0 >= k && ld1 >= k, "%s: a row stride is smaller than the row", what);
+  if (rows > kSkinnyRows && k % 16 == 0)
+    NN_REQUIRE(aligned16(q, ldq) && aligned16(w0, ld0) && aligned16(w1, ld1),
+               "%s: with k a multiple of 16 rows have to start at 16-byte boundaries", what);
+  return 0;
+}
+
+template <class F>
+int by_dtype(const int32_t dtype, F&& f) {
+  if (dtype == SDFNN_F32) return f(IC<SDFNN_F32>{});
+  if (dtype == SDFNN_BF16) return f(IC<SDFNN_BF16>{});
+  return f(IC<SDFNN_F16>{});
+}
+
+// ---------------------------------------------------------------------------------------------- gated MLP
+template <int DT> struct Kind {  // of the tile and of the few-row product
+  static constexpr int tile = DT == SDFNN_F16 ? 1 : 0, few = DT == SDFNN_F32 ? 3 : DT == SDFNN_F16 ? 1 : 0;
+  static constexpr int terms = DT == SDFNN_F32 ? 6 : 1, es = elem_size(DT);
+  static constexpr bool f32 = DT == SDFNN_F32;
+};
+
+// [rows, cols] with its k along the row: where it lies if the tiles can read it there (direct: 16-bit rows of a multiple of 8), else a copy
+template <int DT>
+int row_operand(Call& c, const void* p, const int64_t ld, const int64_t rows, const int64_t cols, const bool direct, Operand& o) {
+  if (direct && !Kind<DT>::f32) {
+    o = {(const char*)p, ld * 2, 0};
+    return 0;
+  }
+  return pack_rows<Kind<DT>::es>(c, p, ld, rows, cols, round_up(cols, 64), o);
+}
+
+template <int DT>
+int gated_forward(Call& c, const void* x, const int64_t ldx, const void* wg, const void* wu, const void* wd, const int act, const int64_t M,
+                  const int64_t D, const int64_t F, const int64_t O, const bool save, void* saved, void* y) {
+  typedef elem_t<DT> T;
+  typedef Kind<DT> K;
+  const int64_t Fp = round_up(F, 64), es = K::es;
+  T *gs = nullptr, *us = nullptr, *a;
+  if (save) gs = (T*)saved, us = gs + M * Fp, a = us + M * Fp;
+  else a = (T*)c.take(M * Fp * es);
+  const GatedEpi<DT> ge{a, gs, us, (int)Fp, act};
+  const StoreEpi<DT> se{(T*)y, nullptr, M, M, 0, O, (int)O};
+  if (M <= kSkinnyRows) {
+    const Operand xo{(const char*)x, ldx * es, 0}, g{(const char*)wg, D * es, 0}, u{(const char*)wu, D * es, 0};
+    const Operand ao{(const char*)a, Fp * es, 0}, d{(const char*)wd, F * es, 0};
+    NN_TRY((skinny<K::few, true>(c, xo, g, u, M, F, D * es, Fp, ge)));
+    return skinny<K::few, false>(c, ao, d, d, M, O, F * es, O, se);
+  }
+  const bool d8 = D % 8 == 0, f8 = F % 8 == 0;
+  Operand xo, g, u, ao, d;
+  NN_TRY(row_operand<DT>(c, x, ldx, M, D, d8, xo));
+  NN_TRY(row_operand<DT>(c, wg, D, F, D, d8, g));
+  NN_TRY(row_operand<DT>(c, wu, D, F, D, d8, u));
+  NN_TRY((product<K::tile, K::terms, true>(c, xo, g, u, M, F, (d8 && !K::f32 ? D : round_up(D, 64)) * 2, ge)));
+  NN_TRY(row_operand<DT>(c, a, Fp, M, Fp, true, ao));
+  NN_TRY(row_operand<DT>(c, wd, F, O, F, f8, d));
+  return product<K::tile, K::terms, false>(c, ao, d, d, M, O, (f8 && !K::f32 ? F : Fp) * 2, se);
+}
+
+template <int DT>
+int gated_backward(Call& c, const void* x, const int64_t ldx, const void* wg, const void* wu, const void* wd, const void* saved, const void* dy,
+                   const int64_t lddy, const int act, const int64_t M, const int64_t D, const int64_t F, const int64_t O, void* dx, void* dwg,
+                   void* dwu, void* dwd) {
+  typedef elem_t<DT> T;
+  typedef Kind<DT> K;
+  constexpr bool F32 = K::f32;
+  const int64_t Fp = round_up(F, 64), Op = round_up(O, 64), Mp = round_up(M, 64);
+  const T *gs = (const T*)saved, *us = gs + M * Fp, *a = us + M * Fp;
+  T* dgu = (T*)c.take(M * 2 * Fp * K::es);
+  const bool o8 = O % 8 == 0;
+  const int64_t start = c.used;  // the operands of one product make room for those of the next
+  int64_t most = start;
+  auto next = [&]() { most = std::max(most, c.used), c.used = start; };
+  if (dx || dwg) {
+    Operand dyo, wdt = take_operand<F32>(c, F, Op);
+    NN_TRY(row_operand<DT>(c, dy, lddy, M, O, o8, dyo));
+    NN_TRY(pack_transposed<F32>(c, wd, F, O, F, Op, 0, wdt));
+    const GatedBwdEpi<DT> be{gs, us, dgu, (int)Fp, act};
+    NN_TRY((product<K::tile, K::terms, false>(c, dyo, wdt, wdt, M, F, (o8 && !F32 ? O : Op) * 2, be)));
+    next();
+  }
+  if (dx) {
+    Operand d, w = take_operand<F32>(c, D, 2 * Fp);
+    NN_TRY(row_operand<DT>(c, dgu, 2 * Fp, M, 2 * Fp, true, d));
+    NN_TRY(pack_transposed<F32>(c, wg, D, F, D, Fp, 0, w));
+    NN_TRY(pack_transposed<F32>(c, wu, D, F, D, Fp, Fp, w));
+    const StoreEpi<DT> se{(T*)dx, nullptr, M, M, 0, D, (int)D};
+    NN_TRY((product<K::tile, K::terms, false>(c, d, w, w, M, D, 2 * Fp * 2, se)));
+    next();
+  }
+  if (dwd) {
+    Operand dyt = take_operand<F32>(c, O, Mp), at = take_operand<F32>(c, F, Mp);
+    NN_TRY(pack_transposed<F32>(c, dy, lddy, M, O, Mp, 0, dyt));
+    NN_TRY(pack_transposed<F32>(c, a, Fp, M, F, Mp, 0, at));
+    const StoreEpi<DT> se{(T*)dwd, nullptr, O, O, 0, F, (int)F};
+    NN_TRY((product<K::tile, K::terms, false>(c, dyt, at, at, O, F, Mp * 2, se)));
+    next();
+  }
+  if (dwg) {
+    Operand dt = take_operand<F32>(c, 2 * Fp, Mp), xt = take_operand<F32>(c, D, Mp);
+    NN_TRY(pack_transposed<F32>(c, dgu, 2 * Fp, M, 2 * Fp, Mp, 0, dt));
+    NN_TRY(pack_transposed<F32>(c, x, ldx, M, D, Mp, 0, xt));
+    const StoreEpi<DT> se{(T*)dwg, (T*)dwu, Fp, F, F, D, (int)D};
+    NN_TRY((product<K::tile, K::terms, false>(c, dt, xt, xt, 2 * Fp, D, Mp * 2, se)));
+    next();
+  }
+  c.used = most;
+  return 0;
+}
+
+int check_gated(const char* what, const int32_t dtype, const int32_t act, const int64_t rows, const int64_t dim, const int64_t hidden,
+                const int64_t out) {
+  NN_REQUIRE(dtype >= SDFNN_F32 && dtype <= SDFNN_F16, "%s: dtype %d", what, dtype);
+  NN_REQUIRE(act >= SDFNN_SILU && act <= SDFNN_RELU, "%s: activation %d", what, act);
+  NN_REQUIRE(rows >= 0 && rows <= kMaxRows, "%s: %lld rows", what, (long long)rows);
+  NN_REQUIRE(dim >= 1 && hidden >= 1 && out >= 1 && dim <= 1 << 20 && hidden <= 1 << 20 && out <= 1 << 20,
+             "%s: widths %lld, %lld, %lld (1 .. 2^20)", what, (long long)dim, (long long)hidden, (long long)out);
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sdfnn_version(void) { return 100; }
+const char* sdfnn_last_error(void) { return g_err; }
+
+int sdfnn_rms_norm_forward(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int32_t dtype, int64_t rows,
+                           int64_t dim, float eps, void* y, void* h, float* inv, sdfnn_stream_t stream) {
+  NN_TRY(check_norm("rms_norm_forward", x, ldx, residual, ldr, dtype, rows, dim));
+  NN_REQUIRE(weight && y, "rms_norm_forward: null tensor");
+  NN_REQUIRE(eps >= 0.0f && eps < INFINITY, "rms_norm_forward: eps %g", (double)eps);
+  if (rows == 0) return 0;
+  NormArgs a{};
+  a.x = x, a.ldx = ldx, a.r = residual, a.ldr = ldr, a.w = weight, a.rows = rows, a.dim = dim, a.eps = eps;
+  a.y = y, a.h = residual ? h : nullptr, a.inv = inv;
+  return by_dtype(dtype, [&](auto dt) { return norm_forward<decltype(dt)::value>(a, (hipStream_t)stream); });
+}
+
+int64_t sdfnn_rms_norm_backward_workspace_size(int64_t rows, int64_t dim) {
+  if (rows < 0 || rows > kMaxRows || dim < 1 || dim > kMaxDim) return -1;
+  return bwd_groups(rows, dim) * dim * 4;
+}
+
+int sdfnn_rms_norm_backward(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, const float* inv,
+                            const void* dy, int64_t lddy, const void* dh, int64_t lddh, int32_t dtype, int64_t rows, int64_t dim, void* dx,
+                            void* dweight, void* workspace, int64_t workspace_bytes, sdfnn_stream_t stream) {
+  NN_TRY(check_norm("rms_norm_backward", x, ldx, residual, ldr, dtype, rows, dim));
+  NN_REQUIRE(weight && inv, "rms_norm_backward: null tensor");
+  NN_REQUIRE(dy || dh, "rms_norm_backward: neither output has a gradient");
+  NN_REQUIRE((!dy || lddy >= dim) && (!dh || lddh >= dim), "rms_norm_backward: a row stride is smaller than the row");
+  NN_REQUIRE(!dweight || (workspace && workspace_bytes >= sdfnn_rms_norm_backward_workspace_size(rows, dim)),
+             "rms_norm_backward: the workspace is too small");
+  if (!dx && !dweight) return 0;
+  NormArgs a{};
+  a.x = x, a.ldx = ldx, a.r = residual, a.ldr = ldr, a.w = weight, a.rows = rows, a.dim = dim;
+  a.dy = dy, a.lddy = lddy, a.dh = dh, a.lddh = lddh, a.dx = dx, a.inv = const_cast<float*>(inv), a.partial = (float*)workspace;
+  return by_dtype(dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    return norm_backward<DT>(a, (elem_t<DT>*)dweight, (hipStream_t)stream);
+  });
+}
+
+int sdfnn_rms_norm_quantize(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int32_t dtype, int64_t rows,
+                            int64_t dim, float eps, int8_t* q, float* scales, void* h, sdfnn_stream_t stream) {
+  NN_TRY(check_norm("rms_norm_quantize", x, ldx, residual, ldr, dtype, rows, dim));
+  NN_REQUIRE(q && scales, "rms_norm_quantize: null tensor");
+  NN_REQUIRE(!weight || (eps >= 0.0f && eps < INFINITY), "rms_norm_quantize: eps %g", (double)eps);
+  if (rows == 0) return 0;
+  NormArgs a{};
+  a.x = x, a.ldx = ldx, a.r = residual, a.ldr = ldr, a.w = weight, a.rows = rows, a.dim = dim, a.eps = eps;
+  a.q = q, a.scales = scales, a.h = residual ? h : nullptr;
+  return by_dtype(dtype, [&](auto dt) { return norm_quantize<decltype(dt)::value>(a, (hipStream_t)stream); });
+}
+
+int64_t sdfnn_int8_linear_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t projections) {
+  if (rows < 0 || rows > kMaxRows || n < 1 || n > kMaxDim || k < 1 || k > 131072 || projections < 1 || projections > 2) return -1;
+  Call c{nullptr, 0, nullptr};
+  const Int8Epi<SDFNN_F32> epi{};
+  if (projections == 1) int8_products<SDFNN_F32, false>(c, nullptr, k, nullptr, k, nullptr, k, rows, n, k, epi);
+  else int8_products<SDFNN_F32, true>(c, nullptr, k, nullptr, k, nullptr, k, rows, n, k, epi);
+  return c.used;
+}
+
+int sdfnn_int8_linear(const int8_t* q, int64_t ldq, const float* sq, const int8_t* w, int64_t ldw, const float* sw, const float* bias,
+                      int32_t dtype, int64_t rows, int64_t n, int64_t k, void* y, void* workspace, int64_t workspace_bytes,
+                      sdfnn_stream_t stream) {
+  NN_TRY(check_int8("int8_linear", q, ldq, w, ldw, w, ldw, dtype, rows, n, k));
+  NN_REQUIRE(sq && sw && y, "int8_linear: null tensor");
+  const int64_t need = sdfnn_int8_linear_workspace_size(rows, n, k, 1);
+  NN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "int8_linear: the workspace is too small (%lld of %lld bytes)",
+             (long long)workspace_bytes, (long long)need);
+  if (rows == 0) return 0;
+  Call c{workspace ? (char*)workspace : (char*)y, 0, (hipStream_t)stream};
+  return by_dtype(dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    const Int8Epi<DT> epi{(elem_t<DT>*)y, sq, sw, nullptr, bias, (int)n, 0};
+    return int8_products<DT, false>(c, q, ldq, w, ldw, w, ldw, rows, n, k, epi);
+  });
+}
+
+int sdfnn_int8_gated_linear(const int8_t* q, int64_t ldq, const float* sq, const int8_t* w_gate, int64_t ldg, const float* s_gate,
+                            const int8_t* w_up, int64_t ldu, const float* s_up, int32_t act, int32_t dtype, int64_t rows, int64_t n,
+                            int64_t k, void* y, void* workspace, int64_t workspace_bytes, sdfnn_stream_t stream) {
+  NN_TRY(check_int8("int8_gated_linear", q, ldq, w_gate, ldg, w_up, ldu, dtype, rows, n, k));
+  NN_REQUIRE(act >= SDFNN_SILU && act <= SDFNN_RELU, "int8_gated_linear: activation %d", act);
+  NN_REQUIRE(sq && s_gate && s_up && y, "int8_gated_linear: null tensor");
+  const int64_t need = sdfnn_int8_linear_workspace_size(rows, n, k, 2);
+  NN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "int8_gated_linear: the workspace is too small (%lld of %lld bytes)",
+             (long long)workspace_bytes, (long long)need);
+  if (rows == 0) return 0;
+  Call c{workspace ? (char*)workspace : (char*)y, 0, (hipStream_t)stream};
+  return by_dtype(dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    const Int8Epi<DT> epi{(elem_t<DT>*)y, sq, s_gate, s_up, nullptr, (int)n, act};
+    return int8_products<DT, true>(c, q, ldq, w_gate, ldg, w_up, ldu, rows, n, k, epi);
+  });
+}
+
+int64_t sdfnn_gated_saved_size(int32_t dtype, int64_t rows, int64_t hidden) {
+  if (dtype < SDFNN_F32 || dtype > SDFNN_F16 || rows < 0 || rows > kMaxRows || hidden < 1 || hidden > 1 << 20) return -1;
+  return 3 * rows * round_up(hidden, 64) * elem_size(dtype);
+}
+
+int64_t sdfnn_gated_workspace_size(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden, int64_t out, int32_t backward) {
+  if (check_gated("gated_workspace_size", dtype, 0, rows, dim, hidden, out)) return -1;
+  Call c{nullptr, 0, nullptr};
+  char some = 0;
+  by_dtype(dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (backward) return gated_backward<DT>(c, nullptr, dim, nullptr, nullptr, nullptr, nullptr, nullptr, out, 0, rows, dim, hidden, out, &some, &some, &some, &some);
+    return gated_forward<DT>(c, nullptr, dim, nullptr, nullptr, nullptr, 0, rows, dim, hidden, out, false, nullptr, nullptr);
+  });
+  return c.used;
+}
+
+int sdfnn_gated_forward(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* w_down, int32_t dtype, int32_t act,
+                        int64_t rows, int64_t dim, int64_t hidden, int64_t out, void* saved, void* y, void* workspace,
+                        int64_t workspace_bytes, sdfnn_stream_t stream) {
+  NN_TRY(check_gated("gated_forward", dtype, act, rows, dim, hidden, out));
+  NN_REQUIRE(x && w_gate && w_up && w_down && y, "gated_forward: null tensor");
+  NN_REQUIRE(ldx >= dim, "gated_forward: a row stride is smaller than the row");
+  const int64_t es = elem_size(dtype);
+  if (rows > kSkinnyRows && es == 2) {
+    NN_REQUIRE(dim % 8 || (aligned16(x, ldx * es) && aligned16(w_gate, 0) && aligned16(w_up, 0)),
+               "gated_forward: with dim a multiple of 8 rows have to start at 16-byte boundaries");
+    NN_REQUIRE(hidden % 8 || aligned16(w_down, 0), "gated_forward: with hidden a multiple of 8 w_down has to start at a 16-byte boundary");
+  }
+  NN_REQUIRE(!saved || aligned16(saved, 0), "gated_forward: saved has to start at a 16-byte boundary");
+  const int64_t need = sdfnn_gated_workspace_size(dtype, rows, dim, hidden, out, 0);
+  NN_REQUIRE(rows == 0 || (workspace && aligned16(workspace, 0) && workspace_bytes >= need),
+             "gated_forward: the workspace is too small or not aligned (%lld of %lld bytes)", (long long)workspace_bytes, (long long)need);
+  if (rows == 0) return 0;
+  Call c{(char*)workspace, 0, (hipStream_t)stream};
+  return by_dtype(dtype, [&](auto dt) {
+    return gated_forward<decltype(dt)::value>(c, x, ldx, w_gate, w_up, w_down, act, rows, dim, hidden, out, saved != nullptr, saved, y);
+  });
+}
+
+int sdfnn_gated_backward(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* w_down, const void* saved,
+                         const void* dy, int64_t lddy, int32_t dtype, int32_t act, int64_t rows, int64_t dim, int64_t hidden, int64_t out,
+                         void* dx, void* dw_gate, void* dw_up, void* dw_down, void* workspace, int64_t workspace_bytes,
+                         sdfnn_stream_t stream) {
+  NN_TRY(check_gated("gated_backward", dtype, act, rows, dim, hidden, out));
+  NN_REQUIRE(x && w_gate && w_up && w_down && dy && saved, "gated_backward: null tensor");
+  NN_REQUIRE(ldx >= dim && lddy >= out, "gated_backward: a row stride is smaller than the row");
+  NN_REQUIRE(!dw_gate == !dw_up, "gated_backward: dw_gate and dw_up are computed together");
+  const int64_t es = elem_size(dtype);
+  NN_REQUIRE(es == 4 || out % 8 || aligned16(dy, lddy * es), "gated_backward: with out a multiple of 8 rows of dy have to start at 16-byte boundaries");
+  NN_REQUIRE(aligned16(saved, 0), "gated_backward: saved has to start at a 16-byte boundary");
+  const int64_t need = sdfnn_gated_workspace_size(dtype, rows, dim, hidden, out, 1);
+  NN_REQUIRE(need == 0 || (workspace && aligned16(workspace, 0) && workspace_bytes >= need),
+             "gated_backward: the workspace is too small or not aligned (%lld of %lld bytes)", (long long)workspace_bytes, (long long)need);
+  Call c{workspace ? (char*)workspace : (char*)saved, 0, (hipStream_t)stream};
+  return by_dtype(dtype, [&](auto dt) {
+    return gated_backward<decltype(dt)::value>(c, x, ldx, w_gate, w_up, w_down, saved, dy, lddy, act, rows, dim, hidden, out, dx, dw_gate,
+                                               dw_up, dw_down);
+  });
+}
+
+}  // extern "C"

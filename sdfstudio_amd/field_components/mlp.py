@@ -1,0 +1,151 @@
+"""Gated feed-forward blocks for a field's features: act(x Wg^T) * (x Wu^T) Wd^T with its gradients, and the pre-norm residual stack of such
+blocks in its training form and its 8-bit serving form.
+
+The reference's MLP (field_components/mlp.py:25-100) is evaluated inside the fused field kernels; these blocks stand beside it as layers of
+their own, at widths up to thousands.  Runs on libsdfnn.so (include/sdfnn.h); no CPU path.
+"""
+from typing import Optional
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from sdfstudio_amd import _nn
+from sdfstudio_amd.field_components.normalization import RMSNorm
+from sdfstudio_amd.field_components.quantization import Int8Linear, int8_gated_linear, quantize_rows
+
+
+class _GatedMLP(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, act):
+        lib, code = _nn.load(), _nn.dtype_code(x, "gated_mlp")
+        dev = _nn.on_device("gated_mlp", x, w_gate, w_up, w_down)
+        hidden, out = w_gate.shape[0], w_down.shape[0]
+        save = any(ctx.needs_input_grad)
+        with torch.cuda.device(dev):
+            x2, ldx = _nn.rows_of(x, align=True)
+            wg, wu, wd = _nn.aligned(w_gate), _nn.aligned(w_up), _nn.aligned(w_down)
+            rows, dim = x2.shape
+            y = torch.empty((*x.shape[:-1], out), dtype=x.dtype, device=dev)
+            saved = _nn.workspace(lib.sdfnn_gated_saved_size(code, rows, hidden), dev) if save else None
+            if rows:
+                size = lib.sdfnn_gated_workspace_size(code, rows, dim, hidden, out, 0)
+                ws = _nn.workspace(size, dev)
+                _nn.check(lib.sdfnn_gated_forward(x2.data_ptr(), ldx, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), code, act, rows, dim, hidden,
+                                                  out, _nn.ptr(saved), y.data_ptr(), ws.data_ptr(), ws.numel(), _nn.stream()),
+                          "sdfnn_gated_forward")
+        if save:
+            ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
+            ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w_gate, w_up, w_down, saved = ctx.saved_tensors
+        lib, code, dev = _nn.load(), _nn.dtype_code(x, "gated_mlp"), x.device
+        hidden, out = w_gate.shape[0], w_down.shape[0]
+        need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
+        with torch.cuda.device(dev):
+            x2, ldx = _nn.rows_of(x, align=True)
+            g2, ldg = _nn.rows_of(dy, align=True)
+            wg, wu, wd = _nn.aligned(w_gate), _nn.aligned(w_up), _nn.aligned(w_down)
+            rows, dim = x2.shape
+            dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+            dwg = torch.empty(hidden, dim, dtype=x.dtype, device=dev) if need_g or need_u else None
+            dwu = torch.empty(hidden, dim, dtype=x.dtype, device=dev) if need_g or need_u else None
+            dwd = torch.empty(out, hidden, dtype=x.dtype, device=dev) if need_d else None
+            if rows == 0:
+                return dx, *(None if t is None else t.zero_() for t in (dwg, dwu, dwd)), None
+            ws = _nn.workspace(lib.sdfnn_gated_workspace_size(code, rows, dim, hidden, out, 1), dev)
+            _nn.check(lib.sdfnn_gated_backward(x2.data_ptr(), ldx, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), saved.data_ptr(), g2.data_ptr(),
+                                               ldg, code, ctx.act, rows, dim, hidden, out, _nn.ptr(dx), _nn.ptr(dwg), _nn.ptr(dwu),
+                                               _nn.ptr(dwd), ws.data_ptr(), ws.numel(), _nn.stream()), "sdfnn_gated_backward")
+        return dx, dwg if need_g else None, dwu if need_u else None, dwd, None
+
+
+def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """(activation(x w_gate^T) * (x w_up^T)) w_down^T: x [..., dim], w_gate / w_up [hidden, dim], w_down [out, hidden], all float32, bfloat16
+    or float16; activation "silu", "gelu" (with the error function) or "relu".  Gradients for all four (not differentiable twice); under
+    torch.no_grad() nothing is kept for them.  float32 runs at float32 accuracy."""
+    what = "gated_mlp"
+    act = _nn.activation_code(activation, what)
+    if x.dim() < 1 or w_gate.dim() != 2 or w_down.dim() != 2 or w_gate.shape != w_up.shape:
+        raise ValueError(f"{what}: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}, w_down {tuple(w_down.shape)}")
+    if w_gate.shape[1] != x.shape[-1] or w_down.shape[1] != w_gate.shape[0] or 0 in w_gate.shape or 0 in w_down.shape:
+        raise ValueError(f"{what}: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_down {tuple(w_down.shape)} do not chain")
+    if not (x.dtype == w_gate.dtype == w_up.dtype == w_down.dtype):
+        raise TypeError(f"{what}: x {x.dtype}, weights {w_gate.dtype}, {w_up.dtype}, {w_down.dtype}: one type")
+    return _GatedMLP.apply(x, w_gate, w_up, w_down, act)
+
+
+class GatedMLP(nn.Module):
+    """gated_mlp with its weights, initialised as nn.Linear's (uniform within 1 / sqrt(fan-in)); no biases."""
+
+    def __init__(self, in_dim: int, hidden_dim: int, out_dim: Optional[int] = None, activation: str = "silu") -> None:
+        super().__init__()
+        _nn.activation_code(activation, "GatedMLP")
+        self.activation = activation
+        out_dim = in_dim if out_dim is None else out_dim
+
+        def weight(o, i):
+            return nn.Parameter(torch.empty(o, i).uniform_(-(i ** -0.5), i ** -0.5))
+
+        self.w_gate, self.w_up, self.w_down = weight(hidden_dim, in_dim), weight(hidden_dim, in_dim), weight(out_dim, hidden_dim)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return gated_mlp(x, self.w_gate, self.w_up, self.w_down, self.activation)
+
+
+class Int8GatedMLP(nn.Module):
+    """A trained GatedMLP in 8 bits: weights quantised once by channel; takes and multiplies codes, quantises its hidden row in between."""
+
+    def __init__(self, mlp: GatedMLP) -> None:
+        super().__init__()
+        self.activation = mlp.activation
+        self.gate, self.up, self.down = Int8Linear(mlp.w_gate), Int8Linear(mlp.w_up), Int8Linear(mlp.w_down)
+
+    def forward(self, q: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        hidden = int8_gated_linear(q, scales, self.gate.weight_q, self.gate.weight_scales, self.up.weight_q, self.up.weight_scales,
+                                   self.activation, out_dtype)
+        return self.down(*quantize_rows(hidden), out_dtype)
+
+
+class GatedStack(nn.Module):
+    """num_blocks pre-norm residual blocks  h <- h + mlp(norm(h))  and a last norm.  Every addition happens inside the norm that follows it.
+
+    quantize() makes the 8-bit serving form: from then on a call that needs no gradient (torch.no_grad()) runs the blocks on 8-bit products,
+    with weights quantised from the parameters as they were; training calls are unaffected.  dequantize() drops it."""
+
+    def __init__(self, dim: int, hidden_dim: int, num_blocks: int, activation: str = "silu", eps: float = 1e-6) -> None:
+        super().__init__()
+        if num_blocks < 1:
+            raise ValueError(f"GatedStack: {num_blocks} blocks")
+        self.norms = nn.ModuleList(RMSNorm(dim, eps) for _ in range(num_blocks + 1))
+        self.mlps = nn.ModuleList(GatedMLP(dim, hidden_dim, dim, activation) for _ in range(num_blocks))
+        self._served = None  # not a submodule: state_dict holds the parameters alone
+
+    def quantize(self) -> "GatedStack":
+        self._served = [Int8GatedMLP(m) for m in self.mlps]
+        return self
+
+    def dequantize(self) -> "GatedStack":
+        self._served = None
+        return self
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        h, delta = x, None
+        serve = self._served is not None and not torch.is_grad_enabled()
+        for i, norm in enumerate(self.norms[:-1]):
+            if serve:
+                out = norm.quantized(h, delta)
+                if delta is not None:
+                    h = out[2]
+                delta = self._served[i](out[0], out[1], h.dtype)
+            else:
+                out = norm(h, delta)
+                y = out
+                if delta is not None:
+                    y, h = out
+                delta = self.mlps[i](y)
+        return self.norms[-1](h, delta)[0]

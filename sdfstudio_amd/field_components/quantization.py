@@ -1,0 +1,108 @@
+"""8-bit serving form of a field's linear layers: rows quantised symmetrically (one scale a token / point, one a channel of the weights),
+products on the integer matrix cores with exact 32-bit sums.  Runs on libsdfnn.so (include/sdfnn.h); no CPU path, no gradients.
+"""
+from typing import Optional, Tuple
+
+import torch
+from torch import nn
+
+from sdfstudio_amd import _nn
+from sdfstudio_amd.field_components.normalization import _check, _quantize
+
+MAX_K = 131072  # 127 * 127 * k stays below 2^31
+
+
+@torch.no_grad()
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x [..., dim] -> (codes int8 [..., dim] in [-127, 127], scales float32 [...]): code = round(127 x / max|x|) half to even, scale =
+    max|x| / 127 of its row (a row of zeros: scale 0).  Serves activations (a scale a token) and weights [out, in] (a scale a channel)."""
+    _check("quantize_rows", x, None, None)
+    return _quantize("quantize_rows", x, None, None, 0.0)
+
+
+def _check_operand(what: str, name: str, q: torch.Tensor, scales: torch.Tensor, k: Optional[int] = None) -> None:
+    if q.dtype != torch.int8 or q.dim() < 1:
+        raise TypeError(f"{what}: {name} {tuple(q.shape)} {q.dtype}: int8 rows expected")
+    if k is not None and (q.dim() != 2 or q.shape[1] != k):
+        raise ValueError(f"{what}: {name} {tuple(q.shape)} does not fit k = {k}")
+    if scales.dtype != torch.float32 or scales.shape != q.shape[:-1]:
+        raise ValueError(f"{what}: scales {tuple(scales.shape)} {scales.dtype} of {name} {tuple(q.shape)}: one float32 a row")
+
+
+def _prepare(what, q, scales, weights, out_dtype):
+    _check_operand(what, "q", q, scales)
+    k = q.shape[-1]
+    for name, (w, s) in weights.items():
+        _check_operand(what, name, w, s, k)
+    if not 1 <= k <= MAX_K:
+        raise ValueError(f"{what}: k = {k}: the 32-bit sum is exact for 1 .. {MAX_K}")
+    if out_dtype not in _nn.DTYPES:
+        raise TypeError(f"{what}: out_dtype {out_dtype} (float32, bfloat16, float16)")
+
+
+@torch.no_grad()
+def int8_linear(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, weight_scales: torch.Tensor,
+                bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """y[..., n] = (sum_k q[..., k] weight_q[n, k]) scales[...] weight_scales[n] + bias[n] in out_dtype.  q int8 [..., k] with scales
+    float32 [...], weight_q int8 [n, k] with weight_scales float32 [n], bias float32 [n]."""
+    what = "int8_linear"
+    _prepare(what, q, scales, {"weight_q": (weight_q, weight_scales)}, out_dtype)
+    n = weight_q.shape[0]
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (n,)):
+        raise ValueError(f"{what}: bias {tuple(bias.shape)} {bias.dtype} for {n} channels: float32")
+    lib, dev = _nn.load(), _nn.on_device(what, q, scales, weight_q, weight_scales, bias)
+    with torch.cuda.device(dev):
+        q2, ldq = _nn.rows_of(q, align=True)
+        w2, ldw = _nn.rows_of(weight_q, align=True)
+        sq, sw = scales.contiguous(), weight_scales.contiguous()
+        b = bias.contiguous() if bias is not None else None
+        rows, k = q2.shape
+        y = torch.empty((*q.shape[:-1], n), dtype=out_dtype, device=dev)
+        if rows and n:
+            size = lib.sdfnn_int8_linear_workspace_size(rows, n, k, 1)
+            ws = _nn.workspace(size, dev) if size else None
+            _nn.check(lib.sdfnn_int8_linear(q2.data_ptr(), ldq, sq.data_ptr(), w2.data_ptr(), ldw, sw.data_ptr(), _nn.ptr(b),
+                                            _nn.DTYPES[out_dtype], rows, n, k, y.data_ptr(), _nn.ptr(ws), size, _nn.stream()),
+                      "sdfnn_int8_linear")
+    return y
+
+
+@torch.no_grad()
+def int8_gated_linear(q: torch.Tensor, scales: torch.Tensor, gate_q: torch.Tensor, gate_scales: torch.Tensor, up_q: torch.Tensor,
+                      up_scales: torch.Tensor, activation: str = "silu", out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """activation(gate) * up of two int8_linear products of the same rows, in one kernel: neither product is written out."""
+    what = "int8_gated_linear"
+    _prepare(what, q, scales, {"gate_q": (gate_q, gate_scales), "up_q": (up_q, up_scales)}, out_dtype)
+    if gate_q.shape != up_q.shape:
+        raise ValueError(f"{what}: gate_q {tuple(gate_q.shape)} and up_q {tuple(up_q.shape)}")
+    act = _nn.activation_code(activation, what)
+    n = gate_q.shape[0]
+    lib, dev = _nn.load(), _nn.on_device(what, q, scales, gate_q, gate_scales, up_q, up_scales)
+    with torch.cuda.device(dev):
+        q2, ldq = _nn.rows_of(q, align=True)
+        g2, ldg = _nn.rows_of(gate_q, align=True)
+        u2, ldu = _nn.rows_of(up_q, align=True)
+        sq, sg, su = scales.contiguous(), gate_scales.contiguous(), up_scales.contiguous()
+        rows, k = q2.shape
+        y = torch.empty((*q.shape[:-1], n), dtype=out_dtype, device=dev)
+        if rows and n:
+            size = lib.sdfnn_int8_linear_workspace_size(rows, n, k, 2)
+            ws = _nn.workspace(size, dev) if size else None
+            _nn.check(lib.sdfnn_int8_gated_linear(q2.data_ptr(), ldq, sq.data_ptr(), g2.data_ptr(), ldg, sg.data_ptr(), u2.data_ptr(), ldu,
+                                                  su.data_ptr(), act, _nn.DTYPES[out_dtype], rows, n, k, y.data_ptr(), _nn.ptr(ws), size,
+                                                  _nn.stream()), "sdfnn_int8_gated_linear")
+    return y
+
+
+class Int8Linear(nn.Module):
+    """A trained linear layer in 8 bits: its weight quantised once, by channel; takes the codes and scales of its input."""
+
+    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> None:
+        super().__init__()
+        codes, scales = quantize_rows(weight.detach())
+        self.register_buffer("weight_q", codes)
+        self.register_buffer("weight_scales", scales)
+        self.register_buffer("bias", bias.detach().float().clone() if bias is not None else None)
+
+    def forward(self, q: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        return int8_linear(q, scales, self.weight_q, self.weight_scales, self.bias, out_dtype)
