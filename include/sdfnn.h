@@ -66,7 +66,7 @@ int sdfnn_int8_gated_linear(const int8_t* q, int64_t ldq, const float* sq, const
  * g = x Wg^T, u = x Wu^T, a = act(g) u, y = a Wd^T.  x [rows, dim] (stride ldx), w_gate / w_up [hidden, dim], w_down [out, hidden], all
  * contiguous, y [rows, out] contiguous.  16-bit types: products of those types with fp32 sums; a is rounded to the type before the second
  * product.  fp32: every operand as three bf16 parts that hold its 24 bits, six products, fp32 sums (a non-finite input gives NaN).
- * saved: sdfnn_gated_saved_size bytes, what the backward needs (g, u and a, g and u rounded to the type); NULL when none will follow. */
+ * saved: sdfnn_gated_saved_size bytes, what the backward needs (act(g) and u act'(g) in fp32, a in the type); NULL when none will follow. */
 int64_t sdfnn_gated_saved_size(int32_t dtype, int64_t rows, int64_t hidden);
 int64_t sdfnn_gated_workspace_size(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden, int64_t out, int32_t backward);
 int sdfnn_gated_forward(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* w_down, int32_t dtype, int32_t act,
@@ -75,9 +75,8 @@ int sdfnn_gated_forward(const void* x, int64_t ldx, const void* w_gate, const vo
 /* dy [rows, out] (stride lddy).  dx [rows, dim], dw_gate, dw_up [hidden, dim], dw_down [out, hidden] are overwritten; each may be NULL
  * (dw_gate and dw_up together). */
 int sdfnn_gated_backward(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* w_down, const void* saved,
-                         const void* dy, int64_t lddy, int32_t dtype, int32_t act, int64_t rows, int64_t dim, int64_t hidden, int64_t out,
-                         void* dx, void* dw_gate, void* dw_up, void* dw_down, void* workspace, int64_t workspace_bytes,
-                         sdfnn_stream_t stream);
+                         const void* dy, int64_t lddy, int32_t dtype, int64_t rows, int64_t dim, int64_t hidden, int64_t out, void* dx,
+                         void* dw_gate, void* dw_up, void* dw_down, void* workspace, int64_t workspace_bytes, sdfnn_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -25,7 +25,7 @@ _SIGNATURES = {
     "sdfnn_gated_saved_size": (_i64, [_i32, _i64, _i64]),
     "sdfnn_gated_workspace_size": (_i64, [_i32, _i64, _i64, _i64, _i64, _i32]),
     "sdfnn_gated_forward": (ctypes.c_int, [_p, _i64, _p, _p, _p, _i32, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p]),
-    "sdfnn_gated_backward": (ctypes.c_int, [_p, _i64, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p]),
+    "sdfnn_gated_backward": (ctypes.c_int, [_p, _i64, _p, _p, _p, _p, _p, _i64, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p]),
 }
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}

@@ -165,10 +165,11 @@ int gated_forward(Call& c, const void* x, const int64_t ldx, const void* wg, con
   typedef elem_t<DT> T;
   typedef Kind<DT> K;
   const int64_t Fp = round_up(F, 64), es = K::es;
-  T *gs = nullptr, *us = nullptr, *a;
-  if (save) gs = (T*)saved, us = gs + M * Fp, a = us + M * Fp;
+  float *fu = nullptr, *fg = nullptr;
+  T* a;
+  if (save) fu = (float*)saved, fg = fu + M * Fp, a = (T*)(fg + M * Fp);
   else a = (T*)c.take(M * Fp * es);
-  const GatedEpi<DT> ge{a, gs, us, (int)Fp, act};
+  const GatedEpi<DT> ge{a, fu, fg, (int)Fp, act};
   const StoreEpi<DT> se{(T*)y, nullptr, M, M, 0, O, (int)O};
   if (M <= kSkinnyRows) {
     const Operand xo{(const char*)x, ldx * es, 0}, g{(const char*)wg, D * es, 0}, u{(const char*)wu, D * es, 0};
@@ -189,13 +190,14 @@ int gated_forward(Call& c, const void* x, const int64_t ldx, const void* wg, con
 
 template <int DT>
 int gated_backward(Call& c, const void* x, const int64_t ldx, const void* wg, const void* wu, const void* wd, const void* saved, const void* dy,
-                   const int64_t lddy, const int act, const int64_t M, const int64_t D, const int64_t F, const int64_t O, void* dx, void* dwg,
+                   const int64_t lddy, const int64_t M, const int64_t D, const int64_t F, const int64_t O, void* dx, void* dwg,
                    void* dwu, void* dwd) {
   typedef elem_t<DT> T;
   typedef Kind<DT> K;
   constexpr bool F32 = K::f32;
   const int64_t Fp = round_up(F, 64), Op = round_up(O, 64), Mp = round_up(M, 64);
-  const T *gs = (const T*)saved, *us = gs + M * Fp, *a = us + M * Fp;
+  const float *fu = (const float*)saved, *fg = fu + M * Fp;
+  const T* a = (const T*)(fg + M * Fp);
   T* dgu = (T*)c.take(M * 2 * Fp * K::es);
   const bool o8 = O % 8 == 0;
   const int64_t start = c.used;  // the operands of one product make room for those of the next
@@ -205,7 +207,7 @@ int gated_backward(Call& c, const void* x, const int64_t ldx, const void* wg, co
     Operand dyo, wdt = take_operand<F32>(c, F, Op);
     NN_TRY(row_operand<DT>(c, dy, lddy, M, O, o8, dyo));
     NN_TRY(pack_transposed<F32>(c, wd, F, O, F, Op, 0, wdt));
-    const GatedBwdEpi<DT> be{gs, us, dgu, (int)Fp, act};
+    const GatedBwdEpi<DT> be{fu, fg, dgu, (int)Fp};
     NN_TRY((product<K::tile, K::terms, false>(c, dyo, wdt, wdt, M, F, (o8 && !F32 ? O : Op) * 2, be)));
     next();
   }
@@ -349,7 +351,7 @@ int sdfnn_int8_gated_linear(const int8_t* q, int64_t ldq, const float* sq, const
 
 int64_t sdfnn_gated_saved_size(int32_t dtype, int64_t rows, int64_t hidden) {
   if (dtype < SDFNN_F32 || dtype > SDFNN_F16 || rows < 0 || rows > kMaxRows || hidden < 1 || hidden > 1 << 20) return -1;
-  return 3 * rows * round_up(hidden, 64) * elem_size(dtype);
+  return rows * round_up(hidden, 64) * (8 + elem_size(dtype));
 }
 
 int64_t sdfnn_gated_workspace_size(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden, int64_t out, int32_t backward) {
@@ -358,7 +360,7 @@ int64_t sdfnn_gated_workspace_size(int32_t dtype, int64_t rows, int64_t dim, int
   char some = 0;
   by_dtype(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (backward) return gated_backward<DT>(c, nullptr, dim, nullptr, nullptr, nullptr, nullptr, nullptr, out, 0, rows, dim, hidden, out, &some, &some, &some, &some);
+    if (backward) return gated_backward<DT>(c, nullptr, dim, nullptr, nullptr, nullptr, nullptr, nullptr, out, rows, dim, hidden, out, &some, &some, &some, &some);
     return gated_forward<DT>(c, nullptr, dim, nullptr, nullptr, nullptr, 0, rows, dim, hidden, out, false, nullptr, nullptr);
   });
   return c.used;
@@ -388,10 +390,10 @@ int sdfnn_gated_forward(const void* x, int64_t ldx, const void* w_gate, const vo
 }
 
 int sdfnn_gated_backward(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* w_down, const void* saved,
-                         const void* dy, int64_t lddy, int32_t dtype, int32_t act, int64_t rows, int64_t dim, int64_t hidden, int64_t out,
+                         const void* dy, int64_t lddy, int32_t dtype, int64_t rows, int64_t dim, int64_t hidden, int64_t out,
                          void* dx, void* dw_gate, void* dw_up, void* dw_down, void* workspace, int64_t workspace_bytes,
                          sdfnn_stream_t stream) {
-  NN_TRY(check_gated("gated_backward", dtype, act, rows, dim, hidden, out));
+  NN_TRY(check_gated("gated_backward", dtype, 0, rows, dim, hidden, out));
   NN_REQUIRE(x && w_gate && w_up && w_down && dy && saved, "gated_backward: null tensor");
   NN_REQUIRE(ldx >= dim && lddy >= out, "gated_backward: a row stride is smaller than the row");
   NN_REQUIRE(!dw_gate == !dw_up, "gated_backward: dw_gate and dw_up are computed together");
@@ -403,7 +405,7 @@ int sdfnn_gated_backward(const void* x, int64_t ldx, const void* w_gate, const v
              "gated_backward: the workspace is too small or not aligned (%lld of %lld bytes)", (long long)workspace_bytes, (long long)need);
   Call c{workspace ? (char*)workspace : (char*)saved, 0, (hipStream_t)stream};
   return by_dtype(dtype, [&](auto dt) {
-    return gated_backward<decltype(dt)::value>(c, x, ldx, w_gate, w_up, w_down, saved, dy, lddy, act, rows, dim, hidden, out, dx, dw_gate,
+    return gated_backward<decltype(dt)::value>(c, x, ldx, w_gate, w_up, w_down, saved, dy, lddy, rows, dim, hidden, out, dx, dw_gate,
                                                dw_up, dw_down);
   });
 }

@@ -66,16 +66,42 @@ NN_D void store8_n(elem_t<DT>* p, const int n, const float (&v)[8]) {
 }
 
 // ---- activations of the gated block and their derivatives.  FAST (16-bit results): the hardware's exponential and reciprocal, one ulp of
-// fp32 each; fp32 results use the library's expf / erff.
+// fp32 each, the exponent rounded to fp32 before it.  fp32 results: the part of x log2(e) that this rounding loses goes back in to first
+// order, and one Newton step follows the reciprocal.  |x| is cut at 87, where the exponential leaves the normal numbers.
 template <bool FAST>
-NN_D float nn_exp(const float x) {
+NN_D float nn_exp(float x) {
   if constexpr (FAST) return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
-  else return expf(x);
+  x = __builtin_amdgcn_fmed3f(x, -87.0f, 87.0f);
+  const float t = x * 1.44269504088896340736f;
+  const float lost = fmaf(x, 1.44269504088896340736f, -t) + x * 1.92596299112661746887e-8f;
+  const float e = __builtin_amdgcn_exp2f(t);
+  return fmaf(e, lost * 0.69314718055994530942f, e);
 }
 template <bool FAST>
-NN_D float nn_recip(const float x) {
-  if constexpr (FAST) return __builtin_amdgcn_rcpf(x);
-  else return 1.0f / x;
+NN_D float nn_recip(const float x) {  // 1 <= x < 2^127
+  const float r = __builtin_amdgcn_rcpf(x);
+  if constexpr (FAST) return r;
+  return fmaf(fmaf(-x, r, 1.0f), r, r);
+}
+// Phi(z), the normal distribution function, and e = exp(-z^2 / 2): for x = |z| / sqrt(2)
+//   erfc(x) = exp(-x^2) t P(t),  t = 1 / (1 + 0.4 x),
+// P of degree 8 fitted to erfc(x) exp(x^2) / t over x >= 0 for the smallest relative error (1.3e-7): one exponential serves the value, its
+// tail to full relative accuracy, and the density in the derivative.
+template <bool FAST>
+NN_D float nn_phi(const float z, float& e) {
+  e = nn_exp<FAST>(-0.5f * z * z);
+  const float t = nn_recip<FAST>(fmaf(0.28284271247461900976f, fabsf(z), 1.0f));
+  float p = 0.0502621084f;
+  p = fmaf(p, t, -0.182901412f);
+  p = fmaf(p, t, 0.169085339f);
+  p = fmaf(p, t, -0.00560746621f);
+  p = fmaf(p, t, 0.141431406f);
+  p = fmaf(p, t, 0.168541983f);
+  p = fmaf(p, t, 0.207842693f);
+  p = fmaf(p, t, 0.225669593f);
+  p = fmaf(p, t, 0.225675866f);
+  const float c = 0.5f * e * t * p;
+  return z < 0.0f ? c : 1.0f - c;
 }
 // a = act(z), d = act'(z)
 template <bool FAST>
@@ -85,9 +111,10 @@ NN_D void act_both(const int act, const float z, float& a, float& d) {
     a = z * s;
     d = s * (1.0f + z * (1.0f - s));
   } else if (act == SDFNN_GELU) {
-    const float phi = 0.5f * erfcf(-0.70710678118654752440f * z);
+    float e;
+    const float phi = nn_phi<FAST>(z, e);
     a = z * phi;
-    d = phi + z * 0.39894228040143267794f * nn_exp<FAST>(-0.5f * z * z);
+    d = fmaf(z * 0.39894228040143267794f, e, phi);
   } else {
     a = z < 0.0f ? 0.0f : z;  // (a NaN stays one)
     d = z > 0.0f ? 1.0f : 0.0f;
@@ -95,9 +122,9 @@ NN_D void act_both(const int act, const float z, float& a, float& d) {
 }
 template <bool FAST>
 NN_D float act_only(const int act, const float z) {
-  if (act == SDFNN_SILU) return z * nn_recip<FAST>(1.0f + nn_exp<FAST>(-z));
-  if (act == SDFNN_GELU) return z * (0.5f * erfcf(-0.70710678118654752440f * z));
-  return z < 0.0f ? 0.0f : z;
+  float a, d;
+  act_both<FAST>(act, z, a, d);  // (what the derivative alone needs is dropped by the compiler)
+  return a;
 }
 
 // ---- host side

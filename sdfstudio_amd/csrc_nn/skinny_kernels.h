@@ -133,8 +133,9 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void skinny_kernel(const GemmArg
         v[p][e] = n0 + half * 8 + e < g.N ? s : (typename S::el)0;  // the padding columns of a workspace are zeros
       }
     if (m < g.M) {
-      if constexpr (DUAL) g.epi.pair(0, m, n0 + half * 8, v[0], v[1]);
-      else g.epi.one(0, m, n0 + half * 8, v[0]);
+      const int c = n0 + half * 8;
+      if constexpr (DUAL) g.epi.pair(0, m, c, v[0], v[1], g.epi.cols(c), g.epi.fetch(m, g.M, c));
+      else g.epi.one(0, m, c, v[0], g.epi.cols(c), g.epi.fetch(m, g.M, c));
     }
   }
 }

@@ -36,7 +36,6 @@ class _GatedMLP(torch.autograd.Function):
                           "sdfnn_gated_forward")
         if save:
             ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
-            ctx.act = act
         return y
 
     @staticmethod
@@ -59,7 +58,7 @@ class _GatedMLP(torch.autograd.Function):
                 return dx, *(None if t is None else t.zero_() for t in (dwg, dwu, dwd)), None
             ws = _nn.workspace(lib.sdfnn_gated_workspace_size(code, rows, dim, hidden, out, 1), dev)
             _nn.check(lib.sdfnn_gated_backward(x2.data_ptr(), ldx, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), saved.data_ptr(), g2.data_ptr(),
-                                               ldg, code, ctx.act, rows, dim, hidden, out, _nn.ptr(dx), _nn.ptr(dwg), _nn.ptr(dwu),
+                                               ldg, code, rows, dim, hidden, out, _nn.ptr(dx), _nn.ptr(dwg), _nn.ptr(dwu),
                                                _nn.ptr(dwd), ws.data_ptr(), ws.numel(), _nn.stream()), "sdfnn_gated_backward")
         return dx, dwg if need_g else None, dwu if need_u else None, dwd, None
 
