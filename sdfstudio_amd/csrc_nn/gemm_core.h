@@ -3,12 +3,10 @@
 // One kernel serves 16-bit floats (v_mfma_f32_32x32x16), 8-bit integers (v_mfma_i32_32x32x32) and fp32 as three bf16 parts a value: to it a
 // row is a string of bytes, a step is 128 of them (64 16-bit or 128 8-bit elements of k), and an operand fragment is 16 bytes a lane
 // whatever they hold.
-//   * Tiles go from HBM / L2 to LDS without passing registers (buffer_load_dwordx4 ... lds), double buffered: one barrier a step; the loads
-//     of step s + 1 are issued when step s begins.  A row past the end of a matrix, and the bytes past k in the last step, lie outside the
-//     buffer's range, where the load returns zeros: ragged sizes cost no branch in the loop.
-//   * LDS rows are 128 bytes = half of the banks, so a fragment read (32 rows at one k) would hit the same 16 bytes of every row: the
-//     16-byte pieces of row r are stored in the order piece ^ (r & 7) instead (the permutation is applied to the GLOBAL address of the
-//     load, LDS itself is written in order), which spreads the reads over all banks.
+//   * Tiles go from HBM / L2 to LDS without passing registers (buffer_load_dwordx4 ... lds).  A row past the end of a matrix, and the bytes past
+//     k in the last step, lie outside the buffer's range, where the load returns zeros: ragged sizes cost no branch in the loop.
+//   * A fragment read takes one 16-byte piece of each of 32 rows: stored in order they would lie in the same few banks.  The pieces of a row are
+//     permuted instead (the permutation is applied to the GLOBAL address of the load, LDS itself is written in order).
 //   * The weights' rows (n) are operand A of the instruction and the tokens' rows (m) operand B: a lane then owns ONE m and runs of 4
 //     consecutive n, which the epilogue stages through LDS in 16-byte pieces.
 //   * fp32: x = p0 + p1 + p2 with p0 = bf16(x), p1 = bf16(x - p0), p2 = bf16(x - p0 - p1) holds all 24 bits; of the nine products of two
@@ -137,11 +135,13 @@ NN_D void put_tile(const ACC (&acc)[MI][NJ], const EPI& epi, const int split, co
 }
 
 // ---- 256 x 256: four wavefronts (one a SIMD) of 128 x 128.  A fragment is used for four instructions, so the operand reads take half of
-// LDS's bandwidth, and the 256 accumulators leave registers for a second set of fragments: the reads of one half step run under the
-// instructions of the other.  Steps of 64 bytes of k in a ring of four LDS buffers: a buffer is refilled as soon as the last wavefront has
-// taken its second half into registers, three steps (~1.3 us) before it is needed.  Rows of 64 bytes: the piece of row r lies at
-// piece ^ ((r >> 1) & 3), so that eight consecutive rows cover all banks.
-constexpr int kRing = 4, kStageBytes = 512 * 64;
+// LDS's bandwidth, and the 256 accumulators leave registers for a second set of fragments: the reads of one quarter step run under the 16
+// instructions of another.  A step is 128 bytes of k - whole lines, the request that L2 serves at full rate - and one operand's 256 rows of it
+// (32 KiB) are the unit of a ring of five, all of LDS: A0 B0 A1 B1 A2.  Both units of a step are free once the last wavefront has taken its
+// fourth quarter into registers; B of the step after next goes into the first of them at once and A of the one behind it into the second.
+// Loads are spread between the instructions, since a load that finds the address unit busy holds back what follows it.
+// The piece of row r lies at piece ^ ((r >> 1) & 7): the 16 rows of one pass over the banks lie in 16 different places.
+constexpr int kUnit = 256 * 128, kRing = 5;
 template <int KIND, int TERMS, bool DUAL, class EPI>
 __global__ __launch_bounds__(256, 1) void gemm256_kernel(const GemmArgs<EPI> g) {
   typedef Mfma<KIND> MM;
@@ -150,35 +150,34 @@ __global__ __launch_bounds__(256, 1) void gemm256_kernel(const GemmArgs<EPI> g) 
   const int wm = wave >> 1, wn = wave & 1;
   const TileId id = tile_of<256, DUAL ? 128 : 256>(g);
 
-  const int lr = lane >> 2, piece = (lane & 3) ^ ((lane >> 3) & 3);
-  const bool up_wave = DUAL && (wave & 2);  // a load moves 16 rows; blocks of 32 rows alternate between the projections
-  const Operand& ob = up_wave ? g.b[1] : g.b[0];
-  unsigned off_a[4], off_b[4];
+  const int lr = lane >> 3, piece = (lane & 7) ^ ((wave & 1) * 4 + (lr >> 1));
+  unsigned off_a[8], off_b[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int grp = i * 4 + wave;
-    off_a[i] = (unsigned)((grp * 16 + lr) * g.a.ld) + piece * 16;
-    off_b[i] = (unsigned)((DUAL ? (grp >> 2) * 32 + (grp & 1) * 16 + lr : grp * 16 + lr) * ob.ld) + piece * 16;
+  for (int i = 0; i < 8; ++i) {  // a load moves 8 rows; DUAL: load i brings rows of projection i & 1 (blocks of 32 rows alternate)
+    off_a[i] = (unsigned)(((i * 4 + wave) * 8 + lr) * g.a.ld) + piece * 16;
+    off_b[i] = (unsigned)((DUAL ? (i >> 1) * 32 + wave * 8 + lr : (i * 4 + wave) * 8 + lr) * g.b[DUAL ? i & 1 : 0].ld) + piece * 16;
   }
   const int steps = g.nk * TERMS;
   const int s0 = id.split * g.per, s1 = s0 + g.per < steps ? s0 + g.per : steps;
-  const __amdgpu_buffer_rsrc_t rs_a = rows_buffer(g.a.p, id.m0, g.M, g.a.ld, g.kb), rs_b = rows_buffer(ob.p, id.n0, g.N, ob.ld, g.kb);
+  const __amdgpu_buffer_rsrc_t rs_a = rows_buffer(g.a.p, id.m0, g.M, g.a.ld, g.kb), rs_b0 = rows_buffer(g.b[0].p, id.n0, g.N, g.b[0].ld, g.kb),
+                               rs_b1 = rows_buffer(g.b[DUAL].p, id.n0, g.N, g.b[DUAL].ld, g.kb);
 
-  // loads of step s; behind the last step they lie out of range and write zeros, so that the count of loads in flight stays the same
-  auto issue = [&](const int s) __attribute__((always_inline)) {
+  // load i of step s of one operand into the unit at `unit`; behind the last step they lie out of range and write zeros, so that the count of
+  // loads in flight stays the same
+  auto issue = [&](const int s, auto second, const int i, const int unit) __attribute__((always_inline)) {
+    constexpr bool B = decltype(second)::value;
     const int kc = TERMS == 1 ? s : s / TERMS, t = TERMS == 1 ? 0 : s - kc * TERMS;
-    const int k = kc * 64;
+    const int k = kc * 128;
     const unsigned beyond = (unsigned)(s >= s1) << 31 | (unsigned)(k + piece * 16 >= g.kb) << 31;  // (buffers end below 2^31)
-    char* base = lds + ((s - s0) & (kRing - 1)) * kStageBytes + wave * 1024;
-    const __amdgpu_buffer_rsrc_t ra = TERMS == 1 ? rs_a : rows_buffer(g.a.p + part_a(t) * g.a.plane, id.m0, g.M, g.a.ld, g.kb);
-    const __amdgpu_buffer_rsrc_t rb = TERMS == 1 ? rs_b : rows_buffer(ob.p + part_b(t) * ob.plane, id.n0, g.N, ob.ld, g.kb);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(base + i * 4096), 16, (off_a[i] + k) | beyond, 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void*)(base + 16384 + i * 4096), 16, (off_b[i] + k) | beyond, 0, 0, 0);
+    __amdgpu_buffer_rsrc_t rs;
+    if constexpr (TERMS == 1) rs = B ? DUAL && (i & 1) ? rs_b1 : rs_b0 : rs_a;
+    else if constexpr (B) rs = rows_buffer(g.b[DUAL ? i & 1 : 0].p + part_b(t) * g.b[0].plane, id.n0, g.N, g.b[DUAL ? i & 1 : 0].ld, g.kb);
+    else rs = rows_buffer(g.a.p + part_a(t) * g.a.plane, id.m0, g.M, g.a.ld, g.kb);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(lds + unit + wave * 1024 + i * 4096), 16,
+                                             ((B ? off_b[i] : off_a[i]) + k) | beyond, 0, 0, 0);
   };
+  const std::integral_constant<bool, false> A{};
+  const std::integral_constant<bool, true> B{};
 
   typename MM::acc acc[4][4];
 #pragma unroll
@@ -188,52 +187,60 @@ __global__ __launch_bounds__(256, 1) void gemm256_kernel(const GemmArgs<EPI> g) 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
-  const int row = lane & 31, c0 = ((lane >> 5) ^ ((row >> 1) & 3)) * 16;
-  const int fa = (wm * 128 + row) * 64 + c0, fb = 16384 + (wn * 128 + row) * 64 + c0;  // half step 1: ^ 32
+  const int row = lane & 31, c0 = ((lane >> 5) ^ ((row >> 1) & 7)) * 16;
+  const int fa = (wm * 128 + row) * 128 + c0, fb = (wn * 128 + row) * 128 + c0;  // quarter q: ^ 32 q
   i32x4 a0[4], b0[4], a1[4], b1[4];
-  auto read = [&](const int s, const int half, i32x4 (&a)[4], i32x4 (&b)[4]) __attribute__((always_inline)) {
-    const char* base = lds + ((s - s0) & (kRing - 1)) * kStageBytes;
-    const char *pa = base + (fa ^ (half * 32)), *pb = base + (fb ^ (half * 32));
+  // a quarter step: the 16 instructions of the fragments (a, b); between them the reads of the next quarter's fragments (na, nb) from the
+  // units ua, ub and NL loads
+  auto quarter = [&](const i32x4 (&a)[4], const i32x4 (&b)[4], const int nq, const int ua, const int ub, i32x4 (&na)[4], i32x4 (&nb)[4],
+                     auto nl, auto operand, const int ls, const int lf, const int unit) __attribute__((always_inline)) {
+    constexpr int NL = decltype(nl)::value;
+    const char *pa = lds + ua + (fa ^ (nq * 32)), *pb = lds + ub + (fb ^ (nq * 32));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = *(const i32x4*)(pa + i * 2048);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = *(const i32x4*)(pb + i * 2048);
+    for (int i = 0; i < 4; ++i) {
+      acc[i][0] = MM::run(b[0], a[i], acc[i][0]);
+      acc[i][1] = MM::run(b[1], a[i], acc[i][1]);
+      if (i < 2) nb[2 * i] = *(const i32x4*)(pb + 8192 * i), nb[2 * i + 1] = *(const i32x4*)(pb + 8192 * i + 4096), na[i] = *(const i32x4*)(pa + 4096 * i);
+      if (i == 2) na[2] = *(const i32x4*)(pa + 8192), na[3] = *(const i32x4*)(pa + 12288);
+      if constexpr (NL == 8) issue(ls, operand, lf + 2 * i, unit);
+      __builtin_amdgcn_sched_barrier(0);
+      acc[i][2] = MM::run(b[2], a[i], acc[i][2]);
+      acc[i][3] = MM::run(b[3], a[i], acc[i][3]);
+      if constexpr (NL == 8) issue(ls, operand, lf + 2 * i + 1, unit);
+      if constexpr (NL == 4) issue(ls, operand, lf + i, unit);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
-  auto multiply = [&](const i32x4 (&a)[4], const i32x4 (&b)[4]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = MM::run(b[j], a[i], acc[i][j]);
-  };
+  const std::integral_constant<int, 0> none{};
+  const std::integral_constant<int, 4> four{};
+  const std::integral_constant<int, 8> eight{};
+  auto behind = [](const int unit, const int n) { return unit + n * kUnit >= kRing * kUnit ? unit + (n - kRing) * kUnit : unit + n * kUnit; };
 
   if (s0 < s1) {
 #pragma unroll
-    for (int p = 0; p < kRing; ++p) issue(s0 + p);
-    asm volatile("s_waitcnt vmcnt(24)" ::: "memory");  // step s0 has landed (8 loads a step, three steps may be under way)
+    for (int x = 0; x < 32; ++x) {
+      if (x & 8) issue(s0 + x / 16, B, x & 7, (x / 8) * kUnit);
+      else issue(s0 + x / 16, A, x & 7, (x / 8) * kUnit);
+    }
+    asm volatile("s_waitcnt vmcnt(16)" ::: "memory");  // step s0 has landed
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    read(s0, 0, a0, b0);
-    for (int s = s0; s < s1; ++s) {
-      read(s, 1, a1, b1);
-      multiply(a0, b0);
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-      // own loads of step s + 1 have landed, own reads of step s are done: after the barrier both hold for every wavefront
-      asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
+    for (int i = 0; i < 4; ++i) a0[i] = *(const i32x4*)(lds + fa + i * 4096), b0[i] = *(const i32x4*)(lds + kUnit + fb + i * 4096);
+    int ua = 0;
+    for (int s = s0; s < s1; ++s) {
+      const int ub = behind(ua, 1), na = behind(ua, 2), nb = behind(ua, 3), la = behind(ua, 4);
+      quarter(a0, b0, 1, ua, ub, a1, b1, four, A, s + 2, 0, la);
+      quarter(a1, b1, 2, ua, ub, a0, b0, four, A, s + 2, 4, la);
+      quarter(a0, b0, 3, ua, ub, a1, b1, none, A, 0, 0, 0);
+      // own loads of step s + 1 have landed (the eight of A of s + 2 may be under way), own reads of step s are done: after the barrier both
+      // hold for every wavefront
+      asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      read(s + 1, 0, a0, b0);  // (behind the last step: zeros)
-      issue(s + kRing);
-      multiply(a1, b1);
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 2, 1);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
-        __builtin_amdgcn_sched_group_barrier(0x20, 1, 1);
-      }
+      __builtin_amdgcn_sched_barrier(0);
+      quarter(a1, b1, 0, na, nb, a0, b0, eight, B, s + 2, 0, ua);  // (the fragments behind the last step: zeros)
+      ua = na;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may still be on its way into LDS
     __syncthreads();
@@ -241,98 +248,78 @@ __global__ __launch_bounds__(256, 1) void gemm256_kernel(const GemmArgs<EPI> g) 
   put_tile<DUAL, typename MM::el>(acc, g.epi, id.split, g.M, id.m0 + wm * 128, id.n0 + wn * (DUAL ? 64 : 128), lane, lds + wave * Stage<4>::bytes);
 }
 
-template <int KIND, int BM, int BN, int WGM, int WGN, int TERMS, bool DUAL, class EPI>
-__global__ __launch_bounds__(WGM* WGN * 64, 2) void gemm_kernel(const GemmArgs<EPI> g) {
+// ---- 128 x 128: four wavefronts of 64 x 64, two workgroups a CU.  Steps of 128 bytes of k in two LDS buffers, one barrier a step; the other
+// workgroup covers its waits.  The piece of row r lies at piece ^ ((r >> 1) & 7).
+constexpr int kHalfBytes = 256 * 128;
+template <int KIND, int TERMS, bool DUAL, class EPI>
+__global__ __launch_bounds__(256, 2) void gemm128_kernel(const GemmArgs<EPI> g) {
   typedef Mfma<KIND> MM;
-  constexpr int NW = WGM * WGN, MI = BM / WGM / 32, NJ = BN / WGN / 32;
-  constexpr int GA = BM / 8 / NW, GB = BN / 8 / NW;  // 1 KiB loads of a wave a step
-  constexpr int BUF = (BM + BN) * 128;
-  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && (!DUAL || NJ % 2 == 0), "tile");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / WGN, wn = wave % WGN;
+  const int wm = wave >> 1, wn = wave & 1;
+  const TileId id = tile_of<128, DUAL ? 64 : 128>(g);
 
-  const TileId id = tile_of<BM, DUAL ? BN / 2 : BN>(g);
-  const int64_t m0 = id.m0;
-  const int n0 = id.n0, split = id.split;
-
-  const int lr = lane >> 3, piece = (lane & 7) ^ lr;
-  unsigned off_a[GA], off_b[GB];
-  __amdgpu_buffer_rsrc_t rs_a = rows_buffer(g.a.p, m0, g.M, g.a.ld, g.kb);
+  const int lr = lane >> 3, piece = (lane & 7) ^ ((wave & 1) * 4 + (lr >> 1));
+  unsigned off_a[4], off_b[4];
 #pragma unroll
-  for (int i = 0; i < GA; ++i) off_a[i] = (unsigned)(((i * NW + wave) * 8 + lr) * g.a.ld) + piece * 16;
-  __amdgpu_buffer_rsrc_t rs_b[2];
-  rs_b[0] = rows_buffer(g.b[0].p, n0, g.N, g.b[0].ld, g.kb);
-  rs_b[1] = DUAL ? rows_buffer(g.b[1].p, n0, g.N, g.b[1].ld, g.kb) : rs_b[0];
-#pragma unroll
-  for (int i = 0; i < GB; ++i) {
-    const int grp = i * NW + wave;  // DUAL: blocks of 32 rows alternate between the projections
-    const int row = DUAL ? (grp >> 3) * 32 + (grp & 3) * 8 + lr : grp * 8 + lr;
-    off_b[i] = (unsigned)(row * (DUAL && ((grp >> 2) & 1) ? g.b[1].ld : g.b[0].ld)) + piece * 16;
+  for (int i = 0; i < 4; ++i) {  // a load moves 8 rows; DUAL: load i brings 32 rows of projection i & 1
+    off_a[i] = (unsigned)(((i * 4 + wave) * 8 + lr) * g.a.ld) + piece * 16;
+    off_b[i] = (unsigned)((DUAL ? (i >> 1) * 32 + wave * 8 + lr : (i * 4 + wave) * 8 + lr) * g.b[DUAL ? i & 1 : 0].ld) + piece * 16;
   }
-  const bool up_wave = NW == 8 && ((wave >> 2) & 1);  // NW == 8: the projection of a load is the wave's, NW == 4: the load's
-
   const int steps = g.nk * TERMS;
-  const int s0 = split * g.per, s1 = s0 + g.per < steps ? s0 + g.per : steps;
+  const int s0 = id.split * g.per, s1 = s0 + g.per < steps ? s0 + g.per : steps;
 
-  auto issue = [&](const int s, const int buf) __attribute__((always_inline)) {
+  auto issue = [&](const int s) __attribute__((always_inline)) {
     const int kc = TERMS == 1 ? s : s / TERMS, t = TERMS == 1 ? 0 : s - kc * TERMS;
     const int k = kc * 128;
-    const bool beyond = k + piece * 16 >= g.kb;
-    const int pa = TERMS == 1 ? 0 : part_a(t) , pb = TERMS == 1 ? 0 : part_b(t);
-    char* base = lds + buf * BUF;
+    const unsigned beyond = (unsigned)(k + piece * 16 >= g.kb) << 31;  // (buffers end below 2^31)
+    const int64_t pa = TERMS == 1 ? 0 : part_a(t) * g.a.plane, pb = TERMS == 1 ? 0 : part_b(t) * g.b[0].plane;
+    char* base = lds + ((s - s0) & 1) * kHalfBytes + wave * 1024;
+    const __amdgpu_buffer_rsrc_t ra = rows_buffer(g.a.p + pa, id.m0, g.M, g.a.ld, g.kb);
+    const __amdgpu_buffer_rsrc_t rb[2] = {rows_buffer(g.b[0].p + pb, id.n0, g.N, g.b[0].ld, g.kb),
+                                          rows_buffer(g.b[DUAL].p + pb, id.n0, g.N, g.b[DUAL].ld, g.kb)};
 #pragma unroll
-    for (int i = 0; i < GA; ++i) {
-      const unsigned o = beyond ? 0x80000000u : off_a[i] + k;
-      const __amdgpu_buffer_rsrc_t rs = TERMS == 1 ? rs_a : rows_buffer(g.a.p + pa * g.a.plane, m0, g.M, g.a.ld, g.kb);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(base + (i * NW + wave) * 1024), 16, o, 0, 0, 0);
-    }
+    for (int i = 0; i < 4; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(base + i * 4096), 16, (off_a[i] + k) | beyond, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < GB; ++i) {
-      const unsigned o = beyond ? 0x80000000u : off_b[i] + k;
-      const bool up = DUAL && (NW == 8 ? up_wave : ((i * NW) >> 2) & 1);
-      const __amdgpu_buffer_rsrc_t rs =
-          TERMS == 1 ? (up ? rs_b[1] : rs_b[0]) : rows_buffer((up ? g.b[1].p : g.b[0].p) + pb * g.b[0].plane, n0, g.N, up ? g.b[1].ld : g.b[0].ld, g.kb);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(base + BM * 128 + (i * NW + wave) * 1024), 16, o, 0, 0, 0);
-    }
+    for (int i = 0; i < 4; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb[DUAL ? i & 1 : 0], (__attribute__((address_space(3))) void*)(base + 16384 + i * 4096), 16, (off_b[i] + k) | beyond, 0, 0, 0);
   };
 
-  typename MM::acc acc[MI][NJ];
+  typename MM::acc acc[2][2];
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
   const int hi = lane >> 5, row = lane & 31;
-  const int fa = (wm * MI * 32 + row) * 128, fb = BM * 128 + (wn * NJ * 32 + row) * 128;
-  if (s0 < s1) issue(s0, 0);
+  const int fa = (wm * 64 + row) * 128, fb = 16384 + (wn * 64 + row) * 128;
+  if (s0 < s1) issue(s0);
   for (int s = s0; s < s1; ++s) {
-    const int buf = (s - s0) & 1;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();  // step s has landed for every wave, and nobody reads the other buffer any more
+    __builtin_amdgcn_s_barrier();  // step s has landed for every wavefront, and nobody reads the other buffer any more
     asm volatile("" ::: "memory");
-    if (s + 1 < s1) issue(s + 1, buf ^ 1);
-    const char* base = lds + buf * BUF;
+    if (s + 1 < s1) issue(s + 1);
+    const char* base = lds + ((s - s0) & 1) * kHalfBytes;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      const int c = ((kk * 2 + hi) ^ (row & 7)) * 16;
-      i32x4 av[MI], bv[NJ];
+      const int c = ((kk * 2 + hi) ^ ((row >> 1) & 7)) * 16;
+      i32x4 av[2], bv[2];
 #pragma unroll
-      for (int i = 0; i < MI; ++i) av[i] = *(const i32x4*)(base + fa + i * 4096 + c);
+      for (int i = 0; i < 2; ++i) av[i] = *(const i32x4*)(base + fa + i * 4096 + c);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) bv[j] = *(const i32x4*)(base + fb + j * 4096 + c);
+      for (int j = 0; j < 2; ++j) bv[j] = *(const i32x4*)(base + fb + j * 4096 + c);
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = MM::run(bv[j], av[i], acc[i][j]);
+        for (int j = 0; j < 2; ++j) acc[i][j] = MM::run(bv[j], av[i], acc[i][j]);
     }
   }
-
   __syncthreads();
-  static_assert(NW * Stage<NJ>::bytes <= 2 * BUF, "the epilogue's pieces lie in the steps' buffers");
-  put_tile<DUAL, typename MM::el>(acc, g.epi, split, g.M, m0 + wm * MI * 32, n0 + wn * NJ * (DUAL ? 16 : 32), lane, lds + wave * Stage<NJ>::bytes);
+  static_assert(4 * Stage<2>::bytes <= 2 * kHalfBytes && 4 * Stage<4>::bytes <= kRing * kUnit, "the epilogue's pieces lie in the steps' buffers");
+  put_tile<DUAL, typename MM::el>(acc, g.epi, id.split, g.M, id.m0 + wm * 64, id.n0 + wn * (DUAL ? 32 : 64), lane, lds + wave * Stage<2>::bytes);
 }
 
 // ---- epilogues: one(split, m, n, v, cols, row): eight sums of row m from column n on; pair: of both projections.  n may lie beyond the

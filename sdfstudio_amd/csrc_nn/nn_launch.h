@@ -30,17 +30,16 @@ struct Tiling {
   int gm, gn, splits, per;
 };
 // Two tile sizes: 256 x 256 (one workgroup a CU) and 128 x 128 (two workgroups a CU).  The choice is the smaller estimate of
-//   rounds of workgroups over the 256 CUs x steps x time of a step (0.65 us for 64 bytes of k of a 256, 0.9 us for 128 bytes of two 128s side by
-// side) + the joining pass of a split k.
+//   rounds of workgroups over the 256 CUs x steps x time of a step (1.3 us, 0.9 us for two 128s side by side) + the joining pass of a split k.
 inline Tiling choose_tiling(const int64_t M, const int64_t N, const int64_t kb, const int terms) {
   Tiling best = {};
   double best_us = 1e30;
   for (int tile : {256, 128}) {
     const int64_t gm = ceil_div(M, tile), gn = ceil_div(N, tile), tiles = gm * gn;
     const int64_t slots = tile == 256 ? 256 : 512;
-    const int steps = (int)ceil_div(kb, tile == 256 ? 64 : 128) * terms;
-    const double step_us = tile == 256 ? 0.65 : 0.9;
-    const int most = (int)std::max<int64_t>(1, std::min<int64_t>(steps / (tile == 256 ? 8 : 4), 2 * slots / std::max<int64_t>(tiles, 1)));
+    const int steps = (int)ceil_div(kb, 128) * terms;
+    const double step_us = tile == 256 ? 1.3 : 0.9;
+    const int most = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 4, 2 * slots / std::max<int64_t>(tiles, 1)));
     for (int s = 1; s <= most; s = s < 4 ? s + 1 : s + s / 4) {
       const int per = (int)ceil_div(std::max(steps, 1), s);
       const double join = s == 1 ? 0.0 : 6.0 + (double)(s + 1) * (double)M * (double)N * 4.0 / 3e6;
@@ -58,12 +57,10 @@ int launch_gemm(Call& c, const Tiling& t, GemmArgs<EPI> g) {
   if (grid == 0) return 0;
   if (t.tile == 256) {
     auto* k = gemm256_kernel<KIND, TERMS, DUAL, EPI>;
-    ask_lds(k, kRing * kStageBytes);
-    g.nk = (int)ceil_div(g.kb, 64);
-    hipLaunchKernelGGL(k, dim3(grid), dim3(256), kRing * kStageBytes, c.stream, g);
+    ask_lds(k, kRing * kUnit);
+    hipLaunchKernelGGL(k, dim3(grid), dim3(256), kRing * kUnit, c.stream, g);
   } else {
-    auto* k = gemm_kernel<KIND, 128, 128, 2, 2, TERMS, DUAL, EPI>;
-    hipLaunchKernelGGL(k, dim3(grid), dim3(256), 2 * 256 * 128, c.stream, g);
+    hipLaunchKernelGGL((gemm128_kernel<KIND, TERMS, DUAL, EPI>), dim3(grid), dim3(256), 2 * kHalfBytes, c.stream, g);
   }
   NN_LAUNCHED("product");
   return 0;
