@@ -1,12 +1,13 @@
-// sdfnn — matrix products C[m, n] = sum_k A[m, k] B[n, k] on the matrix cores, both operands with their k adjacent in memory.
+// sdfnn — matrix products C[m, n] = sum_k A[m, k] B[n, k] on the matrix cores.
 //
-// One kernel serves 16-bit floats (v_mfma_f32_32x32x16), 8-bit integers (v_mfma_i32_32x32x32) and fp32 as three bf16 parts a value: to it a
-// row is a string of bytes, a step is 128 of them (64 16-bit or 128 8-bit elements of k), and an operand fragment is 16 bytes a lane
-// whatever they hold.
+// One scheme serves 16-bit floats (v_mfma_f32_32x32x16), 8-bit integers (v_mfma_i32_32x32x32) and fp32 as three bf16 parts a value: to it a
+// step is 128 bytes of k (64 16-bit or 128 8-bit elements), and an operand fragment is 16 bytes a lane whatever they hold.
 //   * Tiles go from HBM / L2 to LDS without passing registers (buffer_load_dwordx4 ... lds).  A row past the end of a matrix, and the bytes past
 //     k in the last step, lie outside the buffer's range, where the load returns zeros: ragged sizes cost no branch in the loop.
-//   * A fragment read takes one 16-byte piece of each of 32 rows: stored in order they would lie in the same few banks.  The pieces of a row are
-//     permuted instead (the permutation is applied to the GLOBAL address of the load, LDS itself is written in order).
+//   * A 16-bit operand may also lie with its k running DOWN the rows (x and dy in a weight's gradient, a weight in dx): its 64 rows of a step go
+//     to LDS as they are and ds_read_b64_tr_b16 turns 4 x 16 pieces of them into fragments, so that no transposed copy is ever made.
+//   * A fragment read takes one piece of many LDS rows: stored in order they would lie in the same few banks.  The pieces of a row are permuted
+//     instead (the permutation is applied to the GLOBAL address of the load, LDS itself is written in order).
 //   * The weights' rows (n) are operand A of the instruction and the tokens' rows (m) operand B: a lane then owns ONE m and runs of 4
 //     consecutive n, which the epilogue stages through LDS in 16-byte pieces.
 //   * fp32: x = p0 + p1 + p2 with p0 = bf16(x), p1 = bf16(x - p0), p2 = bf16(x - p0 - p1) holds all 24 bits; of the nine products of two
@@ -22,15 +23,17 @@ struct Operand {
   const char* p;
   int64_t ld;     // bytes between rows
   int64_t plane;  // bytes between the parts of an fp32 matrix
+  int64_t rows;   // k along the row: rows of the matrix; k down the rows: k
+  int64_t width;  // bytes of a row
 };
 
 template <class EPI>
 struct GemmArgs {
-  Operand a, b[2];  // b[1]: the second projection of a gated product
+  Operand a, b[2];  // b[1]: the second projection of a gated product, or what follows b[0] along k from step `turn` on
   int64_t M;
   int N;            // rows of one projection
-  int kb;           // bytes of k in a row (a multiple of 16)
-  int nk;           // steps of one pass: ceil(kb / 128)
+  int nk;           // steps of one pass
+  int turn;
   int per;          // steps (over all passes) of one split
   int gm, gn, splits;
   EPI epi;
@@ -57,12 +60,21 @@ template <> struct Mfma<2> {
 
 typedef __attribute__((address_space(3))) char lds_char;
 
-// the buffer over the rows of an operand from `row` on: its range ends with the last row's last byte
-NN_D __amdgpu_buffer_rsrc_t rows_buffer(const char* base, const int64_t row, const int64_t rows, const int64_t ld, const int kb) {
+// the buffer (descriptor words) over the rows of an operand (part `part`) from `row` on: its range ends with the last row's last byte
+NN_D i32x4 rows_buffer(const char* p, const int64_t ld, const int64_t rows, const int64_t width, const int64_t row) {
   const int64_t left = rows - row;
-  int64_t bytes = left > 0 ? (left - 1) * ld + kb : 0;
+  const uint64_t at = (uint64_t)p + (uint64_t)(row * ld);
+  int64_t bytes = (left - 1) * ld + width;
   bytes = bytes > 0x7ffffff0 ? 0x7ffffff0 : bytes;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + (left > 0 ? row * ld : 0)), 0, (int)bytes, 0x00020000);
+  bytes = left > 0 ? bytes : 0;
+  return i32x4{(int)(uint32_t)at, (int)(uint32_t)(at >> 32), (int)bytes, 0x00020000};
+}
+
+// 1 KiB, 16 bytes a lane, from the buffer to LDS (byte address `to`, the wavefront's).  Written as an instruction because the compiler, which
+// cannot tell the units of the ring apart, waits for every load it knows to write LDS before it reads any of LDS with
+// ds_read_b64_tr_b16.  It returns no register, and the loops wait for it by count.  m0 is written here and nowhere else in these kernels.
+NN_D void load_lds(const i32x4 buffer, const unsigned offset, const unsigned to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(buffer), "s"(to) : "memory");
 }
 
 // the parts multiplied by pass t of an fp32 product, smallest terms first
@@ -134,50 +146,116 @@ NN_D void put_tile(const ACC (&acc)[MI][NJ], const EPI& epi, const int split, co
   }
 }
 
+// ---- one operand's unit of a step in LDS: ROWS matrix rows x 128 bytes of k, moved by loads of 1 KiB, four wavefronts taking turns.
+// k along the row: LDS rows are matrix rows, piece c (16 bytes) of row r lies at c ^ ((r >> 1) & 7).
+// k down the rows (KM): LDS rows are the 64 k of a step, ROWS 16-bit elements each; piece c (32 bytes = 16 elements) of row r lies at
+// c ^ (2 (r & 3) + ((r >> 3) & 1)).  Either way the accesses of one pass over the banks lie in different places.
+template <int ROWS, bool KM>
+struct Side {
+  static constexpr int LOADS = ROWS / 32, RB = KM ? ROWS * 2 : 128;
+  // what load i of wavefront `wave` fetches: byte offset of the lane from the unit's first row
+  static NN_D unsigned offset(const int i, const int wave, const int lane, const int64_t ld) {
+    if constexpr (!KM) {
+      const int grp = i * 4 + wave, lr = lane >> 3;
+      return (unsigned)((grp * 8 + lr) * ld) + ((lane & 7) ^ ((grp & 1) * 4 + (lr >> 1))) * 16;
+    } else {
+      constexpr int RPL = 1024 / RB, LPR = 64 / RPL;
+      const int r = (i * 4 + wave) * RPL + lane / LPR, c = lane % LPR;
+      return (unsigned)(r * ld) + (((c >> 1) ^ ((r & 3) * 2 + ((r >> 3) & 1))) * 2 + (c & 1)) * 16;
+    }
+  }
+  // the lane's address of quarter 0 of block 0 of the wavefront's rows (from `first` on)
+  static NN_D int base(const int first, const int lane) {
+    if constexpr (!KM) return (first + (lane & 31)) * 128 + (((lane >> 5) ^ ((lane >> 1) & 7)) * 16);
+    const int r = (lane >> 5) * 8 + ((lane >> 2) & 3), f = (r & 3) * 2 + (lane >> 5);
+    return r * RB + (((first >> 4) + ((lane >> 4) & 1)) ^ f) * 32 + (lane & 3) * 8;
+  }
+  // the fragment of block i (32 rows), quarter q (32 bytes of k, resp. 16 k)
+  static NN_D i32x4 fragment(const char* lds, const int unit, const int base, const int i, const int q) {
+    if constexpr (!KM) return *(const i32x4*)(lds + unit + (base ^ (q * 32)) + i * 4096);
+    else {
+      typedef __attribute__((address_space(3))) s16x4* P;
+      const char* p = lds + unit + (base ^ (i * 64)) + q * 16 * RB;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)p), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p + 4 * RB));
+      return __builtin_bit_cast(i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+// loads of one operand.  TURN: it may go over to a second matrix along k
+template <int ROWS, bool KM, int TERMS, bool SECOND, bool TURN>
+struct Loader {
+  unsigned off[Side<ROWS, KM>::LOADS];
+  int piece;  // bytes of k in front of the lane's piece (k along the row)
+  template <class F>
+  NN_D void init(const int wave, const int lane, const int64_t first, F&& ld_of) {  // first: matrix row (KM: column) of the tile
+#pragma unroll
+    for (int i = 0; i < Side<ROWS, KM>::LOADS; ++i)
+      off[i] = Side<ROWS, KM>::offset(i, wave, lane, ld_of(i)) + (KM ? (unsigned)first * 2 : 0);
+    piece = ((lane & 7) ^ ((wave & 1) * 4 + (lane >> 4))) * 16;
+  }
+  // the buffer of step s
+  NN_D i32x4 buffer(const Operand& one, const Operand& two, const int turn, const int64_t row, const int s) const {
+    const int kc = TERMS == 1 ? s : s / TERMS, t = s - kc * TERMS;
+    const int part = TERMS == 1 ? 0 : SECOND ? part_b(t) : part_a(t);
+    if constexpr (!KM) return rows_buffer(one.p + part * one.plane, one.ld, one.rows, one.width, row);
+    const bool after = TURN && kc >= turn;
+    const int64_t at = (int64_t)(after ? kc - turn : kc) * 64;
+    return rows_buffer((after ? two.p : one.p) + part * (after ? two.plane : one.plane), one.ld, one.rows, one.width, at);
+  }
+  // load i of step s.  Steps behind the last one (beyond) lie out of range (buffers end below 2^31) and write zeros, so that the count of
+  // loads in flight stays the same
+  NN_D void issue(const i32x4 buf, const int64_t width, const int s, const bool beyond, const int i, const unsigned to) const {
+    const int kc = TERMS == 1 ? s : s / TERMS;
+    unsigned o = (unsigned)beyond << 31;
+    if constexpr (KM) o |= off[i];
+    else o |= (unsigned)(kc * 128 + piece >= (int)width) << 31 | (off[i] + kc * 128);
+    load_lds(buf, o, to);
+  }
+};
+
 // ---- 256 x 256: four wavefronts (one a SIMD) of 128 x 128.  A fragment is used for four instructions, so the operand reads take half of
 // LDS's bandwidth, and the 256 accumulators leave registers for a second set of fragments: the reads of one quarter step run under the 16
 // instructions of another.  A step is 128 bytes of k - whole lines, the request that L2 serves at full rate - and one operand's 256 rows of it
 // (32 KiB) are the unit of a ring of five, all of LDS: A0 B0 A1 B1 A2.  Both units of a step are free once the last wavefront has taken its
 // fourth quarter into registers; B of the step after next goes into the first of them at once and A of the one behind it into the second.
 // Loads are spread between the instructions, since a load that finds the address unit busy holds back what follows it.
-// The piece of row r lies at piece ^ ((r >> 1) & 7): the 16 rows of one pass over the banks lie in 16 different places.
 constexpr int kUnit = 256 * 128, kRing = 5;
-template <int KIND, int TERMS, bool DUAL, class EPI>
+template <int KIND, int TERMS, bool DUAL, bool AK, bool BK, class EPI>
 __global__ __launch_bounds__(256, 1) void gemm256_kernel(const GemmArgs<EPI> g) {
+  static_assert(!DUAL || (!AK && !BK), "gated products read k along the rows");
   typedef Mfma<KIND> MM;
+  typedef Side<256, AK> SA;
+  typedef Side<256, BK> SB;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1;
   const TileId id = tile_of<256, DUAL ? 128 : 256>(g);
 
-  const int lr = lane >> 3, piece = (lane & 7) ^ ((wave & 1) * 4 + (lr >> 1));
-  unsigned off_a[8], off_b[8];
+  Loader<256, AK, TERMS, false, false> la;
+  Loader<256, BK, TERMS, true, !AK> lb;
+  la.init(wave, lane, id.m0, [&](int) { return g.a.ld; });
+  lb.init(wave, lane, id.n0, [&](int i) { return g.b[DUAL ? i & 1 : 0].ld; });
+  if constexpr (DUAL) {  // load i brings rows of projection i & 1 (blocks of 32 rows alternate)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {  // a load moves 8 rows; DUAL: load i brings rows of projection i & 1 (blocks of 32 rows alternate)
-    off_a[i] = (unsigned)(((i * 4 + wave) * 8 + lr) * g.a.ld) + piece * 16;
-    off_b[i] = (unsigned)((DUAL ? (i >> 1) * 32 + wave * 8 + lr : (i * 4 + wave) * 8 + lr) * g.b[DUAL ? i & 1 : 0].ld) + piece * 16;
+    for (int i = 0; i < 8; ++i) lb.off[i] = (unsigned)(((i >> 1) * 32 + wave * 8 + (lane >> 3)) * g.b[i & 1].ld) + lb.piece;
   }
   const int steps = g.nk * TERMS;
   const int s0 = id.split * g.per, s1 = s0 + g.per < steps ? s0 + g.per : steps;
-  const __amdgpu_buffer_rsrc_t rs_a = rows_buffer(g.a.p, id.m0, g.M, g.a.ld, g.kb), rs_b0 = rows_buffer(g.b[0].p, id.n0, g.N, g.b[0].ld, g.kb),
-                               rs_b1 = rows_buffer(g.b[DUAL].p, id.n0, g.N, g.b[DUAL].ld, g.kb);
-
-  // load i of step s of one operand into the unit at `unit`; behind the last step they lie out of range and write zeros, so that the count of
-  // loads in flight stays the same
-  auto issue = [&](const int s, auto second, const int i, const int unit) __attribute__((always_inline)) {
-    constexpr bool B = decltype(second)::value;
-    const int kc = TERMS == 1 ? s : s / TERMS, t = TERMS == 1 ? 0 : s - kc * TERMS;
-    const int k = kc * 128;
-    const unsigned beyond = (unsigned)(s >= s1) << 31 | (unsigned)(k + piece * 16 >= g.kb) << 31;  // (buffers end below 2^31)
-    __amdgpu_buffer_rsrc_t rs;
-    if constexpr (TERMS == 1) rs = B ? DUAL && (i & 1) ? rs_b1 : rs_b0 : rs_a;
-    else if constexpr (B) rs = rows_buffer(g.b[DUAL ? i & 1 : 0].p + part_b(t) * g.b[0].plane, id.n0, g.N, g.b[DUAL ? i & 1 : 0].ld, g.kb);
-    else rs = rows_buffer(g.a.p + part_a(t) * g.a.plane, id.m0, g.M, g.a.ld, g.kb);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(lds + unit + wave * 1024 + i * 4096), 16,
-                                             ((B ? off_b[i] : off_a[i]) + k) | beyond, 0, 0, 0);
-  };
+  const unsigned ring = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds + wave * 1024;
   const std::integral_constant<bool, false> A{};
   const std::integral_constant<bool, true> B{};
+  i32x4 buf_a, buf_b[2];  // buffers of the step being loaded
+  auto aim_a = [&](const int s) __attribute__((always_inline)) { buf_a = la.buffer(g.a, g.a, 0, id.m0, s); };
+  auto aim_b = [&](const int s) __attribute__((always_inline)) {
+    buf_b[0] = lb.buffer(g.b[0], g.b[1], g.turn, id.n0, s);
+    if constexpr (DUAL) buf_b[1] = lb.buffer(g.b[1], g.b[1], g.turn, id.n0, s);
+  };
+  auto issue = [&](const int s, auto second, const int i, const int unit) __attribute__((always_inline)) {
+    const unsigned to = ring + unit + i * 4096;
+    if constexpr (decltype(second)::value) lb.issue(buf_b[DUAL ? i & 1 : 0], g.b[0].width, s, s >= s1, i, to);
+    else la.issue(buf_a, g.a.width, s, s >= s1, i, to);
+  };
 
   typename MM::acc acc[4][4];
 #pragma unroll
@@ -187,21 +265,23 @@ __global__ __launch_bounds__(256, 1) void gemm256_kernel(const GemmArgs<EPI> g) 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
-  const int row = lane & 31, c0 = ((lane >> 5) ^ ((row >> 1) & 7)) * 16;
-  const int fa = (wm * 128 + row) * 128 + c0, fb = (wn * 128 + row) * 128 + c0;  // quarter q: ^ 32 q
+  const int fa = SA::base(wm * 128, lane), fb = SB::base(wn * 128, lane);
   i32x4 a0[4], b0[4], a1[4], b1[4];
-  // a quarter step: the 16 instructions of the fragments (a, b); between them the reads of the next quarter's fragments (na, nb) from the
-  // units ua, ub and NL loads
+  // a quarter step: the 16 instructions of the fragments (a, b); between them the reads of quarter nq of the units ua, ub (na, nb) and NL
+  // loads
   auto quarter = [&](const i32x4 (&a)[4], const i32x4 (&b)[4], const int nq, const int ua, const int ub, i32x4 (&na)[4], i32x4 (&nb)[4],
                      auto nl, auto operand, const int ls, const int lf, const int unit) __attribute__((always_inline)) {
     constexpr int NL = decltype(nl)::value;
-    const char *pa = lds + ua + (fa ^ (nq * 32)), *pb = lds + ub + (fb ^ (nq * 32));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       acc[i][0] = MM::run(b[0], a[i], acc[i][0]);
       acc[i][1] = MM::run(b[1], a[i], acc[i][1]);
-      if (i < 2) nb[2 * i] = *(const i32x4*)(pb + 8192 * i), nb[2 * i + 1] = *(const i32x4*)(pb + 8192 * i + 4096), na[i] = *(const i32x4*)(pa + 4096 * i);
-      if (i == 2) na[2] = *(const i32x4*)(pa + 8192), na[3] = *(const i32x4*)(pa + 12288);
+      if (i < 2) {
+        nb[2 * i] = SB::fragment(lds, ub, fb, 2 * i, nq);
+        nb[2 * i + 1] = SB::fragment(lds, ub, fb, 2 * i + 1, nq);
+        na[i] = SA::fragment(lds, ua, fa, i, nq);
+      }
+      if (i == 2) na[2] = SA::fragment(lds, ua, fa, 2, nq), na[3] = SA::fragment(lds, ua, fa, 3, nq);
       if constexpr (NL == 8) issue(ls, operand, lf + 2 * i, unit);
       __builtin_amdgcn_sched_barrier(0);
       acc[i][2] = MM::run(b[2], a[i], acc[i][2]);
@@ -219,6 +299,7 @@ __global__ __launch_bounds__(256, 1) void gemm256_kernel(const GemmArgs<EPI> g) 
   if (s0 < s1) {
 #pragma unroll
     for (int x = 0; x < 32; ++x) {
+      if (x % 16 == 0) aim_a(s0 + x / 16), aim_b(s0 + x / 16);
       if (x & 8) issue(s0 + x / 16, B, x & 7, (x / 8) * kUnit);
       else issue(s0 + x / 16, A, x & 7, (x / 8) * kUnit);
     }
@@ -226,12 +307,14 @@ __global__ __launch_bounds__(256, 1) void gemm256_kernel(const GemmArgs<EPI> g) 
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a0[i] = *(const i32x4*)(lds + fa + i * 4096), b0[i] = *(const i32x4*)(lds + kUnit + fb + i * 4096);
+    for (int i = 0; i < 4; ++i) a0[i] = SA::fragment(lds, 0, fa, i, 0), b0[i] = SB::fragment(lds, kUnit, fb, i, 0);
     int ua = 0;
     for (int s = s0; s < s1; ++s) {
-      const int ub = behind(ua, 1), na = behind(ua, 2), nb = behind(ua, 3), la = behind(ua, 4);
-      quarter(a0, b0, 1, ua, ub, a1, b1, four, A, s + 2, 0, la);
-      quarter(a1, b1, 2, ua, ub, a0, b0, four, A, s + 2, 4, la);
+      const int ub = behind(ua, 1), na = behind(ua, 2), nb = behind(ua, 3), next = behind(ua, 4);
+      aim_a(s + 2);
+      aim_b(s + 2);
+      quarter(a0, b0, 1, ua, ub, a1, b1, four, A, s + 2, 0, next);
+      quarter(a1, b1, 2, ua, ub, a0, b0, four, A, s + 2, 4, next);
       quarter(a0, b0, 3, ua, ub, a1, b1, none, A, 0, 0, 0);
       // own loads of step s + 1 have landed (the eight of A of s + 2 may be under way), own reads of step s are done: after the barrier both
       // hold for every wavefront
@@ -248,42 +331,39 @@ __global__ __launch_bounds__(256, 1) void gemm256_kernel(const GemmArgs<EPI> g) 
   put_tile<DUAL, typename MM::el>(acc, g.epi, id.split, g.M, id.m0 + wm * 128, id.n0 + wn * (DUAL ? 64 : 128), lane, lds + wave * Stage<4>::bytes);
 }
 
-// ---- 128 x 128: four wavefronts of 64 x 64, two workgroups a CU.  Steps of 128 bytes of k in two LDS buffers, one barrier a step; the other
-// workgroup covers its waits.  The piece of row r lies at piece ^ ((r >> 1) & 7).
+// ---- 128 x 128: four wavefronts of 64 x 64, two workgroups a CU.  Two LDS buffers of a step, one barrier a step; the other workgroup covers its
+// waits.
 constexpr int kHalfBytes = 256 * 128;
-template <int KIND, int TERMS, bool DUAL, class EPI>
+template <int KIND, int TERMS, bool DUAL, bool AK, bool BK, class EPI>
 __global__ __launch_bounds__(256, 2) void gemm128_kernel(const GemmArgs<EPI> g) {
   typedef Mfma<KIND> MM;
+  typedef Side<128, AK> SA;
+  typedef Side<128, BK> SB;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1;
   const TileId id = tile_of<128, DUAL ? 64 : 128>(g);
 
-  const int lr = lane >> 3, piece = (lane & 7) ^ ((wave & 1) * 4 + (lr >> 1));
-  unsigned off_a[4], off_b[4];
+  Loader<128, AK, TERMS, false, false> la;
+  Loader<128, BK, TERMS, true, !AK> lb;
+  la.init(wave, lane, id.m0, [&](int) { return g.a.ld; });
+  lb.init(wave, lane, id.n0, [&](int i) { return g.b[DUAL ? i & 1 : 0].ld; });
+  if constexpr (DUAL) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {  // a load moves 8 rows; DUAL: load i brings 32 rows of projection i & 1
-    off_a[i] = (unsigned)(((i * 4 + wave) * 8 + lr) * g.a.ld) + piece * 16;
-    off_b[i] = (unsigned)((DUAL ? (i >> 1) * 32 + wave * 8 + lr : (i * 4 + wave) * 8 + lr) * g.b[DUAL ? i & 1 : 0].ld) + piece * 16;
+    for (int i = 0; i < 4; ++i) lb.off[i] = (unsigned)(((i >> 1) * 32 + wave * 8 + (lane >> 3)) * g.b[i & 1].ld) + lb.piece;
   }
   const int steps = g.nk * TERMS;
   const int s0 = id.split * g.per, s1 = s0 + g.per < steps ? s0 + g.per : steps;
-
+  const unsigned ring = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds + wave * 1024;
   auto issue = [&](const int s) __attribute__((always_inline)) {
-    const int kc = TERMS == 1 ? s : s / TERMS, t = TERMS == 1 ? 0 : s - kc * TERMS;
-    const int k = kc * 128;
-    const unsigned beyond = (unsigned)(k + piece * 16 >= g.kb) << 31;  // (buffers end below 2^31)
-    const int64_t pa = TERMS == 1 ? 0 : part_a(t) * g.a.plane, pb = TERMS == 1 ? 0 : part_b(t) * g.b[0].plane;
-    char* base = lds + ((s - s0) & 1) * kHalfBytes + wave * 1024;
-    const __amdgpu_buffer_rsrc_t ra = rows_buffer(g.a.p + pa, id.m0, g.M, g.a.ld, g.kb);
-    const __amdgpu_buffer_rsrc_t rb[2] = {rows_buffer(g.b[0].p + pb, id.n0, g.N, g.b[0].ld, g.kb),
-                                          rows_buffer(g.b[DUAL].p + pb, id.n0, g.N, g.b[DUAL].ld, g.kb)};
+    const unsigned to = ring + ((s - s0) & 1) * kHalfBytes;
+    const i32x4 buf_a = la.buffer(g.a, g.a, 0, id.m0, s), buf_b = lb.buffer(g.b[0], g.b[1], g.turn, id.n0, s);
+    i32x4 buf_u = buf_b;
+    if constexpr (DUAL) buf_u = lb.buffer(g.b[1], g.b[1], g.turn, id.n0, s);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(base + i * 4096), 16, (off_a[i] + k) | beyond, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) la.issue(buf_a, g.a.width, s, false, i, to + i * 4096);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb[DUAL ? i & 1 : 0], (__attribute__((address_space(3))) void*)(base + 16384 + i * 4096), 16, (off_b[i] + k) | beyond, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) lb.issue(i & 1 ? buf_u : buf_b, g.b[0].width, s, false, i, to + 16384 + i * 4096);
   };
 
   typename MM::acc acc[2][2];
@@ -294,23 +374,19 @@ __global__ __launch_bounds__(256, 2) void gemm128_kernel(const GemmArgs<EPI> g) 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
-  const int hi = lane >> 5, row = lane & 31;
-  const int fa = (wm * 64 + row) * 128, fb = 16384 + (wn * 64 + row) * 128;
+  const int fa = SA::base(wm * 64, lane), fb = SB::base(wn * 64, lane);
   if (s0 < s1) issue(s0);
   for (int s = s0; s < s1; ++s) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();  // step s has landed for every wavefront, and nobody reads the other buffer any more
     asm volatile("" ::: "memory");
     if (s + 1 < s1) issue(s + 1);
-    const char* base = lds + ((s - s0) & 1) * kHalfBytes;
+    const int unit = ((s - s0) & 1) * kHalfBytes;
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      const int c = ((kk * 2 + hi) ^ ((row >> 1) & 7)) * 16;
+    for (int q = 0; q < 4; ++q) {
       i32x4 av[2], bv[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) av[i] = *(const i32x4*)(base + fa + i * 4096 + c);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) bv[j] = *(const i32x4*)(base + fb + j * 4096 + c);
+      for (int i = 0; i < 2; ++i) av[i] = SA::fragment(lds, unit, fa, i, q), bv[i] = SB::fragment(lds, unit + 16384, fb, i, q);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -386,6 +462,7 @@ struct GatedEpi {
   static constexpr int kUnroll = 1;
   typedef Nothing Row;
   elem_t<DT>* a;
+  int64_t plane;   // fp32: 0: a as it is; else its three bf16 parts, as the second product reads them, this many bytes apart
   float *fu, *fg;  // factors of du and dg; NULL: inference
   int F, act;
   NN_D Nothing cols(int) const { return {}; }
@@ -407,17 +484,19 @@ struct GatedEpi {
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = act_only<DT != SDFNN_F32>(act, v[i]) * u[i];
     }
-    store8<DT>(a + m * F + n, o);
+    if (DT == SDFNN_F32 && plane) store_parts((char*)a + (m * F + n) * 2, plane, o);
+    else store8<DT>(a + m * F + n, o);
   }
 };
 
-// the gradient of a in, those of g and u out: [M][2 F], dg | du
+// the gradient of a in, those of g and u out: [M][2 F], dg | du (fp32: as three bf16 parts)
 template <int DT>
 struct GatedBwdEpi {
   static constexpr int kUnroll = 8;
   struct Row { float p[8], q[8]; };
   const float *fu, *fg;
-  elem_t<DT>* d;
+  char* d;
+  int64_t plane;
   int F;
   NN_D Nothing cols(int) const { return {}; }
   NN_D Row fetch(const int64_t m, const int64_t M, const int n) const {
@@ -433,8 +512,14 @@ struct GatedBwdEpi {
     float p[8], q[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = r.p[i] * v[i], q[i] = r.q[i] * v[i];
-    store8<DT>(d + m * 2 * F + n, q);
-    store8<DT>(d + m * 2 * F + F + n, p);
+    const int64_t at = m * 2 * F + n;
+    if constexpr (DT == SDFNN_F32) {
+      store_parts(d + at * 2, plane, q);
+      store_parts(d + (at + F) * 2, plane, p);
+    } else {
+      store8<DT>((elem_t<DT>*)d + at, q);
+      store8<DT>((elem_t<DT>*)d + at + F, p);
+    }
   }
 };
 

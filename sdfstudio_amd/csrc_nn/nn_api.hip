@@ -100,7 +100,7 @@ int norm_backward(NormArgs a, elem_t<DT>* dw, hipStream_t s) {
 // an operand that the tiles read where it lies, or its copy with rows of whole steps
 int int8_operand(Call& c, const int8_t* p, const int64_t ld, const int64_t rows, const int64_t k, const bool direct, Operand& o) {
   if (direct) {
-    o = {(const char*)p, ld, 0};
+    o = {(const char*)p, ld, 0, rows, k};
     return 0;
   }
   return pack_rows<1>(c, p, ld, rows, k, round_up(k, 128), o);
@@ -110,15 +110,16 @@ template <int DT, bool DUAL>
 int int8_products(Call& c, const int8_t* q, const int64_t ldq, const int8_t* w0, const int64_t ld0, const int8_t* w1, const int64_t ld1,
                   const int64_t rows, const int64_t n, const int64_t k, const Int8Epi<DT>& epi) {
   if (rows <= kSkinnyRows) {
-    const Operand a{(const char*)q, ldq, 0}, b0{(const char*)w0, ld0, 0}, b1{(const char*)w1, ld1, 0};
-    return skinny<2, DUAL>(c, a, b0, b1, rows, n, k, n, epi);
+    const Operand a{(const char*)q, ldq, 0, rows, k}, b0{(const char*)w0, ld0, 0, n, k}, b1{(const char*)w1, ld1, 0, n, k};
+    return skinny<2, DUAL>(c, a, b0, b1, rows, n, n, epi);
   }
   const bool direct = k % 16 == 0;
   Operand a{}, b0{}, b1{};
   NN_TRY(int8_operand(c, q, ldq, rows, k, direct, a));
   NN_TRY(int8_operand(c, w0, ld0, n, k, direct, b0));
   if (DUAL) NN_TRY(int8_operand(c, w1, ld1, n, k, direct, b1));
-  return product<2, 1, DUAL>(c, a, b0, b1, rows, n, direct ? k : round_up(k, 128), epi);
+  const int64_t nk = ceil_div(k, 128);
+  return product<2, 1, DUAL, kRows>(c, a, b0, b1, rows, n, nk, nk, epi);
 }
 
 int check_int8(const char* what, const int8_t* q, const int64_t ldq, const int8_t* w0, const int64_t ld0, const int8_t* w1, const int64_t ld1,
@@ -149,91 +150,101 @@ template <int DT> struct Kind {  // of the tile and of the few-row product
   static constexpr bool f32 = DT == SDFNN_F32;
 };
 
-// [rows, cols] with its k along the row: where it lies if the tiles can read it there (direct: 16-bit rows of a multiple of 8), else a copy
+// [rows, cols] where it lies if the tiles can read it there (16-bit rows of a multiple of 8), else a copy with rows of whole steps
 template <int DT>
-int row_operand(Call& c, const void* p, const int64_t ld, const int64_t rows, const int64_t cols, const bool direct, Operand& o) {
-  if (direct && !Kind<DT>::f32) {
-    o = {(const char*)p, ld * 2, 0};
+int operand(Call& c, const void* p, const int64_t ld, const int64_t rows, const int64_t cols, Operand& o) {
+  if (!Kind<DT>::f32 && cols % 8 == 0) {
+    o = {(const char*)p, ld * 2, 0, rows, cols * 2};
     return 0;
   }
   return pack_rows<Kind<DT>::es>(c, p, ld, rows, cols, round_up(cols, 64), o);
 }
 
+// what a forward pass keeps: fu, fg [rows][Fp] fp32 (GatedEpi), then a [rows][Fp]: 16-bit types and few rows of fp32 as it is, else as the
+// three bf16 parts that the products read
+template <int DT>
+struct Saved {
+  float *fu, *fg;
+  char* a;
+  int64_t plane;
+  Saved(void* p, const int64_t M, const int64_t Fp) : fu((float*)p), fg(fu + M * Fp), a((char*)(fg + M * Fp)), plane(parts(M) ? M * Fp * 2 : 0) {}
+  static bool parts(const int64_t M) { return Kind<DT>::f32 && M > kSkinnyRows; }
+  static int64_t a_size(const int64_t M, const int64_t Fp) { return M * Fp * (parts(M) ? 6 : Kind<DT>::es); }
+  static int64_t size(const int64_t M, const int64_t Fp) { return M * Fp * 8 + a_size(M, Fp); }
+};
+
 template <int DT>
 int gated_forward(Call& c, const void* x, const int64_t ldx, const void* wg, const void* wu, const void* wd, const int act, const int64_t M,
-                  const int64_t D, const int64_t F, const int64_t O, const bool save, void* saved, void* y) {
+                  const int64_t D, const int64_t F, const int64_t O, void* saved, void* y) {
   typedef elem_t<DT> T;
   typedef Kind<DT> K;
   const int64_t Fp = round_up(F, 64), es = K::es;
-  float *fu = nullptr, *fg = nullptr;
-  T* a;
-  if (save) fu = (float*)saved, fg = fu + M * Fp, a = (T*)(fg + M * Fp);
-  else a = (T*)c.take(M * Fp * es);
-  const GatedEpi<DT> ge{a, fu, fg, (int)Fp, act};
+  Saved<DT> sv(saved, M, Fp);
+  if (!saved) sv.fu = sv.fg = nullptr, sv.a = c.take(Saved<DT>::a_size(M, Fp));
+  const GatedEpi<DT> ge{(T*)sv.a, sv.plane, sv.fu, sv.fg, (int)Fp, act};
   const StoreEpi<DT> se{(T*)y, nullptr, M, M, 0, O, (int)O};
   if (M <= kSkinnyRows) {
-    const Operand xo{(const char*)x, ldx * es, 0}, g{(const char*)wg, D * es, 0}, u{(const char*)wu, D * es, 0};
-    const Operand ao{(const char*)a, Fp * es, 0}, d{(const char*)wd, F * es, 0};
-    NN_TRY((skinny<K::few, true>(c, xo, g, u, M, F, D * es, Fp, ge)));
-    return skinny<K::few, false>(c, ao, d, d, M, O, F * es, O, se);
+    const Operand xo{(const char*)x, ldx * es, 0, M, D * es}, g{(const char*)wg, D * es, 0, F, D * es}, u{(const char*)wu, D * es, 0, F, D * es};
+    const Operand ao{sv.a, Fp * es, 0, M, F * es}, d{(const char*)wd, F * es, 0, O, F * es};
+    NN_TRY((skinny<K::few, true>(c, xo, g, u, M, F, Fp, ge)));
+    return skinny<K::few, false>(c, ao, d, d, M, O, O, se);
   }
-  const bool d8 = D % 8 == 0, f8 = F % 8 == 0;
-  Operand xo, g, u, ao, d;
-  NN_TRY(row_operand<DT>(c, x, ldx, M, D, d8, xo));
-  NN_TRY(row_operand<DT>(c, wg, D, F, D, d8, g));
-  NN_TRY(row_operand<DT>(c, wu, D, F, D, d8, u));
-  NN_TRY((product<K::tile, K::terms, true>(c, xo, g, u, M, F, (d8 && !K::f32 ? D : round_up(D, 64)) * 2, ge)));
-  NN_TRY(row_operand<DT>(c, a, Fp, M, Fp, true, ao));
-  NN_TRY(row_operand<DT>(c, wd, F, O, F, f8, d));
-  return product<K::tile, K::terms, false>(c, ao, d, d, M, O, (f8 && !K::f32 ? F : Fp) * 2, se);
+  Operand xo, g, u, d;
+  NN_TRY(operand<DT>(c, x, ldx, M, D, xo));
+  NN_TRY(operand<DT>(c, wg, D, F, D, g));
+  NN_TRY(operand<DT>(c, wu, D, F, D, u));
+  const int64_t nd = ceil_div(D, 64), nf = Fp / 64;
+  NN_TRY((product<K::tile, K::terms, true, kRows>(c, xo, g, u, M, F, nd, nd, ge)));
+  NN_TRY(operand<DT>(c, wd, F, O, F, d));
+  const Operand ao{sv.a, Fp * 2, sv.plane, M, Fp * 2};
+  return product<K::tile, K::terms, false, kRows>(c, ao, d, d, M, O, nf, nf, se);
 }
 
 template <int DT>
 int gated_backward(Call& c, const void* x, const int64_t ldx, const void* wg, const void* wu, const void* wd, const void* saved, const void* dy,
-                   const int64_t lddy, const int64_t M, const int64_t D, const int64_t F, const int64_t O, void* dx, void* dwg,
-                   void* dwu, void* dwd) {
+                   const int64_t lddy, const int64_t M, const int64_t D, const int64_t F, const int64_t O, void* dx, void* dwg, void* dwu,
+                   void* dwd) {
   typedef elem_t<DT> T;
   typedef Kind<DT> K;
-  constexpr bool F32 = K::f32;
-  const int64_t Fp = round_up(F, 64), Op = round_up(O, 64), Mp = round_up(M, 64);
-  const float *fu = (const float*)saved, *fg = fu + M * Fp;
-  const T* a = (const T*)(fg + M * Fp);
-  T* dgu = (T*)c.take(M * 2 * Fp * K::es);
-  const bool o8 = O % 8 == 0;
+  const int64_t Fp = round_up(F, 64);
+  const Saved<DT> sv(const_cast<void*>(saved), M, Fp);
+  // gradients of g and u, side by side
+  const int64_t dplane = M * 2 * Fp * 2;
+  const Operand dgu{c.take((K::f32 ? 3 : 1) * dplane), 2 * Fp * 2, dplane, M, 2 * Fp * 2};
+  const int64_t nm = ceil_div(M, 64), nf = Fp / 64;
+  Operand dyo;
+  NN_TRY(operand<DT>(c, dy, lddy, M, O, dyo));
   const int64_t start = c.used;  // the operands of one product make room for those of the next
   int64_t most = start;
   auto next = [&]() { most = std::max(most, c.used), c.used = start; };
   if (dx || dwg) {
-    Operand dyo, wdt = take_operand<F32>(c, F, Op);
-    NN_TRY(row_operand<DT>(c, dy, lddy, M, O, o8, dyo));
-    NN_TRY(pack_transposed<F32>(c, wd, F, O, F, Op, 0, wdt));
-    const GatedBwdEpi<DT> be{fu, fg, dgu, (int)Fp};
-    NN_TRY((product<K::tile, K::terms, false>(c, dyo, wdt, wdt, M, F, (o8 && !F32 ? O : Op) * 2, be)));
+    Operand w;
+    NN_TRY(operand<DT>(c, wd, F, O, F, w));
+    const GatedBwdEpi<DT> be{sv.fu, sv.fg, const_cast<char*>(dgu.p), dgu.plane, (int)Fp};
+    const int64_t no = ceil_div(O, 64);
+    NN_TRY((product<K::tile, K::terms, false, kRowsDown>(c, dyo, w, w, M, F, no, no, be)));
     next();
   }
   if (dx) {
-    Operand d, w = take_operand<F32>(c, D, 2 * Fp);
-    NN_TRY(row_operand<DT>(c, dgu, 2 * Fp, M, 2 * Fp, true, d));
-    NN_TRY(pack_transposed<F32>(c, wg, D, F, D, Fp, 0, w));
-    NN_TRY(pack_transposed<F32>(c, wu, D, F, D, Fp, Fp, w));
+    Operand g, u;
+    NN_TRY(operand<DT>(c, wg, D, F, D, g));
+    NN_TRY(operand<DT>(c, wu, D, F, D, u));
     const StoreEpi<DT> se{(T*)dx, nullptr, M, M, 0, D, (int)D};
-    NN_TRY((product<K::tile, K::terms, false>(c, d, w, w, M, D, 2 * Fp * 2, se)));
+    NN_TRY((product<K::tile, K::terms, false, kRowsDown>(c, dgu, g, u, M, D, 2 * nf, nf, se)));
     next();
   }
   if (dwd) {
-    Operand dyt = take_operand<F32>(c, O, Mp), at = take_operand<F32>(c, F, Mp);
-    NN_TRY(pack_transposed<F32>(c, dy, lddy, M, O, Mp, 0, dyt));
-    NN_TRY(pack_transposed<F32>(c, a, Fp, M, F, Mp, 0, at));
+    Operand a{sv.a, Fp * 2, sv.plane, M, Fp * 2};
+    if (K::f32 && !Saved<DT>::parts(M)) NN_TRY(pack_rows<4>(c, sv.a, Fp, M, Fp, Fp, a));
     const StoreEpi<DT> se{(T*)dwd, nullptr, O, O, 0, F, (int)F};
-    NN_TRY((product<K::tile, K::terms, false>(c, dyt, at, at, O, F, Mp * 2, se)));
+    NN_TRY((product<K::tile, K::terms, false, kDown>(c, dyo, a, a, O, F, nm, nm, se)));
     next();
   }
   if (dwg) {
-    Operand dt = take_operand<F32>(c, 2 * Fp, Mp), xt = take_operand<F32>(c, D, Mp);
-    NN_TRY(pack_transposed<F32>(c, dgu, 2 * Fp, M, 2 * Fp, Mp, 0, dt));
-    NN_TRY(pack_transposed<F32>(c, x, ldx, M, D, Mp, 0, xt));
+    Operand xo;
+    NN_TRY(operand<DT>(c, x, ldx, M, D, xo));
     const StoreEpi<DT> se{(T*)dwg, (T*)dwu, Fp, F, F, D, (int)D};
-    NN_TRY((product<K::tile, K::terms, false>(c, dt, xt, xt, 2 * Fp, D, Mp * 2, se)));
+    NN_TRY((product<K::tile, K::terms, false, kDown>(c, dgu, xo, xo, 2 * Fp, D, nm, nm, se)));
     next();
   }
   c.used = most;
@@ -351,7 +362,8 @@ int sdfnn_int8_gated_linear(const int8_t* q, int64_t ldq, const float* sq, const
 
 int64_t sdfnn_gated_saved_size(int32_t dtype, int64_t rows, int64_t hidden) {
   if (dtype < SDFNN_F32 || dtype > SDFNN_F16 || rows < 0 || rows > kMaxRows || hidden < 1 || hidden > 1 << 20) return -1;
-  return rows * round_up(hidden, 64) * (8 + elem_size(dtype));
+  const int64_t Fp = round_up(hidden, 64);
+  return dtype == SDFNN_F32 ? Saved<SDFNN_F32>::size(rows, Fp) : Saved<SDFNN_BF16>::size(rows, Fp);
 }
 
 int64_t sdfnn_gated_workspace_size(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden, int64_t out, int32_t backward) {
@@ -361,7 +373,7 @@ int64_t sdfnn_gated_workspace_size(int32_t dtype, int64_t rows, int64_t dim, int
   by_dtype(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     if (backward) return gated_backward<DT>(c, nullptr, dim, nullptr, nullptr, nullptr, nullptr, nullptr, out, rows, dim, hidden, out, &some, &some, &some, &some);
-    return gated_forward<DT>(c, nullptr, dim, nullptr, nullptr, nullptr, 0, rows, dim, hidden, out, false, nullptr, nullptr);
+    return gated_forward<DT>(c, nullptr, dim, nullptr, nullptr, nullptr, 0, rows, dim, hidden, out, nullptr, nullptr);
   });
   return c.used;
 }
@@ -385,7 +397,7 @@ int sdfnn_gated_forward(const void* x, int64_t ldx, const void* w_gate, const vo
   if (rows == 0) return 0;
   Call c{(char*)workspace, 0, (hipStream_t)stream};
   return by_dtype(dtype, [&](auto dt) {
-    return gated_forward<decltype(dt)::value>(c, x, ldx, w_gate, w_up, w_down, act, rows, dim, hidden, out, saved != nullptr, saved, y);
+    return gated_forward<decltype(dt)::value>(c, x, ldx, w_gate, w_up, w_down, act, rows, dim, hidden, out, saved, y);
   });
 }
 
@@ -398,7 +410,9 @@ int sdfnn_gated_backward(const void* x, int64_t ldx, const void* w_gate, const v
   NN_REQUIRE(ldx >= dim && lddy >= out, "gated_backward: a row stride is smaller than the row");
   NN_REQUIRE(!dw_gate == !dw_up, "gated_backward: dw_gate and dw_up are computed together");
   const int64_t es = elem_size(dtype);
-  NN_REQUIRE(es == 4 || out % 8 || aligned16(dy, lddy * es), "gated_backward: with out a multiple of 8 rows of dy have to start at 16-byte boundaries");
+  NN_REQUIRE(es == 4 || ((out % 8 || aligned16(dy, lddy * es)) && (hidden % 8 || aligned16(w_down, 0)) &&
+                         (dim % 8 || (aligned16(x, ldx * es) && aligned16(w_gate, 0) && aligned16(w_up, 0)))),
+             "gated_backward: rows of a multiple of 8 elements have to start at 16-byte boundaries");
   NN_REQUIRE(aligned16(saved, 0), "gated_backward: saved has to start at a 16-byte boundary");
   const int64_t need = sdfnn_gated_workspace_size(dtype, rows, dim, hidden, out, 1);
   NN_REQUIRE(need == 0 || (workspace && aligned16(workspace, 0) && workspace_bytes >= need),

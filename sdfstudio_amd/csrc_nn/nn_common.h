@@ -65,6 +65,27 @@ NN_D void store8_n(elem_t<DT>* p, const int n, const float (&v)[8]) {
     if (i < n) p[i] = (elem_t<DT>)v[i];
 }
 
+// x = p0 + p1 + p2, each a bf16.  The largest finite values round to infinity as bf16: they are cut instead.  A value that is not finite is
+// its first part alone.
+NN_D void split3(const float x, uint16_t& p0, uint16_t& p1, uint16_t& p2) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, x);
+  uint16_t h = __builtin_bit_cast(uint16_t, (__bf16)x);
+  const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
+  if ((h & 0x7fffu) == 0x7f80u && finite) h = (uint16_t)(bits >> 16);
+  const float r = finite ? x - __builtin_bit_cast(float, (uint32_t)h << 16) : 0.0f;
+  p0 = h;
+  p1 = __builtin_bit_cast(uint16_t, (__bf16)r);
+  p2 = __builtin_bit_cast(uint16_t, (__bf16)(r - __builtin_bit_cast(float, (uint32_t)p1 << 16)));
+}
+// eight values as their three parts, `plane` bytes apart
+NN_D void store_parts(char* p, const int64_t plane, const float (&v)[8]) {
+  alignas(16) uint16_t h[3][8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) split3(v[e], h[0][e], h[1][e], h[2][e]);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) *(uint4*)(p + k * plane) = *(const uint4*)h[k];
+}
+
 // ---- activations of the gated block and their derivatives.  FAST (16-bit results): the hardware's exponential and reciprocal, one ulp of
 // fp32 each, the exponent rounded to fp32 before it.  fp32 results: the part of x log2(e) that this rounding loses goes back in to first
 // order, and one Newton step follows the reciprocal.  |x| is cut at 87, where the exponential leaves the normal numbers.

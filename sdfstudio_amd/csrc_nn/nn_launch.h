@@ -31,13 +31,13 @@ struct Tiling {
 };
 // Two tile sizes: 256 x 256 (one workgroup a CU) and 128 x 128 (two workgroups a CU).  The choice is the smaller estimate of
 //   rounds of workgroups over the 256 CUs x steps x time of a step (1.3 us, 0.9 us for two 128s side by side) + the joining pass of a split k.
-inline Tiling choose_tiling(const int64_t M, const int64_t N, const int64_t kb, const int terms) {
+inline Tiling choose_tiling(const int64_t M, const int64_t N, const int nk, const int terms) {
   Tiling best = {};
   double best_us = 1e30;
   for (int tile : {256, 128}) {
     const int64_t gm = ceil_div(M, tile), gn = ceil_div(N, tile), tiles = gm * gn;
     const int64_t slots = tile == 256 ? 256 : 512;
-    const int steps = (int)ceil_div(kb, 128) * terms;
+    const int steps = nk * terms;
     const double step_us = tile == 256 ? 1.3 : 0.9;
     const int most = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 4, 2 * slots / std::max<int64_t>(tiles, 1)));
     for (int s = 1; s <= most; s = s < 4 ? s + 1 : s + s / 4) {
@@ -50,39 +50,44 @@ inline Tiling choose_tiling(const int64_t M, const int64_t N, const int64_t kb, 
   return best;
 }
 
-template <int KIND, int TERMS, bool DUAL, class EPI>
+// k along the rows of an operand, or down them (KM)
+enum Sides { kRows, kRowsDown, kDown };  // A B: row row, row down, down down
+
+template <int KIND, int TERMS, bool DUAL, int SIDES, class EPI>
 int launch_gemm(Call& c, const Tiling& t, GemmArgs<EPI> g) {
+  constexpr bool AK = SIDES == kDown, BK = SIDES != kRows;
   g.gm = t.gm, g.gn = t.gn, g.splits = t.splits, g.per = t.per;
   const unsigned grid = (unsigned)((int64_t)t.gm * t.gn * t.splits);
   if (grid == 0) return 0;
   if (t.tile == 256) {
-    auto* k = gemm256_kernel<KIND, TERMS, DUAL, EPI>;
+    auto* k = gemm256_kernel<KIND, TERMS, DUAL, AK, BK, EPI>;
     ask_lds(k, kRing * kUnit);
     hipLaunchKernelGGL(k, dim3(grid), dim3(256), kRing * kUnit, c.stream, g);
   } else {
-    hipLaunchKernelGGL((gemm128_kernel<KIND, TERMS, DUAL, EPI>), dim3(grid), dim3(256), 2 * kHalfBytes, c.stream, g);
+    hipLaunchKernelGGL((gemm128_kernel<KIND, TERMS, DUAL, AK, BK, EPI>), dim3(grid), dim3(256), 2 * kHalfBytes, c.stream, g);
   }
   NN_LAUNCHED("product");
   return 0;
 }
 
-// one product (DUAL: two under a gate) through `epi`; k split where the tiles are few
-template <int KIND, int TERMS, bool DUAL, class EPI>
-int product(Call& c, const Operand& a, const Operand& b0, const Operand& b1, const int64_t M, const int64_t N, const int64_t kb, const EPI& epi) {
-  const int nk = (int)ceil_div(kb, 128);
-  const Tiling t = choose_tiling(M, DUAL ? 2 * N : N, kb, TERMS);
+// One product through `epi`; k split where the tiles are few.  DUAL: two under a gate.  Otherwise b1 follows b0 along k from step `turn` on.
+// nk: steps of 128 bytes of k
+template <int KIND, int TERMS, bool DUAL, int SIDES, class EPI>
+int product(Call& c, const Operand& a, const Operand& b0, const Operand& b1, const int64_t M, const int64_t N, const int64_t nk, const int64_t turn,
+            const EPI& epi) {
+  const Tiling t = choose_tiling(M, DUAL ? 2 * N : N, (int)nk, TERMS);
   const int64_t ld = (DUAL ? 2 : 1) * round_up(N, 64);
   char* part = t.splits > 1 ? c.take((int64_t)t.splits * M * ld * 4) : nullptr;
   if (c.dry() || M == 0 || N == 0) return 0;
   NN_REQUIRE(256 * std::max(a.ld, std::max(b0.ld, b1.ld)) < 0x7fffffff, "rows of more than 8 MiB are not supported");
-  NN_REQUIRE((int64_t)t.gm * t.gn * t.splits < 0x7fffffff, "too many tiles");
+  NN_REQUIRE((int64_t)t.gm * t.gn * t.splits < 0x7fffffff && nk * TERMS < 0x7fffffff, "too many tiles");
   if (t.splits == 1) {
-    GemmArgs<EPI> g{a, {b0, b1}, M, (int)N, (int)kb, nk, 0, 0, 0, 0, epi};
-    return launch_gemm<KIND, TERMS, DUAL>(c, t, g);
+    GemmArgs<EPI> g{a, {b0, b1}, M, (int)N, (int)nk, (int)turn, 0, 0, 0, 0, epi};
+    return launch_gemm<KIND, TERMS, DUAL, SIDES>(c, t, g);
   }
   PartialEpi pe{(uint32_t*)part, M, ld};
-  GemmArgs<PartialEpi> g{a, {b0, b1}, M, (int)N, (int)kb, nk, 0, 0, 0, 0, pe};
-  if (const int rc = launch_gemm<KIND, TERMS, DUAL>(c, t, g)) return rc;
+  GemmArgs<PartialEpi> g{a, {b0, b1}, M, (int)N, (int)nk, (int)turn, 0, 0, 0, 0, pe};
+  if (const int rc = launch_gemm<KIND, TERMS, DUAL, SIDES>(c, t, g)) return rc;
   const int64_t groups = round_up(N, 64) / 8 * M;
   hipLaunchKernelGGL((split_reduce_kernel<typename Mfma<KIND>::el, DUAL, EPI>), dim3((unsigned)ceil_div(groups, 256)), dim3(256), 0, c.stream,
                      (const typename Mfma<KIND>::el*)part, t.splits, M, ld, epi);
@@ -94,10 +99,9 @@ constexpr int64_t kSkinnyRows = 32;
 
 // the same for at most kSkinnyRows rows.  cols: columns that the epilogue writes (>= N)
 template <int KIND, bool DUAL, class EPI>
-int skinny(Call& c, const Operand& a, const Operand& b0, const Operand& b1, const int64_t M, const int64_t N, const int64_t kb, const int64_t cols,
-           const EPI& epi) {
+int skinny(Call& c, const Operand& a, const Operand& b0, const Operand& b1, const int64_t M, const int64_t N, const int64_t cols, const EPI& epi) {
   if (c.dry() || M == 0 || N == 0) return 0;
-  GemmArgs<EPI> g{a, {b0, b1}, M, (int)N, (int)kb, 0, 0, 0, 0, 0, epi};
+  GemmArgs<EPI> g{a, {b0, b1}, M, (int)N, 0, 0, 0, 0, 0, 0, epi};
   const dim3 grid((unsigned)ceil_div(cols, 16)), block(kSkinnyWaves * 64);
   if (M <= 16) hipLaunchKernelGGL((skinny_kernel<KIND, 1, DUAL, EPI>), grid, block, 0, c.stream, g);
   else hipLaunchKernelGGL((skinny_kernel<KIND, 2, DUAL, EPI>), grid, block, 0, c.stream, g);
@@ -105,31 +109,15 @@ int skinny(Call& c, const Operand& a, const Operand& b0, const Operand& b1, cons
   return 0;
 }
 
-// ---- operands.  ES: bytes of an element (4: three bf16 parts)
+// a copy of src with rows of whole steps.  ES: bytes of an element (4: three bf16 parts)
 template <int ES>
 int pack_rows(Call& c, const void* src, const int64_t ld, const int64_t rows, const int64_t cols, const int64_t pad, Operand& o) {
   const int64_t es = ES == 1 ? 1 : 2, plane = rows * pad * 2;
   char* dst = c.take(ES == 4 ? 3 * plane : rows * pad * es);
-  o = {dst, pad * es, plane};
+  o = {dst, pad * es, plane, rows, pad * es};
   if (c.dry() || rows == 0 || pad == 0) return 0;
   const PackArgs a{src, ld, rows, cols, dst, pad, plane, pad};
   hipLaunchKernelGGL((pack_rows_kernel<ES>), dim3((unsigned)ceil_div(rows * (pad / 8), 256)), dim3(256), 0, c.stream, a);
   NN_LAUNCHED("operand copy");
   return 0;
-}
-// src [rows, cols] into columns [at, at + pad) of dst: [cols] rows of dst_ld elements
-template <bool F32>
-int pack_transposed(Call& c, const void* src, const int64_t ld, const int64_t rows, const int64_t cols, const int64_t pad, const int64_t at,
-                    const Operand& o) {
-  if (c.dry() || cols == 0 || pad == 0) return 0;
-  const PackArgs a{src, ld, rows, cols, const_cast<char*>(o.p) + at * 2, o.ld / 2, o.plane, pad};
-  NN_REQUIRE(ceil_div(cols, 64) < 65536, "a transposed operand has at most 4194240 columns");
-  hipLaunchKernelGGL((pack_transposed_kernel<F32>), dim3((unsigned)(pad / 64), (unsigned)ceil_div(cols, 64)), dim3(256), 0, c.stream, a);
-  NN_LAUNCHED("operand transposition");
-  return 0;
-}
-template <bool F32>
-Operand take_operand(Call& c, const int64_t rows, const int64_t cols) {  // [rows][cols], cols a multiple of 64
-  const int64_t plane = rows * cols * 2;
-  return {c.take((F32 ? 3 : 1) * plane), cols * 2, plane};
 }

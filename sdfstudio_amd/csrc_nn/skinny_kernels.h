@@ -60,6 +60,7 @@ constexpr int kSkinnyWaves = 8, kSkinnyUnroll = 4;
 template <int KIND, int MT, bool DUAL, class EPI>
 __global__ __launch_bounds__(kSkinnyWaves * 64) void skinny_kernel(const GemmArgs<EPI> g) {
   typedef Small<KIND> S;
+  const int64_t kb = g.b[0].width;
   constexpr int NP = DUAL ? 2 : 1, U = kSkinnyUnroll;
   __shared__ typename S::el part[kSkinnyWaves][NP * MT][4][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -83,9 +84,9 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void skinny_kernel(const GemmArg
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) acc[p][i][r] = 0;
-  for (int64_t k = wave * (U * 64); k < g.kb; k += kSkinnyWaves * U * 64) {
+  for (int64_t k = wave * (U * 64); k < kb; k += kSkinnyWaves * U * 64) {
     i32x4 wv[U][NP], xv[U][MT];
-    if (k + U * 64 <= g.kb) {
+    if (k + U * 64 <= kb) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void skinny_kernel(const GemmArg
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t left = g.kb - (k + u * 64 + grp * 16);
+        const int64_t left = kb - (k + u * 64 + grp * 16);
 #pragma unroll
         for (int p = 0; p < NP; ++p) wv[u][p] = load16<S::ES>(w[p] + k + u * 64, left);
 #pragma unroll
