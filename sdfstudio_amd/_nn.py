@@ -3,6 +3,7 @@
 No fallback, as _lib.py: a missing library or a failing call raises.  PyTorch provides device memory and the stream.
 """
 import ctypes
+import functools
 import os
 from typing import Optional, Tuple
 
@@ -85,24 +86,22 @@ def on_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -
     return first.device
 
 
-def rows_of(t: torch.Tensor, align: bool = False) -> Tuple[torch.Tensor, int]:
-    """t [..., dim] as rows: ([rows, dim] whose rows the kernels can walk, row stride in elements).  A view wherever that is possible; a
-    copy for rows that are not adjacent in memory, overlap, or - with `align` - do not start at 16-byte boundaries although their width
-    would allow it."""
+def rows_of(t: torch.Tensor, align: bool = False) -> Tuple[torch.Tensor, int, int, int]:
+    """t [..., dim] as rows the kernels can walk: (tensor to keep alive, its address, rows, row stride in elements).  The tensor itself or a
+    view wherever that is possible; a copy for rows that are not adjacent in memory, overlap, or - with `align` - do not start at 16-byte
+    boundaries although their width would allow it."""
     dim = t.shape[-1]
-    rows = 1
-    for s in t.shape[:-1]:
-        rows *= s
+    whole = align and dim * t.element_size() % 16 == 0
+    if t.is_contiguous():
+        at = t.data_ptr()
+        if not (whole and at % 16):
+            return t, at, t.numel() // dim, dim
+    rows = t.numel() // dim
     t2 = t.reshape(rows, dim)
     stride = t2.stride(0) if rows > 1 else dim
-    es = t2.element_size()
-    bad = (dim > 1 and t2.stride(1) != 1) or (dim == 1 and rows > 1 and stride < 1) or stride < dim
-    if align and dim * es % 16 == 0:
-        bad = bad or t2.data_ptr() % 16 != 0 or stride * es % 16 != 0
-    if bad:
-        t2 = t2.clone(memory_format=torch.contiguous_format)
-        stride = dim
-    return t2, stride
+    if (dim > 1 and t2.stride(1) != 1) or stride < dim or (whole and (t2.data_ptr() % 16 or stride * t2.element_size() % 16)):
+        t2, stride = t2.clone(memory_format=torch.contiguous_format), dim
+    return t2, t2.data_ptr(), rows, stride
 
 
 def aligned(t: torch.Tensor) -> torch.Tensor:
@@ -118,10 +117,36 @@ def ptr(t: Optional[torch.Tensor]):
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     """Scratch memory of one call, from the caching allocator: it goes back when the call has been issued, in stream order, and inside a
     graph capture it belongs to that graph's pool - no two calls or graphs share one."""
-    if nbytes < 0:
-        raise SdfNnError("sizes refused by the library")
     return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
 
 
-def stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+class on:
+    """The call's device as the current one for the length of a `with` block (nothing is touched where it is already); `.stream` is its
+    current stream."""
+
+    __slots__ = ("device", "stream", "before")
+
+    def __init__(self, device: torch.device) -> None:
+        self.device = device
+
+    def __enter__(self) -> "on":
+        index = self.device.index
+        before = torch.cuda.current_device()
+        self.before = before if before != index else None
+        if self.before is not None:
+            torch.cuda.set_device(index)
+        self.stream = torch.cuda.current_stream(index).cuda_stream
+        return self
+
+    def __exit__(self, *exc) -> None:
+        if self.before is not None:
+            torch.cuda.set_device(self.before)
+
+
+@functools.lru_cache(maxsize=4096)
+def size(query: str, *args: int) -> int:
+    """A size query of the library (a function of sizes alone)."""
+    n = getattr(load(), query)(*args)
+    if n < 0:
+        raise SdfNnError(f"{query}{args}: refused")
+    return n

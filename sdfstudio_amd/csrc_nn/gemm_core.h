@@ -214,31 +214,37 @@ struct Loader {
   }
 };
 
-// ---- 256 x 256: four wavefronts (one a SIMD) of 128 x 128.  A fragment is used for four instructions, so the operand reads take half of
-// LDS's bandwidth, and the 256 accumulators leave registers for a second set of fragments: the reads of one quarter step run under the 16
-// instructions of another.  A step is 128 bytes of k - whole lines, the request that L2 serves at full rate - and one operand's 256 rows of it
-// (32 KiB) are the unit of a ring of five, all of LDS: A0 B0 A1 B1 A2.  Both units of a step are free once the last wavefront has taken its
-// fourth quarter into registers; B of the step after next goes into the first of them at once and A of the one behind it into the second.
-// Loads are spread between the instructions, since a load that finds the address unit busy holds back what follows it.
-constexpr int kUnit = 256 * 128, kRing = 5;
-template <int KIND, int TERMS, bool DUAL, bool AK, bool BK, class EPI>
-__global__ __launch_bounds__(256, 1) void gemm256_kernel(const GemmArgs<EPI> g) {
+// ---- the product: T x T tiles of four wavefronts, each a quarter of the tile.
+//   T = 256  one workgroup a CU (one wavefront a SIMD): a fragment is used for four instructions, so the operand reads take half of LDS's
+//            bandwidth; the 256 accumulators leave registers for a second set of fragments.
+//   T = 128  two workgroups a CU: more operand traffic, but one's epilogue runs under the other's instructions, and small products
+//            have four times the tiles.
+// The reads of one quarter step run under the instructions of another.  A step is 128 bytes of k - whole lines, the request that L2 serves at
+// full rate - and one operand's T rows of it are the unit of a ring of five in LDS: A0 B0 A1 B1 A2.  Both units of a step are free once the
+// last wavefront has taken its fourth quarter into registers; B of the step after next goes into the first of them at once and A of the
+// one behind it into the second.  Loads are spread between the instructions, since a load that finds the address unit busy holds back what
+// follows it.
+constexpr int kRing = 5;
+template <int T> struct Unit { static constexpr int bytes = T * 128, ring = kRing * bytes; };
+template <int T, int KIND, int TERMS, bool DUAL, bool AK, bool BK, class EPI>
+__global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(const GemmArgs<EPI> g) {
   static_assert(!DUAL || (!AK && !BK), "gated products read k along the rows");
   typedef Mfma<KIND> MM;
-  typedef Side<256, AK> SA;
-  typedef Side<256, BK> SB;
+  typedef Side<T, AK> SA;
+  typedef Side<T, BK> SB;
+  constexpr int MI = T / 64, LOADS = T / 32, UNIT = Unit<T>::bytes;  // blocks of a wavefront each way; its loads a unit
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1;
-  const TileId id = tile_of<256, DUAL ? 128 : 256>(g);
+  const TileId id = tile_of<T, DUAL ? T / 2 : T>(g);
 
-  Loader<256, AK, TERMS, false, false> la;
-  Loader<256, BK, TERMS, true, !AK> lb;
+  Loader<T, AK, TERMS, false, false> la;
+  Loader<T, BK, TERMS, true, !AK> lb;
   la.init(wave, lane, id.m0, [&](int) { return g.a.ld; });
   lb.init(wave, lane, id.n0, [&](int i) { return g.b[DUAL ? i & 1 : 0].ld; });
   if constexpr (DUAL) {  // load i brings rows of projection i & 1 (blocks of 32 rows alternate)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) lb.off[i] = (unsigned)(((i >> 1) * 32 + wave * 8 + (lane >> 3)) * g.b[i & 1].ld) + lb.piece;
+    for (int i = 0; i < LOADS; ++i) lb.off[i] = (unsigned)(((i >> 1) * 32 + wave * 8 + (lane >> 3)) * g.b[i & 1].ld) + lb.piece;
   }
   const int steps = g.nk * TERMS;
   const int s0 = id.split * g.per, s1 = s0 + g.per < steps ? s0 + g.per : steps;
@@ -246,8 +252,8 @@ __global__ __launch_bounds__(256, 1) void gemm256_kernel(const GemmArgs<EPI> g) 
   const std::integral_constant<bool, false> A{};
   const std::integral_constant<bool, true> B{};
   i32x4 buf_a, buf_b[2];  // buffers of the step being loaded
-  auto aim_a = [&](const int s) __attribute__((always_inline)) { buf_a = la.buffer(g.a, g.a, 0, id.m0, s); };
-  auto aim_b = [&](const int s) __attribute__((always_inline)) {
+  auto aim = [&](const int s) __attribute__((always_inline)) {
+    buf_a = la.buffer(g.a, g.a, 0, id.m0, s);
     buf_b[0] = lb.buffer(g.b[0], g.b[1], g.turn, id.n0, s);
     if constexpr (DUAL) buf_b[1] = lb.buffer(g.b[1], g.b[1], g.turn, id.n0, s);
   };
@@ -257,153 +263,91 @@ __global__ __launch_bounds__(256, 1) void gemm256_kernel(const GemmArgs<EPI> g) 
     else la.issue(buf_a, g.a.width, s, s >= s1, i, to);
   };
 
-  typename MM::acc acc[4][4];
+  typename MM::acc acc[MI][MI];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < MI; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
-  const int fa = SA::base(wm * 128, lane), fb = SB::base(wn * 128, lane);
-  i32x4 a0[4], b0[4], a1[4], b1[4];
-  // a quarter step: the 16 instructions of the fragments (a, b); between them the reads of quarter nq of the units ua, ub (na, nb) and NL
-  // loads
-  auto quarter = [&](const i32x4 (&a)[4], const i32x4 (&b)[4], const int nq, const int ua, const int ub, i32x4 (&na)[4], i32x4 (&nb)[4],
+  const int fa = SA::base(wm * (T / 2), lane), fb = SB::base(wn * (T / 2), lane);
+  i32x4 a0[MI], b0[MI], a1[MI], b1[MI];
+  // a quarter step: the instructions of the fragments (a, b); between them the reads of quarter nq of the units ua, ub (na, nb) and NL loads
+  auto quarter = [&](const i32x4 (&a)[MI], const i32x4 (&b)[MI], const int nq, const int ua, const int ub, i32x4 (&na)[MI], i32x4 (&nb)[MI],
                      auto nl, auto operand, const int ls, const int lf, const int unit) __attribute__((always_inline)) {
     constexpr int NL = decltype(nl)::value;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      acc[i][0] = MM::run(b[0], a[i], acc[i][0]);
-      acc[i][1] = MM::run(b[1], a[i], acc[i][1]);
-      if (i < 2) {
+    for (int i = 0; i < MI; ++i) {
+#pragma unroll
+      for (int j = 0; j < MI / 2; ++j) acc[i][j] = MM::run(b[j], a[i], acc[i][j]);
+      if (i < MI / 2) {
         nb[2 * i] = SB::fragment(lds, ub, fb, 2 * i, nq);
         nb[2 * i + 1] = SB::fragment(lds, ub, fb, 2 * i + 1, nq);
         na[i] = SA::fragment(lds, ua, fa, i, nq);
       }
-      if (i == 2) na[2] = SA::fragment(lds, ua, fa, 2, nq), na[3] = SA::fragment(lds, ua, fa, 3, nq);
-      if constexpr (NL == 8) issue(ls, operand, lf + 2 * i, unit);
+      if (i == MI / 2) {
+#pragma unroll
+        for (int x = MI / 2; x < MI; ++x) na[x] = SA::fragment(lds, ua, fa, x, nq);
+      }
+      if constexpr (NL == LOADS) issue(ls, operand, lf + 2 * i, unit);
       __builtin_amdgcn_sched_barrier(0);
-      acc[i][2] = MM::run(b[2], a[i], acc[i][2]);
-      acc[i][3] = MM::run(b[3], a[i], acc[i][3]);
-      if constexpr (NL == 8) issue(ls, operand, lf + 2 * i + 1, unit);
-      if constexpr (NL == 4) issue(ls, operand, lf + i, unit);
+#pragma unroll
+      for (int j = MI / 2; j < MI; ++j) acc[i][j] = MM::run(b[j], a[i], acc[i][j]);
+      if constexpr (NL == LOADS) issue(ls, operand, lf + 2 * i + 1, unit);
+      if constexpr (NL == LOADS / 2) issue(ls, operand, lf + i, unit);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   const std::integral_constant<int, 0> none{};
-  const std::integral_constant<int, 4> four{};
-  const std::integral_constant<int, 8> eight{};
-  auto behind = [](const int unit, const int n) { return unit + n * kUnit >= kRing * kUnit ? unit + (n - kRing) * kUnit : unit + n * kUnit; };
+  const std::integral_constant<int, LOADS / 2> some{};
+  const std::integral_constant<int, LOADS> all{};
+  auto behind = [](const int unit, const int n) { return unit + n * UNIT >= kRing * UNIT ? unit + (n - kRing) * UNIT : unit + n * UNIT; };
 
   if (s0 < s1) {
 #pragma unroll
-    for (int x = 0; x < 32; ++x) {
-      if (x % 16 == 0) aim_a(s0 + x / 16), aim_b(s0 + x / 16);
-      if (x & 8) issue(s0 + x / 16, B, x & 7, (x / 8) * kUnit);
-      else issue(s0 + x / 16, A, x & 7, (x / 8) * kUnit);
+    for (int x = 0; x < 4 * LOADS; ++x) {
+      if (x % (2 * LOADS) == 0) aim(s0 + x / (2 * LOADS));
+      if (x & LOADS) issue(s0 + x / (2 * LOADS), B, x % LOADS, (x / LOADS) * UNIT);
+      else issue(s0 + x / (2 * LOADS), A, x % LOADS, (x / LOADS) * UNIT);
     }
-    asm volatile("s_waitcnt vmcnt(16)" ::: "memory");  // step s0 has landed
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");  // step s0 has landed
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a0[i] = SA::fragment(lds, 0, fa, i, 0), b0[i] = SB::fragment(lds, kUnit, fb, i, 0);
+    for (int i = 0; i < MI; ++i) a0[i] = SA::fragment(lds, 0, fa, i, 0), b0[i] = SB::fragment(lds, UNIT, fb, i, 0);
     int ua = 0;
     for (int s = s0; s < s1; ++s) {
       const int ub = behind(ua, 1), na = behind(ua, 2), nb = behind(ua, 3), next = behind(ua, 4);
-      aim_a(s + 2);
-      aim_b(s + 2);
-      quarter(a0, b0, 1, ua, ub, a1, b1, four, A, s + 2, 0, next);
-      quarter(a1, b1, 2, ua, ub, a0, b0, four, A, s + 2, 4, next);
+      aim(s + 2);
+      quarter(a0, b0, 1, ua, ub, a1, b1, some, A, s + 2, 0, next);
+      quarter(a1, b1, 2, ua, ub, a0, b0, some, A, s + 2, LOADS / 2, next);
       quarter(a0, b0, 3, ua, ub, a1, b1, none, A, 0, 0, 0);
-      // own loads of step s + 1 have landed (the eight of A of s + 2 may be under way), own reads of step s are done: after the barrier both
-      // hold for every wavefront
-      asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+      // own loads of step s + 1 have landed (those of A of s + 2 may be under way), own reads of step s are done: after the barrier both hold
+      // for every wavefront
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
-      quarter(a1, b1, 0, na, nb, a0, b0, eight, B, s + 2, 0, ua);  // (the fragments behind the last step: zeros)
+      quarter(a1, b1, 0, na, nb, a0, b0, all, B, s + 2, 0, ua);  // (the fragments behind the last step: zeros)
       ua = na;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may still be on its way into LDS
     __syncthreads();
   }
-  put_tile<DUAL, typename MM::el>(acc, g.epi, id.split, g.M, id.m0 + wm * 128, id.n0 + wn * (DUAL ? 64 : 128), lane, lds + wave * Stage<4>::bytes);
-}
-
-// ---- 128 x 128: four wavefronts of 64 x 64, two workgroups a CU.  Two LDS buffers of a step, one barrier a step; the other workgroup covers its
-// waits.
-constexpr int kHalfBytes = 256 * 128;
-template <int KIND, int TERMS, bool DUAL, bool AK, bool BK, class EPI>
-__global__ __launch_bounds__(256, 2) void gemm128_kernel(const GemmArgs<EPI> g) {
-  typedef Mfma<KIND> MM;
-  typedef Side<128, AK> SA;
-  typedef Side<128, BK> SB;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
-  const TileId id = tile_of<128, DUAL ? 64 : 128>(g);
-
-  Loader<128, AK, TERMS, false, false> la;
-  Loader<128, BK, TERMS, true, !AK> lb;
-  la.init(wave, lane, id.m0, [&](int) { return g.a.ld; });
-  lb.init(wave, lane, id.n0, [&](int i) { return g.b[DUAL ? i & 1 : 0].ld; });
-  if constexpr (DUAL) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) lb.off[i] = (unsigned)(((i >> 1) * 32 + wave * 8 + (lane >> 3)) * g.b[i & 1].ld) + lb.piece;
-  }
-  const int steps = g.nk * TERMS;
-  const int s0 = id.split * g.per, s1 = s0 + g.per < steps ? s0 + g.per : steps;
-  const unsigned ring = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds + wave * 1024;
-  auto issue = [&](const int s) __attribute__((always_inline)) {
-    const unsigned to = ring + ((s - s0) & 1) * kHalfBytes;
-    const i32x4 buf_a = la.buffer(g.a, g.a, 0, id.m0, s), buf_b = lb.buffer(g.b[0], g.b[1], g.turn, id.n0, s);
-    i32x4 buf_u = buf_b;
-    if constexpr (DUAL) buf_u = lb.buffer(g.b[1], g.b[1], g.turn, id.n0, s);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) la.issue(buf_a, g.a.width, s, false, i, to + i * 4096);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) lb.issue(i & 1 ? buf_u : buf_b, g.b[0].width, s, false, i, to + 16384 + i * 4096);
-  };
-
-  typename MM::acc acc[2][2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
-
-  const int fa = SA::base(wm * 64, lane), fb = SB::base(wn * 64, lane);
-  if (s0 < s1) issue(s0);
-  for (int s = s0; s < s1; ++s) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();  // step s has landed for every wavefront, and nobody reads the other buffer any more
-    asm volatile("" ::: "memory");
-    if (s + 1 < s1) issue(s + 1);
-    const int unit = ((s - s0) & 1) * kHalfBytes;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      i32x4 av[2], bv[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) av[i] = SA::fragment(lds, unit, fa, i, q), bv[i] = SB::fragment(lds, unit + 16384, fb, i, q);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = MM::run(bv[j], av[i], acc[i][j]);
-    }
-  }
-  __syncthreads();
-  static_assert(4 * Stage<2>::bytes <= 2 * kHalfBytes && 4 * Stage<4>::bytes <= kRing * kUnit, "the epilogue's pieces lie in the steps' buffers");
-  put_tile<DUAL, typename MM::el>(acc, g.epi, id.split, g.M, id.m0 + wm * 64, id.n0 + wn * (DUAL ? 32 : 64), lane, lds + wave * Stage<2>::bytes);
+  static_assert(4 * Stage<MI>::bytes <= Unit<T>::ring, "the epilogue's pieces lie in the ring");
+  put_tile<DUAL, typename MM::el>(acc, g.epi, id.split, g.M, id.m0 + wm * (T / 2), id.n0 + wn * (DUAL ? T / 4 : T / 2), lane,
+                                  lds + wave * Stage<MI>::bytes);
 }
 
 // ---- epilogues: one(split, m, n, v, cols, row): eight sums of row m from column n on; pair: of both projections.  n may lie beyond the
 // matrix (in cols and fetch too), m only in fetch.
-// kUnroll: passes of put_tile side by side (few where their code is long)
+// kUnroll: passes of put_tile side by side (few where their code is long).  kCost: ps a column of a 256 x 256 tile's row spends in the epilogue
+// with all CUs at it (bytes at ~16 GB/s a CU and ns, or instructions), for the choice of tiles.
 struct Nothing {};
 // All sums of a split as they are: [split][m][ld] 32-bit words (pair: the second projection at + ld / 2)
 struct PartialEpi {
+  static constexpr int kCost = 250;
   static constexpr int kUnroll = 8;
   typedef Nothing Row;
   uint32_t* p;
@@ -435,6 +379,7 @@ struct PartialEpi {
 // y, or the two halves of one product's rows into two matrices (rows from `split_row` on: the second)
 template <int DT>
 struct StoreEpi {
+  static constexpr int kCost = DT == SDFNN_F32 ? 250 : 120;
   static constexpr int kUnroll = 8;
   typedef Nothing Row;
   elem_t<DT>*c0, *c1;
@@ -459,6 +404,7 @@ struct StoreEpi {
 // (error against 64 bits at 8192 x 4096 x 16384 bf16: 0.0031 of the gradients' size, 0.0024 this way, 0.0017 their own last rounding).
 template <int DT>
 struct GatedEpi {
+  static constexpr int kCost = DT == SDFNN_F32 ? 500 : 400;
   static constexpr int kUnroll = 1;
   typedef Nothing Row;
   elem_t<DT>* a;
@@ -492,6 +438,7 @@ struct GatedEpi {
 // the gradient of a in, those of g and u out: [M][2 F], dg | du (fp32: as three bf16 parts)
 template <int DT>
 struct GatedBwdEpi {
+  static constexpr int kCost = DT == SDFNN_F32 ? 1250 : 750;
   static constexpr int kUnroll = 8;
   struct Row { float p[8], q[8]; };
   const float *fu, *fg;
@@ -525,6 +472,7 @@ struct GatedBwdEpi {
 
 template <int DT>
 struct Int8Epi {
+  static constexpr int kCost = 250;  // (one for all result types: the workspace query does not know it)
   static constexpr int kUnroll = 8;
   struct Cols { float s[8], t[8]; };  // scales of the columns; t: of the second projection, or the bias
   typedef float Row;

@@ -104,24 +104,40 @@ NN_D float nn_recip(const float x) {  // 1 <= x < 2^127
   if constexpr (FAST) return r;
   return fmaf(fmaf(-x, r, 1.0f), r, r);
 }
-// Phi(z), the normal distribution function, and e = exp(-z^2 / 2): for x = |z| / sqrt(2)
-//   erfc(x) = exp(-x^2) t P(t),  t = 1 / (1 + 0.4 x),
-// P of degree 8 fitted to erfc(x) exp(x^2) / t over x >= 0 for the smallest relative error (1.3e-7): one exponential serves the value, its
-// tail to full relative accuracy, and the density in the derivative.
+// Phi(z), the normal distribution function.  For x = |z|:
+//   16-bit results: Phi(-x) = 2^(P(x) - x^2 / (2 ln 2)), P of degree 8 fitted to log2(erfcx(x / sqrt 2) / 2) on [0, 5] and held constant behind
+//   (Phi < 3e-7 there): off by 7e-7 at most, one exponential and no reciprocal.  The epilogues that call it are bound by such instructions.
+//   fp32 results: Phi(-x) = exp(-x^2 / 2) t P(t) / 2 with t = 1 / (1 + 0.4 x / sqrt 2), P of degree 8 fitted for the smallest relative error over
+//   x >= 0 (1.3e-7).
 template <bool FAST>
-NN_D float nn_phi(const float z, float& e) {
-  e = nn_exp<FAST>(-0.5f * z * z);
-  const float t = nn_recip<FAST>(fmaf(0.28284271247461900976f, fabsf(z), 1.0f));
-  float p = 0.0502621084f;
-  p = fmaf(p, t, -0.182901412f);
-  p = fmaf(p, t, 0.169085339f);
-  p = fmaf(p, t, -0.00560746621f);
-  p = fmaf(p, t, 0.141431406f);
-  p = fmaf(p, t, 0.168541983f);
-  p = fmaf(p, t, 0.207842693f);
-  p = fmaf(p, t, 0.225669593f);
-  p = fmaf(p, t, 0.225675866f);
-  const float c = 0.5f * e * t * p;
+NN_D float nn_phi(const float z) {
+  const float x = fabsf(z);
+  float p, c;
+  if constexpr (FAST) {
+    const float y = fminf(x, 5.0f);
+    p = -2.92766572e-07f;
+    p = fmaf(p, y, 4.06725712e-06f);
+    p = fmaf(p, y, 1.34747179e-05f);
+    p = fmaf(p, y, -0.000727434061f);
+    p = fmaf(p, y, 0.0080369357f);
+    p = fmaf(p, y, -0.0533734821f);
+    p = fmaf(p, y, 0.262529612f);
+    p = fmaf(p, y, -1.15117145f);
+    p = fmaf(p, y, -0.999998152f);
+    c = __builtin_amdgcn_exp2f(fmaf(z * z, -0.72134752044448170368f, p));
+  } else {
+    const float t = nn_recip<FAST>(fmaf(0.28284271247461900976f, x, 1.0f));
+    p = 0.0502621084f;
+    p = fmaf(p, t, -0.182901412f);
+    p = fmaf(p, t, 0.169085339f);
+    p = fmaf(p, t, -0.00560746621f);
+    p = fmaf(p, t, 0.141431406f);
+    p = fmaf(p, t, 0.168541983f);
+    p = fmaf(p, t, 0.207842693f);
+    p = fmaf(p, t, 0.225669593f);
+    p = fmaf(p, t, 0.225675866f);
+    c = 0.5f * nn_exp<FAST>(-0.5f * z * z) * t * p;
+  }
   return z < 0.0f ? c : 1.0f - c;
 }
 // a = act(z), d = act'(z)
@@ -132,10 +148,9 @@ NN_D void act_both(const int act, const float z, float& a, float& d) {
     a = z * s;
     d = s * (1.0f + z * (1.0f - s));
   } else if (act == SDFNN_GELU) {
-    float e;
-    const float phi = nn_phi<FAST>(z, e);
+    const float phi = nn_phi<FAST>(z);
     a = z * phi;
-    d = fmaf(z * 0.39894228040143267794f, e, phi);
+    d = fmaf(z * 0.39894228040143267794f, nn_exp<FAST>(-0.5f * z * z), phi);
   } else {
     a = z < 0.0f ? 0.0f : z;  // (a NaN stays one)
     d = z > 0.0f ? 1.0f : 0.0f;

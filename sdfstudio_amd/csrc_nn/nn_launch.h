@@ -29,21 +29,25 @@ struct Tiling {
   int tile;  // 256 or 128
   int gm, gn, splits, per;
 };
-// Two tile sizes: 256 x 256 (one workgroup a CU) and 128 x 128 (two workgroups a CU).  The choice is the smaller estimate of
-//   rounds of workgroups over the 256 CUs x steps x time of a step (1.3 us, 0.9 us for two 128s side by side) + the joining pass of a split k.
-inline Tiling choose_tiling(const int64_t M, const int64_t N, const int nk, const int terms) {
+// Which of the two tile sizes (gemm_core.h), and how often k is split: the smallest estimate of
+//   256: rounds of workgroups x (steps x 1.3 us + 5 us + the epilogue)
+//   128: rounds of pairs    x (max(steps x 1.08 us, two epilogues) + 3 us): one's epilogue runs under the other's steps
+// and, where k is split, the join of the raw sums.  Both sides measured (us, 256 / 128): 8192 x 4096 x 16384 bf16, plain store 800 / 1105;
+// 524288 x 512 x 256 fp32 with the gated backward's epilogue 1845 / 1490; 524288 x 1024 x 256 int8 gated 886 / 650.
+inline Tiling choose_tiling(const int64_t M, const int64_t N, const int nk, const int terms, const int cost) {
   Tiling best = {};
   double best_us = 1e30;
+  const int steps = nk * terms;
   for (int tile : {256, 128}) {
     const int64_t gm = ceil_div(M, tile), gn = ceil_div(N, tile), tiles = gm * gn;
     const int64_t slots = tile == 256 ? 256 : 512;
-    const int steps = nk * terms;
-    const double step_us = tile == 256 ? 1.3 : 0.9;
     const int most = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 4, 2 * slots / std::max<int64_t>(tiles, 1)));
     for (int s = 1; s <= most; s = s < 4 ? s + 1 : s + s / 4) {
       const int per = (int)ceil_div(std::max(steps, 1), s);
+      const double epilogue = 65536e-6 * (s == 1 ? cost : PartialEpi::kCost);
+      const double one = tile == 256 ? per * 1.3 + 5.0 + epilogue : std::max(per * 1.08, epilogue / 2) + 3.0;
       const double join = s == 1 ? 0.0 : 6.0 + (double)(s + 1) * (double)M * (double)N * 4.0 / 3e6;
-      const double us = (double)ceil_div(tiles * s, slots) * (per * step_us + 3.0) + join;
+      const double us = (double)ceil_div(tiles * s, slots) * one + join;
       if (us < best_us) best_us = us, best = {tile, (int)gm, (int)gn, (int)ceil_div(std::max(steps, 1), per), per};
     }
   }
@@ -59,13 +63,14 @@ int launch_gemm(Call& c, const Tiling& t, GemmArgs<EPI> g) {
   g.gm = t.gm, g.gn = t.gn, g.splits = t.splits, g.per = t.per;
   const unsigned grid = (unsigned)((int64_t)t.gm * t.gn * t.splits);
   if (grid == 0) return 0;
-  if (t.tile == 256) {
-    auto* k = gemm256_kernel<KIND, TERMS, DUAL, AK, BK, EPI>;
-    ask_lds(k, kRing * kUnit);
-    hipLaunchKernelGGL(k, dim3(grid), dim3(256), kRing * kUnit, c.stream, g);
-  } else {
-    hipLaunchKernelGGL((gemm128_kernel<KIND, TERMS, DUAL, AK, BK, EPI>), dim3(grid), dim3(256), 2 * kHalfBytes, c.stream, g);
-  }
+  auto start = [&](auto tile) {
+    constexpr int T = decltype(tile)::value;
+    auto* k = gemm_kernel<T, KIND, TERMS, DUAL, AK, BK, EPI>;
+    ask_lds(k, Unit<T>::ring);
+    hipLaunchKernelGGL(k, dim3(grid), dim3(256), Unit<T>::ring, c.stream, g);
+  };
+  if (t.tile == 256) start(std::integral_constant<int, 256>{});
+  else start(std::integral_constant<int, 128>{});
   NN_LAUNCHED("product");
   return 0;
 }
@@ -75,7 +80,7 @@ int launch_gemm(Call& c, const Tiling& t, GemmArgs<EPI> g) {
 template <int KIND, int TERMS, bool DUAL, int SIDES, class EPI>
 int product(Call& c, const Operand& a, const Operand& b0, const Operand& b1, const int64_t M, const int64_t N, const int64_t nk, const int64_t turn,
             const EPI& epi) {
-  const Tiling t = choose_tiling(M, DUAL ? 2 * N : N, (int)nk, TERMS);
+  const Tiling t = choose_tiling(M, DUAL ? 2 * N : N, (int)nk, TERMS, EPI::kCost);
   const int64_t ld = (DUAL ? 2 : 1) * round_up(N, 64);
   char* part = t.splits > 1 ? c.take((int64_t)t.splits * M * ld * 4) : nullptr;
   if (c.dry() || M == 0 || N == 0) return 0;

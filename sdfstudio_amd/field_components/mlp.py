@@ -22,18 +22,17 @@ class _GatedMLP(torch.autograd.Function):
         dev = _nn.on_device("gated_mlp", x, w_gate, w_up, w_down)
         hidden, out = w_gate.shape[0], w_down.shape[0]
         save = any(ctx.needs_input_grad)
-        with torch.cuda.device(dev):
-            x2, ldx = _nn.rows_of(x, align=True)
+        with _nn.on(dev) as cur:
+            x2, px, rows, ldx = _nn.rows_of(x, align=True)
             wg, wu, wd = _nn.aligned(w_gate), _nn.aligned(w_up), _nn.aligned(w_down)
-            rows, dim = x2.shape
+            dim = x.shape[-1]
             y = torch.empty((*x.shape[:-1], out), dtype=x.dtype, device=dev)
-            saved = _nn.workspace(lib.sdfnn_gated_saved_size(code, rows, hidden), dev) if save else None
+            saved = _nn.workspace(_nn.size("sdfnn_gated_saved_size", code, rows, hidden), dev) if save else None
             if rows:
-                size = lib.sdfnn_gated_workspace_size(code, rows, dim, hidden, out, 0)
+                size = _nn.size("sdfnn_gated_workspace_size", code, rows, dim, hidden, out, 0)
                 ws = _nn.workspace(size, dev)
-                _nn.check(lib.sdfnn_gated_forward(x2.data_ptr(), ldx, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), code, act, rows, dim, hidden,
-                                                  out, _nn.ptr(saved), y.data_ptr(), ws.data_ptr(), ws.numel(), _nn.stream()),
-                          "sdfnn_gated_forward")
+                _nn.check(lib.sdfnn_gated_forward(px, ldx, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), code, act, rows, dim, hidden, out,
+                                                  _nn.ptr(saved), y.data_ptr(), ws.data_ptr(), size, cur.stream), "sdfnn_gated_forward")
         if save:
             ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
         return y
@@ -45,21 +44,22 @@ class _GatedMLP(torch.autograd.Function):
         lib, code, dev = _nn.load(), _nn.dtype_code(x, "gated_mlp"), x.device
         hidden, out = w_gate.shape[0], w_down.shape[0]
         need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
-        with torch.cuda.device(dev):
-            x2, ldx = _nn.rows_of(x, align=True)
-            g2, ldg = _nn.rows_of(dy, align=True)
+        with _nn.on(dev) as cur:
+            x2, px, rows, ldx = _nn.rows_of(x, align=True)
+            g2, pg, _, ldg = _nn.rows_of(dy, align=True)
             wg, wu, wd = _nn.aligned(w_gate), _nn.aligned(w_up), _nn.aligned(w_down)
-            rows, dim = x2.shape
+            dim = x.shape[-1]
             dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
             dwg = torch.empty(hidden, dim, dtype=x.dtype, device=dev) if need_g or need_u else None
             dwu = torch.empty(hidden, dim, dtype=x.dtype, device=dev) if need_g or need_u else None
             dwd = torch.empty(out, hidden, dtype=x.dtype, device=dev) if need_d else None
             if rows == 0:
                 return dx, *(None if t is None else t.zero_() for t in (dwg, dwu, dwd)), None
-            ws = _nn.workspace(lib.sdfnn_gated_workspace_size(code, rows, dim, hidden, out, 1), dev)
-            _nn.check(lib.sdfnn_gated_backward(x2.data_ptr(), ldx, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), saved.data_ptr(), g2.data_ptr(),
-                                               ldg, code, rows, dim, hidden, out, _nn.ptr(dx), _nn.ptr(dwg), _nn.ptr(dwu),
-                                               _nn.ptr(dwd), ws.data_ptr(), ws.numel(), _nn.stream()), "sdfnn_gated_backward")
+            size = _nn.size("sdfnn_gated_workspace_size", code, rows, dim, hidden, out, 1)
+            ws = _nn.workspace(size, dev)
+            _nn.check(lib.sdfnn_gated_backward(px, ldx, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), saved.data_ptr(), pg, ldg, code, rows, dim,
+                                               hidden, out, _nn.ptr(dx), _nn.ptr(dwg), _nn.ptr(dwu), _nn.ptr(dwd), ws.data_ptr(), size,
+                                               cur.stream), "sdfnn_gated_backward")
         return dx, dwg if need_g else None, dwu if need_u else None, dwd, None
 
 

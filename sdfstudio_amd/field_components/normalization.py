@@ -27,17 +27,16 @@ class _RMSNorm(torch.autograd.Function):
     def forward(ctx, x, weight, residual, eps):
         lib, code = _nn.load(), _nn.dtype_code(x, "rms_norm")
         dev = _nn.on_device("rms_norm", x, weight, residual)
-        x2, ldx = _nn.rows_of(x)
-        r2, ldr = _nn.rows_of(residual) if residual is not None else (None, 0)
-        w = weight.contiguous()
-        rows, dim = x2.shape
-        with torch.cuda.device(dev):
+        with _nn.on(dev) as cur:
+            x2, px, rows, ldx = _nn.rows_of(x)
+            r2, pr, _, ldr = _nn.rows_of(residual) if residual is not None else (None, None, 0, 0)
+            w = weight.contiguous()
             y = torch.empty(x.shape, dtype=x.dtype, device=dev)
             h = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
             inv = torch.empty(rows, dtype=torch.float32, device=dev)
             if rows:
-                _nn.check(lib.sdfnn_rms_norm_forward(x2.data_ptr(), ldx, _nn.ptr(r2), ldr, w.data_ptr(), code, rows, dim, eps, y.data_ptr(),
-                                                     _nn.ptr(h), inv.data_ptr(), _nn.stream()), "sdfnn_rms_norm_forward")
+                _nn.check(lib.sdfnn_rms_norm_forward(px, ldx, pr, ldr, w.data_ptr(), code, rows, x.shape[-1], eps, y.data_ptr(), _nn.ptr(h),
+                                                     inv.data_ptr(), cur.stream), "sdfnn_rms_norm_forward")
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, weight, residual, inv)
         return y if residual is None else (y, h)
@@ -52,22 +51,20 @@ class _RMSNorm(torch.autograd.Function):
         need_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[2]
         need_w = ctx.needs_input_grad[1]
         dim = x.shape[-1]
-        with torch.cuda.device(dev):
-            x2, ldx = _nn.rows_of(x)
-            r2, ldr = _nn.rows_of(residual) if residual is not None else (None, 0)
+        with _nn.on(dev) as cur:
+            x2, px, rows, ldx = _nn.rows_of(x)
+            r2, pr, _, ldr = _nn.rows_of(residual) if residual is not None else (None, None, 0, 0)
             w = weight.contiguous()
-            g2, ldg = _nn.rows_of(dy) if dy is not None else (None, 0)
-            k2, ldk = _nn.rows_of(dh) if dh is not None else (None, 0)
-            rows = x2.shape[0]
+            g2, pg, _, ldg = _nn.rows_of(dy) if dy is not None else (None, None, 0, 0)
+            k2, pk, _, ldk = _nn.rows_of(dh) if dh is not None else (None, None, 0, 0)
             dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
             dw = torch.empty(dim, dtype=x.dtype, device=dev) if need_w else None
             if rows == 0:
                 return dx, dw.zero_() if need_w else None, dx if residual is not None else None, None
-            size = lib.sdfnn_rms_norm_backward_workspace_size(rows, dim)
+            size = _nn.size("sdfnn_rms_norm_backward_workspace_size", rows, dim) if need_w else 0
             ws = _nn.workspace(size, dev) if need_w else None
-            _nn.check(lib.sdfnn_rms_norm_backward(x2.data_ptr(), ldx, _nn.ptr(r2), ldr, w.data_ptr(), inv.data_ptr(), _nn.ptr(g2), ldg,
-                                                  _nn.ptr(k2), ldk, code, rows, dim, _nn.ptr(dx), _nn.ptr(dw), _nn.ptr(ws),
-                                                  size if need_w else 0, _nn.stream()), "sdfnn_rms_norm_backward")
+            _nn.check(lib.sdfnn_rms_norm_backward(px, ldx, pr, ldr, w.data_ptr(), inv.data_ptr(), pg, ldg, pk, ldk, code, rows, dim, _nn.ptr(dx),
+                                                  _nn.ptr(dw), _nn.ptr(ws), size, cur.stream), "sdfnn_rms_norm_backward")
         return dx, dw, dx if residual is not None else None, None
 
 
@@ -80,28 +77,26 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     return _RMSNorm.apply(x, weight, residual, float(eps))
 
 
-@torch.no_grad()
 def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
     """rms_norm with its output in 8 bits: codes int8 [..., dim] in [-127, 127] and scales float32 [...], codes * scales = y to half a step
     of max|y| / 127 a row.  Returns (codes, scales), with a residual (codes, scales, h).  For serving: no gradients."""
     _check("rms_norm_quantized", x, weight, residual)
-    return _quantize("rms_norm_quantized", x, weight, residual, eps)
+    return _quantize("rms_norm_quantized", x, weight, residual, float(eps))
 
 
 def _quantize(what: str, x: torch.Tensor, weight: Optional[torch.Tensor], residual: Optional[torch.Tensor], eps: float):
     lib, code = _nn.load(), _nn.dtype_code(x, what)
     dev = _nn.on_device(what, x, weight, residual)
-    with torch.cuda.device(dev):
-        x2, ldx = _nn.rows_of(x)
-        r2, ldr = _nn.rows_of(residual) if residual is not None else (None, 0)
+    with _nn.on(dev) as cur:
+        x2, px, rows, ldx = _nn.rows_of(x)
+        r2, pr, _, ldr = _nn.rows_of(residual) if residual is not None else (None, None, 0, 0)
         w = weight.contiguous() if weight is not None else None
-        rows, dim = x2.shape
         q = torch.empty(x.shape, dtype=torch.int8, device=dev)
         scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
         h = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
         if rows:
-            _nn.check(lib.sdfnn_rms_norm_quantize(x2.data_ptr(), ldx, _nn.ptr(r2), ldr, _nn.ptr(w), code, rows, dim, float(eps), q.data_ptr(),
-                                                  scales.data_ptr(), _nn.ptr(h), _nn.stream()), "sdfnn_rms_norm_quantize")
+            _nn.check(lib.sdfnn_rms_norm_quantize(px, ldx, pr, ldr, _nn.ptr(w), code, rows, x.shape[-1], eps, q.data_ptr(), scales.data_ptr(),
+                                                  _nn.ptr(h), cur.stream), "sdfnn_rms_norm_quantize")
     return (q, scales) if residual is None else (q, scales, h)
 
 

@@ -12,7 +12,6 @@ from sdfstudio_amd.field_components.normalization import _check, _quantize
 MAX_K = 131072  # 127 * 127 * k stays below 2^31
 
 
-@torch.no_grad()
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x [..., dim] -> (codes int8 [..., dim] in [-127, 127], scales float32 [...]): code = round(127 x / max|x|) half to even, scale =
     max|x| / 127 of its row (a row of zeros: scale 0).  Serves activations (a scale a token) and weights [out, in] (a scale a channel)."""
@@ -40,7 +39,6 @@ def _prepare(what, q, scales, weights, out_dtype):
         raise TypeError(f"{what}: out_dtype {out_dtype} (float32, bfloat16, float16)")
 
 
-@torch.no_grad()
 def int8_linear(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, weight_scales: torch.Tensor,
                 bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """y[..., n] = (sum_k q[..., k] weight_q[n, k]) scales[...] weight_scales[n] + bias[n] in out_dtype.  q int8 [..., k] with scales
@@ -51,23 +49,21 @@ def int8_linear(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, w
     if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (n,)):
         raise ValueError(f"{what}: bias {tuple(bias.shape)} {bias.dtype} for {n} channels: float32")
     lib, dev = _nn.load(), _nn.on_device(what, q, scales, weight_q, weight_scales, bias)
-    with torch.cuda.device(dev):
-        q2, ldq = _nn.rows_of(q, align=True)
-        w2, ldw = _nn.rows_of(weight_q, align=True)
+    with _nn.on(dev) as cur:
+        q2, pq, rows, ldq = _nn.rows_of(q, align=True)
+        w2, pw, _, ldw = _nn.rows_of(weight_q, align=True)
         sq, sw = scales.contiguous(), weight_scales.contiguous()
         b = bias.contiguous() if bias is not None else None
-        rows, k = q2.shape
+        k = q.shape[-1]
         y = torch.empty((*q.shape[:-1], n), dtype=out_dtype, device=dev)
         if rows and n:
-            size = lib.sdfnn_int8_linear_workspace_size(rows, n, k, 1)
+            size = _nn.size("sdfnn_int8_linear_workspace_size", rows, n, k, 1)
             ws = _nn.workspace(size, dev) if size else None
-            _nn.check(lib.sdfnn_int8_linear(q2.data_ptr(), ldq, sq.data_ptr(), w2.data_ptr(), ldw, sw.data_ptr(), _nn.ptr(b),
-                                            _nn.DTYPES[out_dtype], rows, n, k, y.data_ptr(), _nn.ptr(ws), size, _nn.stream()),
-                      "sdfnn_int8_linear")
+            _nn.check(lib.sdfnn_int8_linear(pq, ldq, sq.data_ptr(), pw, ldw, sw.data_ptr(), _nn.ptr(b), _nn.DTYPES[out_dtype], rows, n, k,
+                                            y.data_ptr(), _nn.ptr(ws), size, cur.stream), "sdfnn_int8_linear")
     return y
 
 
-@torch.no_grad()
 def int8_gated_linear(q: torch.Tensor, scales: torch.Tensor, gate_q: torch.Tensor, gate_scales: torch.Tensor, up_q: torch.Tensor,
                       up_scales: torch.Tensor, activation: str = "silu", out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """activation(gate) * up of two int8_linear products of the same rows, in one kernel: neither product is written out."""
@@ -78,19 +74,19 @@ def int8_gated_linear(q: torch.Tensor, scales: torch.Tensor, gate_q: torch.Tenso
     act = _nn.activation_code(activation, what)
     n = gate_q.shape[0]
     lib, dev = _nn.load(), _nn.on_device(what, q, scales, gate_q, gate_scales, up_q, up_scales)
-    with torch.cuda.device(dev):
-        q2, ldq = _nn.rows_of(q, align=True)
-        g2, ldg = _nn.rows_of(gate_q, align=True)
-        u2, ldu = _nn.rows_of(up_q, align=True)
+    with _nn.on(dev) as cur:
+        q2, pq, rows, ldq = _nn.rows_of(q, align=True)
+        g2, pg, _, ldg = _nn.rows_of(gate_q, align=True)
+        u2, pu, _, ldu = _nn.rows_of(up_q, align=True)
         sq, sg, su = scales.contiguous(), gate_scales.contiguous(), up_scales.contiguous()
-        rows, k = q2.shape
+        k = q.shape[-1]
         y = torch.empty((*q.shape[:-1], n), dtype=out_dtype, device=dev)
         if rows and n:
-            size = lib.sdfnn_int8_linear_workspace_size(rows, n, k, 2)
+            size = _nn.size("sdfnn_int8_linear_workspace_size", rows, n, k, 2)
             ws = _nn.workspace(size, dev) if size else None
-            _nn.check(lib.sdfnn_int8_gated_linear(q2.data_ptr(), ldq, sq.data_ptr(), g2.data_ptr(), ldg, sg.data_ptr(), u2.data_ptr(), ldu,
-                                                  su.data_ptr(), act, _nn.DTYPES[out_dtype], rows, n, k, y.data_ptr(), _nn.ptr(ws), size,
-                                                  _nn.stream()), "sdfnn_int8_gated_linear")
+            _nn.check(lib.sdfnn_int8_gated_linear(pq, ldq, sq.data_ptr(), pg, ldg, sg.data_ptr(), pu, ldu, su.data_ptr(), act,
+                                                  _nn.DTYPES[out_dtype], rows, n, k, y.data_ptr(), _nn.ptr(ws), size, cur.stream),
+                      "sdfnn_int8_gated_linear")
     return y
 
 
