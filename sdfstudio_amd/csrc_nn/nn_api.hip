@@ -28,10 +28,11 @@ constexpr int64_t kMaxRows = 0x7fffffff, kMaxDim = (int64_t)1 << 24;
 bool aligned16(const void* p, const int64_t ld_bytes) { return ((uintptr_t)p & 15) == 0 && (ld_bytes & 15) == 0; }
 
 // ---------------------------------------------------------------------------------------------- norm
-// f(IC<TPR>, IC<NV>, IC<U>) for the row width: how many threads and registers hold a row, how many rows at a time (norm_kernels.h)
+// f(IC<TPR>, IC<NV>, IC<U>) for the row width: how many threads and registers hold a row, how many rows at a time (norm_kernels.h); wide()
+// for rows that they do not hold
 template <int N> using IC = std::integral_constant<int, N>;
-template <class F>
-void pick_row(const int64_t dim, F&& f) {
+template <class F, class W>
+void pick_row(const int64_t dim, F&& f, W&& wide) {
   if (dim <= 64) f(IC<8>{}, IC<1>{}, IC<2>{});
   else if (dim <= 128) f(IC<16>{}, IC<1>{}, IC<2>{});
   else if (dim <= 256) f(IC<32>{}, IC<1>{}, IC<2>{});
@@ -40,12 +41,11 @@ void pick_row(const int64_t dim, F&& f) {
   else if (dim <= 2048) f(IC<64>{}, IC<4>{}, IC<1>{});
   else if (dim <= 4096) f(IC<256>{}, IC<2>{}, IC<1>{});
   else if (dim <= 8192) f(IC<256>{}, IC<4>{}, IC<1>{});
-  else if (dim <= 16384) f(IC<1024>{}, IC<2>{}, IC<1>{});
-  else f(IC<1024>{}, IC<0>{}, IC<1>{});
+  else wide();
 }
 // rows that a workgroup of that shape takes at a time
-int64_t rows_at_once(const int tpr, const int u) { return (tpr > 256 ? 1 : 256 / tpr) * u; }
-// workgroups that walk the rows of a forward pass: eight of 256 threads a CU are resident
+constexpr int64_t rows_at_once(const int tpr, const int u) { return (tpr > 256 ? 1 : 256 / tpr) * u; }
+// workgroups that walk the rows of a forward pass: no more than are resident at the kernels' registers (four of 256 threads a CU and up)
 int64_t row_groups(const int64_t rows, const int tpr, const int u) { return std::min<int64_t>(ceil_div(rows, rows_at_once(tpr, u)), 256 * 8); }
 
 int check_norm(const char* what, const void* x, const int64_t ldx, const void* residual, const int64_t ldr, const int32_t dtype,
@@ -58,21 +58,22 @@ int check_norm(const char* what, const void* x, const int64_t ldx, const void* r
   return 0;
 }
 
+#define NN_ROW_SHAPE constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, U = decltype(u)::value
 template <int DT>
 int norm_forward(const NormArgs& a, hipStream_t s) {
   pick_row(a.dim, [&](auto tpr, auto nv, auto u) {
-    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, U = decltype(u)::value;
-    hipLaunchKernelGGL((rms_norm_fwd_kernel<DT, TPR, NV, U>), dim3((unsigned)row_groups(a.rows, TPR, U)), dim3(TPR > 256 ? TPR : 256), 0, s, a);
-  });
+    NN_ROW_SHAPE;
+    hipLaunchKernelGGL((rms_norm_fwd_kernel<DT, TPR, NV, U>), dim3((unsigned)row_groups(a.rows, TPR, U)), dim3(256), 0, s, a);
+  }, [&] { hipLaunchKernelGGL((rms_norm_fwd_wide_kernel<DT>), dim3((unsigned)row_groups(a.rows, kWide, 1)), dim3(kWide), 0, s, a); });
   NN_LAUNCHED("rms_norm_forward");
   return 0;
 }
 template <int DT>
 int norm_quantize(const NormArgs& a, hipStream_t s) {
   pick_row(a.dim, [&](auto tpr, auto nv, auto u) {
-    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, U = decltype(u)::value;
-    hipLaunchKernelGGL((rms_norm_quant_kernel<DT, TPR, NV, U>), dim3((unsigned)row_groups(a.rows, TPR, U)), dim3(TPR > 256 ? TPR : 256), 0, s, a);
-  });
+    NN_ROW_SHAPE;
+    hipLaunchKernelGGL((rms_norm_quant_kernel<DT, TPR, NV, U>), dim3((unsigned)row_groups(a.rows, TPR, U)), dim3(256), 0, s, a);
+  }, [&] { hipLaunchKernelGGL((rms_norm_quant_wide_kernel<DT>), dim3((unsigned)row_groups(a.rows, kWide, 1)), dim3(kWide), 0, s, a); });
   NN_LAUNCHED("rms_norm_quantize");
   return 0;
 }
@@ -80,26 +81,27 @@ int norm_quantize(const NormArgs& a, hipStream_t s) {
 // workgroups of the backward pass (= partial sums of dweight): enough to fill the chip, but with at least two turns of rows each, so that their
 // sums stay small beside the tensors
 int64_t bwd_groups(const int64_t rows, const int64_t dim) {
-  int64_t groups = 1;
+  int64_t groups = std::min<int64_t>(rows, 256);
   pick_row(dim, [&](auto tpr, auto, auto u) {
     groups = std::min<int64_t>(ceil_div(rows, 2 * rows_at_once(decltype(tpr)::value, decltype(u)::value)), dim <= 8192 ? 1024 : 256);
-  });
+  }, [] {});
   return std::max<int64_t>(1, groups);
 }
 template <int DT>
 int norm_backward(NormArgs a, elem_t<DT>* dw, hipStream_t s) {
   const int64_t groups = bwd_groups(a.rows, a.dim);
-  bool wide = false;
   if (a.rows > 0)
     pick_row(a.dim, [&](auto tpr, auto nv, auto u) {
-      constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, U = decltype(u)::value;
-      wide = NV == 0;
-      if (dw && NV > 0) hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, TPR, NV, U, true>), dim3((unsigned)groups), dim3(TPR > 256 ? TPR : 256), 0, s, a);
-      else if (a.dx) hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, TPR, NV, U, false>), dim3((unsigned)groups), dim3(TPR > 256 ? TPR : 256), 0, s, a);
+      NN_ROW_SHAPE;
+      const dim3 grid((unsigned)groups), block(256);
+      if (dw) hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, TPR, NV, U, true>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, TPR, NV, U, false>), grid, block, 0, s, a);
+    }, [&] {
+      if (a.dx) hipLaunchKernelGGL((rms_norm_bwd_wide_kernel<DT>), dim3((unsigned)row_groups(a.rows, kWide, 1)), dim3(kWide), 0, s, a);
+      if (dw) hipLaunchKernelGGL((rms_norm_dw_wide_kernel<DT>), dim3((unsigned)ceil_div(a.dim, 256), (unsigned)groups), dim3(256), 0, s, a);
     });
   NN_LAUNCHED("rms_norm_backward");
   if (!dw) return 0;
-  if (wide) hipLaunchKernelGGL((rms_norm_dw_wide_kernel<DT>), dim3((unsigned)ceil_div(a.dim, 256), (unsigned)groups), dim3(256), 0, s, a);
   hipLaunchKernelGGL((rms_norm_dw_reduce_kernel<DT>), dim3((unsigned)ceil_div(a.dim, 32)), dim3(1024), 0, s, a.partial,
                      a.rows > 0 ? (int)groups : 0, a.dim, dw);
   NN_LAUNCHED("rms_norm_backward (weight)");

@@ -29,33 +29,49 @@ NN_HD constexpr int elem_size(const int dt) { return dt == SDFNN_F32 ? 4 : 2; }
 template <int N, int ALIGN>
 struct __attribute__((packed, aligned(ALIGN))) Bytes { uint32_t w[N]; };
 
+template <int DT> using Raw8 = Bytes<elem_size(DT) * 2, elem_size(DT)>;  // eight elements as they lie in memory
+
 template <int DT>
-NN_D void load8(const elem_t<DT>* p, float (&v)[8]) {
-  typedef elem_t<DT> T;
-  constexpr int NW = 8 * sizeof(T) / 4;
-  const Bytes<NW, sizeof(T)> raw = *reinterpret_cast<const Bytes<NW, sizeof(T)>*>(p);
-  T t[8];
-  __builtin_memcpy(t, &raw, sizeof(t));
+NN_D void widen8(const Raw8<DT>& raw, float (&v)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (DT == SDFNN_F32) v[i] = __builtin_bit_cast(float, (uint32_t)raw.w[i]);
+    else if constexpr (DT == SDFNN_BF16) v[i] = __builtin_bit_cast(float, i & 1 ? raw.w[i / 2] & 0xffff0000u : raw.w[i / 2] << 16);
+    else v[i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(raw.w[i / 2] >> (16 * (i & 1))));
+  }
 }
+template <int DT>
+NN_D Raw8<DT> raw8(const elem_t<DT>* p) { return *reinterpret_cast<const Raw8<DT>*>(p); }
+// the same with `n` valid elements and zeros behind them
+template <int DT>
+NN_D Raw8<DT> raw8_n(const elem_t<DT>* p, const int n) {
+  if (n >= 8) return raw8<DT>(p);
+  Raw8<DT> raw;
+  if constexpr (DT == SDFNN_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw.w[i] = i < n ? ((const uint32_t*)p)[i] : 0u;
+  } else {
+    const uint16_t* q = (const uint16_t*)p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      raw.w[i] = 2 * i < n ? q[2 * i] : 0u;
+      if (2 * i + 1 < n) raw.w[i] |= (uint32_t)q[2 * i + 1] << 16;
+    }
+  }
+  return raw;
+}
+template <int DT>
+NN_D void load8(const elem_t<DT>* p, float (&v)[8]) { widen8<DT>(raw8<DT>(p), v); }
+template <int DT>
+NN_D void load8_n(const elem_t<DT>* p, const int n, float (&v)[8]) { widen8<DT>(raw8_n<DT>(p, n), v); }
 template <int DT>
 NN_D void store8(elem_t<DT>* p, const float (&v)[8]) {
-  typedef elem_t<DT> T;
-  constexpr int NW = 8 * sizeof(T) / 4;
-  T t[8];
+  elem_t<DT> t[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = (T)v[i];
-  Bytes<NW, sizeof(T)> raw;
+  for (int i = 0; i < 8; ++i) t[i] = (elem_t<DT>)v[i];
+  Raw8<DT> raw;
   __builtin_memcpy(&raw, t, sizeof(t));
-  *reinterpret_cast<Bytes<NW, sizeof(T)>*>(p) = raw;
-}
-// the same with `n` valid elements (zeros behind them on a load)
-template <int DT>
-NN_D void load8_n(const elem_t<DT>* p, const int n, float (&v)[8]) {
-  if (n >= 8) return load8<DT>(p, v);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.0f;
+  *reinterpret_cast<Raw8<DT>*>(p) = raw;
 }
 template <int DT>
 NN_D void store8_n(elem_t<DT>* p, const int n, const float (&v)[8]) {
