@@ -8,6 +8,7 @@ import os
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SDFNN_LIB", os.path.join(_HERE, "libsdfnn.so"))
@@ -120,6 +121,22 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
 
 
+# the stream's handle without the Stream object around it (1 us of a call's host time)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def once(backward):
+    """A backward whose results cannot be differentiated again, as torch's once_differentiable makes it - whose bookkeeping, 20 us of host time, is
+    left out where no graph of the backward is recorded."""
+    guarded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return call
+
+
 class on:
     """The call's device as the current one for the length of a `with` block (nothing is touched where it is already); `.stream` is its
     current stream."""
@@ -135,7 +152,7 @@ class on:
         self.before = before if before != index else None
         if self.before is not None:
             torch.cuda.set_device(index)
-        self.stream = torch.cuda.current_stream(index).cuda_stream
+        self.stream = _raw_stream(index)
         return self
 
     def __exit__(self, *exc) -> None:

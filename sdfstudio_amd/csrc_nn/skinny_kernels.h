@@ -55,14 +55,14 @@ NN_D i32x4 load16(const char* p, const int64_t left) {  // 16 bytes, `left` of t
   return v;
 }
 
-constexpr int kSkinnyWaves = 8, kSkinnyUnroll = 4;
+constexpr int kSkinnyWaves = 8;
 
 template <int KIND, int MT, bool DUAL, class EPI>
 __global__ __launch_bounds__(kSkinnyWaves * 64) void skinny_kernel(const GemmArgs<EPI> g) {
-  typedef Small<KIND> S;
+  typedef Small<KIND> S_;
   const int64_t kb = g.b[0].width;
-  constexpr int NP = DUAL ? 2 : 1, U = kSkinnyUnroll;
-  __shared__ typename S::el part[kSkinnyWaves][NP * MT][4][64];
+  constexpr int NP = DUAL ? 2 : 1, U = (DUAL ? 4 : 8) / MT;  // 8 KiB of weights a wavefront and turn (half of it where x takes the registers)
+  __shared__ typename S_::el part[kSkinnyWaves][NP * MT][4][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int n0 = blockIdx.x * 16;
@@ -77,40 +77,57 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void skinny_kernel(const GemmArg
     const int64_t m = i * 16 + col < g.M ? i * 16 + col : g.M - 1;
     x[i] = g.a.p + m * g.a.ld + grp * 16;
   }
-  typename S::acc acc[NP][MT];
+  typename S_::acc acc[NP][MT];
 #pragma unroll
   for (int p = 0; p < NP; ++p)
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) acc[p][i][r] = 0;
-  for (int64_t k = wave * (U * 64); k < kb; k += kSkinnyWaves * U * 64) {
-    i32x4 wv[U][NP], xv[U][MT];
+  // two sets of fragments: the loads of the next turn are under way while this one's are multiplied
+  i32x4 wv[2][U][NP], xv[2][U][MT];
+  auto load = [&](const int64_t k, auto set) __attribute__((always_inline)) {
+    constexpr int S = decltype(set)::value;
     if (k + U * 64 <= kb) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int p = 0; p < NP; ++p) wv[u][p] = load16<S::ES>(w[p] + k + u * 64, 16);
+        for (int p = 0; p < NP; ++p) wv[S][u][p] = load16<S_::ES>(w[p] + k + u * 64, 16);
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) xv[u][i] = load16<S::ES>(x[i] + k + u * 64, 16);
+        for (int i = 0; i < MT; ++i) xv[S][u][i] = load16<S_::ES>(x[i] + k + u * 64, 16);
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int64_t left = kb - (k + u * 64 + grp * 16);
 #pragma unroll
-        for (int p = 0; p < NP; ++p) wv[u][p] = load16<S::ES>(w[p] + k + u * 64, left);
+        for (int p = 0; p < NP; ++p) wv[S][u][p] = load16<S_::ES>(w[p] + k + u * 64, left);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) xv[u][i] = load16<S::ES>(x[i] + k + u * 64, left);
+        for (int i = 0; i < MT; ++i) xv[S][u][i] = load16<S_::ES>(x[i] + k + u * 64, left);
       }
     }
+  };
+  auto multiply = [&](auto set) __attribute__((always_inline)) {
+    constexpr int S = decltype(set)::value;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int p = 0; p < NP; ++p)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[p][i] = S::run(wv[u][p], xv[u][i], acc[p][i]);
+        for (int i = 0; i < MT; ++i) acc[p][i] = S_::run(wv[S][u][p], xv[S][u][i], acc[p][i]);
+  };
+  const std::integral_constant<int, 0> s0{};
+  const std::integral_constant<int, 1> s1{};
+  constexpr int64_t turn = kSkinnyWaves * U * 64;
+  int64_t k = wave * (U * 64);
+  if (k < kb) load(k, s0);
+  for (; k < kb; k += 2 * turn) {
+    if (k + turn < kb) load(k + turn, s1);
+    multiply(s0);
+    if (k + turn >= kb) break;
+    if (k + 2 * turn < kb) load(k + 2 * turn, s0);
+    multiply(s1);
   }
 #pragma unroll
   for (int p = 0; p < NP; ++p)
@@ -123,15 +140,15 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void skinny_kernel(const GemmArg
   if (threadIdx.x < MT * 32) {
     const int i = threadIdx.x >> 5, half = (threadIdx.x >> 4) & 1, c = threadIdx.x & 15;
     const int64_t m = i * 16 + c;
-    typename S::el v[NP][8];
+    typename S_::el v[NP][8];
 #pragma unroll
     for (int p = 0; p < NP; ++p)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        typename S::el s = 0;
+        typename S_::el s = 0;
 #pragma unroll
         for (int k = 0; k < kSkinnyWaves; ++k) s += part[k][p * MT + i][e & 3][(half * 2 + (e >> 2)) * 16 + c];
-        v[p][e] = n0 + half * 8 + e < g.N ? s : (typename S::el)0;  // the padding columns of a workspace are zeros
+        v[p][e] = n0 + half * 8 + e < g.N ? s : (typename S_::el)0;  // the padding columns of a workspace are zeros
       }
     if (m < g.M) {
       const int c = n0 + half * 8;

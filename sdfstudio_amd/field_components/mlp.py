@@ -8,7 +8,6 @@ from typing import Optional
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from sdfstudio_amd import _nn
 from sdfstudio_amd.field_components.normalization import RMSNorm
@@ -38,7 +37,7 @@ class _GatedMLP(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_nn.once
     def backward(ctx, dy):
         x, w_gate, w_up, w_down, saved = ctx.saved_tensors
         lib, code, dev = _nn.load(), _nn.dtype_code(x, "gated_mlp"), x.device

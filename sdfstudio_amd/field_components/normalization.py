@@ -8,7 +8,6 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from sdfstudio_amd import _nn
 
@@ -42,7 +41,7 @@ class _RMSNorm(torch.autograd.Function):
         return y if residual is None else (y, h)
 
     @staticmethod
-    @once_differentiable
+    @_nn.once
     def backward(ctx, dy, dh=None):
         x, weight, residual, inv = ctx.saved_tensors
         if dy is None and dh is None:
