@@ -8,7 +8,6 @@ import os
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SDFNN_LIB", os.path.join(_HERE, "libsdfnn.so"))
@@ -106,9 +105,10 @@ def rows_of(t: torch.Tensor, align: bool = False) -> Tuple[torch.Tensor, int, in
 
 
 def aligned(t: torch.Tensor) -> torch.Tensor:
-    """A contiguous tensor that starts at a 16-byte boundary (weights: a slice of a flat parameter buffer may not)."""
+    """A contiguous tensor that starts at a 16-byte boundary where the kernels read it in place (16-bit types; a slice of a flat parameter
+    buffer may not)."""
     t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t if t.element_size() == 4 or t.data_ptr() % 16 == 0 else t.clone()
 
 
 def ptr(t: Optional[torch.Tensor]):
@@ -125,14 +125,32 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+class _NotTwice(torch.autograd.Function):
+    """The gradients of a backward pass whose graph is recorded, tied to what they depend on: differentiating them is an error, not zero."""
+
+    @staticmethod
+    def forward(ctx, count, *tensors):
+        return tuple(t.detach() for t in tensors[:count])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("sdfnn operators cannot be differentiated twice: their backward pass has no derivative of its own")
+
+
 def once(backward):
-    """A backward whose results cannot be differentiated again, as torch's once_differentiable makes it - whose bookkeeping, 20 us of host time, is
-    left out where no graph of the backward is recorded."""
-    guarded = once_differentiable(backward)
+    """A backward whose results cannot be differentiated again.  torch's once_differentiable lets them pass as constants where the incoming
+    gradient is one, and costs 20 us of host time in every call; here the graph, where one is recorded, leads to an error."""
 
     @functools.wraps(backward)
     def call(ctx, *grads):
-        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        there = [t for t in out if t is not None]
+        depends = [t for t in (*ctx.saved_tensors, *grads) if isinstance(t, torch.Tensor) and t.requires_grad]
+        guarded = iter(_NotTwice.apply(len(there), *there, *depends))
+        return tuple(None if t is None else next(guarded) for t in out)
 
     return call
 

@@ -2,7 +2,11 @@
 blocks in its training form and its 8-bit serving form.
 
 The reference's MLP (field_components/mlp.py:25-100) is evaluated inside the fused field kernels; these blocks stand beside it as layers of
-their own, at widths up to thousands.  Runs on libsdfnn.so (include/sdfnn.h); no CPU path.
+their own, at widths up to thousands; NeRFField (fields/vanilla_nerf_field.py) puts a stack of them between its density and its colour head.
+Runs on libsdfnn.so (include/sdfnn.h); no CPU path.
+
+Graph capture: every call takes its workspace from the allocator, so captured calls own theirs.  As with any torch operation, a backward pass
+is captured after the eager graphs of the same leaves have been released, or with torch.autograd.grad on leaves made for the capture.
 """
 from typing import Optional
 
@@ -113,7 +117,8 @@ class GatedStack(nn.Module):
     """num_blocks pre-norm residual blocks  h <- h + mlp(norm(h))  and a last norm.  Every addition happens inside the norm that follows it.
 
     quantize() makes the 8-bit serving form: from then on a call that needs no gradient (torch.no_grad()) runs the blocks on 8-bit products,
-    with weights quantised from the parameters as they were; training calls are unaffected.  dequantize() drops it."""
+    with weights quantised from the parameters as they are now; training calls are unaffected, and parameters that change afterwards need another
+    quantize().  dequantize() drops it.  Moving the module to another device or type makes the form anew there (on the CPU: drops it)."""
 
     def __init__(self, dim: int, hidden_dim: int, num_blocks: int, activation: str = "silu", eps: float = 1e-6) -> None:
         super().__init__()
@@ -121,7 +126,7 @@ class GatedStack(nn.Module):
             raise ValueError(f"GatedStack: {num_blocks} blocks")
         self.norms = nn.ModuleList(RMSNorm(dim, eps) for _ in range(num_blocks + 1))
         self.mlps = nn.ModuleList(GatedMLP(dim, hidden_dim, dim, activation) for _ in range(num_blocks))
-        self._served = None  # not a submodule: state_dict holds the parameters alone
+        self._served = None  # a plain list, not submodules: state_dict holds the parameters alone
 
     def quantize(self) -> "GatedStack":
         self._served = [Int8GatedMLP(m) for m in self.mlps]
@@ -131,19 +136,23 @@ class GatedStack(nn.Module):
         self._served = None
         return self
 
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
+        if self._served is not None:
+            self._served = None
+            if self.mlps[0].w_gate.is_cuda:
+                self.quantize()
+        return self
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         h, delta = x, None
         serve = self._served is not None and not torch.is_grad_enabled()
         for i, norm in enumerate(self.norms[:-1]):
+            out = norm.quantized(h, delta) if serve else norm(h, delta)
+            if delta is not None:
+                h = out[-1]
             if serve:
-                out = norm.quantized(h, delta)
-                if delta is not None:
-                    h = out[2]
                 delta = self._served[i](out[0], out[1], h.dtype)
             else:
-                out = norm(h, delta)
-                y = out
-                if delta is not None:
-                    y, h = out
-                delta = self.mlps[i](y)
+                delta = self.mlps[i](out if delta is None else out[0])
         return self.norms[-1](h, delta)[0]

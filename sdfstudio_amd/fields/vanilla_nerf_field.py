@@ -22,6 +22,7 @@ import torch
 from torch import nn
 
 from sdfstudio_amd import _lib
+from sdfstudio_amd.field_components.mlp import GatedStack
 from sdfstudio_amd.fields.field_heads import FieldHeadNames
 
 
@@ -127,7 +128,11 @@ class NeRFField(nn.Module):
     def __init__(self, position_encoding: Optional[nn.Module] = None, direction_encoding: Optional[nn.Module] = None,
                  base_mlp_num_layers: int = 8, base_mlp_layer_width: int = 256, head_mlp_num_layers: int = 2,
                  head_mlp_layer_width: int = 128, skip_connections: Tuple[int, ...] = (4,), field_heads=None,
-                 use_integrated_encoding: bool = False, spatial_distortion=None) -> None:
+                 use_integrated_encoding: bool = False, spatial_distortion=None, feature_blocks: int = 0,
+                 feature_hidden_dim: Optional[int] = None) -> None:
+        """feature_blocks > 0 (not in the reference): that many pre-norm gated residual blocks (field_components/mlp.py GatedStack) on the features
+        between density and colour head; feature_hidden_dim: their hidden width (default: twice the head's).  `feature_blocks.quantize()` serves
+        them in 8 bits under torch.no_grad()."""
         super().__init__()
         # The reference's defaults are Identity encodings and an RGB head (vanilla_nerf_field.py:52-61); the surface models always pass the
         # 10- / 4-frequency encodings (base_surface_model.py:189-200), which is what the fused kernels are built for: an encoding left out
@@ -164,6 +169,7 @@ class NeRFField(nn.Module):
         expect += [(WH, 33 + WH if l == 0 else WH) for l in range(NLC)] + [(3, WH)]
         self._native = NativeBackgroundNet(cfg_c, WH, 0, expect)
         self._widths = (W, WH, NL, NLC, d0, skip)
+        self.feature_blocks = GatedStack(WH, feature_hidden_dim or 2 * WH, feature_blocks) if feature_blocks else None
 
     # ------------------------------------------------------------------ parameters in the library's layout
     def _theta(self) -> torch.Tensor:
@@ -233,6 +239,8 @@ class NeRFField(nn.Module):
         from sdfstudio_amd.fields.sdf_field import _ColorFunction
 
         part, theta, x = density_embedding
+        if self.feature_blocks is not None:
+            part = self.feature_blocks(part)
         _, d, st, _ = unpack_ray_samples(ray_samples)
         n, s = st.shape
         rgb = _ColorFunction.apply(theta, part, torch.zeros_like(x), None, self._native, x, d.contiguous(), n, s)

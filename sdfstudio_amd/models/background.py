@@ -27,7 +27,7 @@ def build_background(model, config) -> None:
         model.field_background = NeRFField(
             position_encoding=NeRFEncoding(in_dim=3, num_frequencies=10, min_freq_exp=0.0, max_freq_exp=9.0, include_input=True),
             direction_encoding=NeRFEncoding(in_dim=3, num_frequencies=4, min_freq_exp=0.0, max_freq_exp=3.0, include_input=True),
-            spatial_distortion=model.scene_contraction)
+            spatial_distortion=model.scene_contraction, feature_blocks=getattr(config, "background_feature_blocks", 0))
     elif config.background_model == "grid":
         model.field_background = TCNNNerfactoField(  # :181-187
             model.scene_box.aabb, spatial_distortion=model.scene_contraction, num_images=model.num_train_data,

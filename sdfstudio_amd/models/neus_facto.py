@@ -184,6 +184,7 @@ class NeuSFactoModelConfig:
     level_init: int = 4
     steps_per_level: int = 10_000
     eval_num_rays_per_chunk: int = 4096  # models/base_model.py:58 (the neus-facto presets set 1024, method_configs.py:476)
+    background_feature_blocks: int = 0  # not in the reference: gated residual blocks in the "mlp" background field (NeRFField.feature_blocks)
 
     def setup(self, **kwargs):
         return self._target(self, **kwargs)
