@@ -106,13 +106,14 @@ NN_D TileId tile_of(const GemmArgs<EPI>& g) {
 // lane, with the lanes side by side along the row: whole lines of every tensor the epilogue reads or writes.  What it reads of other
 // tensors (epi.fetch) is requested for several passes before the first is used; what belongs to columns (epi.cols) is read once.
 template <int NJ> struct Stage { static constexpr int stride = NJ * 128 + 16, bytes = 32 * stride; };
-template <bool DUAL, class E, int MI, int NJ, class ACC, class EPI>
-NN_D void put_tile(const ACC (&acc)[MI][NJ], const EPI& epi, const int split, const int64_t M, const int64_t m, const int n, const int lane,
+template <bool DUAL, int NJ, class EPI>
+NN_D auto put_cols(const EPI& epi, const int n, const int lane) { return epi.cols(n + (lane % (DUAL ? NJ * 2 : NJ * 4)) * 8); }
+template <bool DUAL, class E, int MI, int NJ, class ACC, class EPI, class COLS>
+NN_D void put_tile(const ACC (&acc)[MI][NJ], const EPI& epi, const COLS& cols, const int split, const int64_t M, const int64_t m, const int n, const int lane,
                    char* stage) {
   constexpr int W = DUAL ? NJ * 16 : NJ * 32, LPR = W / 8, RPP = 64 / LPR, PASSES = 32 / RPP, STRIDE = Stage<NJ>::stride;
   const int hi = lane >> 5, row = lane & 31;
   const int c = (lane % LPR) * 8, r0 = lane / LPR;
-  const auto cols = epi.cols(n + c);
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     typename EPI::Row rows[PASSES];
@@ -203,13 +204,11 @@ struct Loader {
     const int64_t at = (int64_t)(after ? kc - turn : kc) * 64;
     return rows_buffer((after ? two.p : one.p) + part * (after ? two.plane : one.plane), one.ld, one.rows, one.width, at);
   }
-  // load i of step s.  Steps behind the last one (beyond) lie out of range (buffers end below 2^31) and write zeros, so that the count of
-  // loads in flight stays the same
+  // load i of step s; beyond: out of range (buffers end below 2^31), where it writes zeros
   NN_D void issue(const i32x4 buf, const int64_t width, const int s, const bool beyond, const int i, const unsigned to) const {
     const int kc = TERMS == 1 ? s : s / TERMS;
-    unsigned o = (unsigned)beyond << 31;
-    if constexpr (KM) o |= off[i];
-    else o |= (unsigned)(kc * 128 + piece >= (int)width) << 31 | (off[i] + kc * 128);
+    unsigned o = (KM ? off[i] : off[i] + kc * 128) | (unsigned)beyond << 31;
+    if constexpr (!KM) o |= (unsigned)(kc * 128 + piece >= (int)width) << 31;  // past k
     load_lds(buf, o, to);
   }
 };
@@ -233,6 +232,9 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(const GemmA
   typedef Side<T, AK> SA;
   typedef Side<T, BK> SB;
   constexpr int MI = T / 64, LOADS = T / 32, UNIT = Unit<T>::bytes;  // blocks of a wavefront each way; its loads a unit
+  // The last two steps, which load nothing, have code of their own at T = 128, where products of a few steps are at home; at T = 256 a second
+  // copy of the loop costs registers, and their loads are out of range instead.
+  constexpr bool PEEL = T == 128;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1;
@@ -259,8 +261,8 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(const GemmA
   };
   auto issue = [&](const int s, auto second, const int i, const int unit) __attribute__((always_inline)) {
     const unsigned to = ring + unit + i * 4096;
-    if constexpr (decltype(second)::value) lb.issue(buf_b[DUAL ? i & 1 : 0], g.b[0].width, s, s >= s1, i, to);
-    else la.issue(buf_a, g.a.width, s, s >= s1, i, to);
+    if constexpr (decltype(second)::value) lb.issue(buf_b[DUAL ? i & 1 : 0], g.b[0].width, s, !PEEL && s >= s1, i, to);
+    else la.issue(buf_a, g.a.width, s, !PEEL && s >= s1, i, to);
   };
 
   typename MM::acc acc[MI][MI];
@@ -290,7 +292,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(const GemmA
 #pragma unroll
         for (int x = MI / 2; x < MI; ++x) na[x] = SA::fragment(lds, ua, fa, x, nq);
       }
-      if constexpr (NL == LOADS) issue(ls, operand, lf + 2 * i, unit);
+      if constexpr (NL > 0 && NL == LOADS) issue(ls, operand, lf + 2 * i, unit);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = MI / 2; j < MI; ++j) acc[i][j] = MM::run(b[j], a[i], acc[i][j]);
@@ -300,44 +302,56 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(const GemmA
     }
   };
   const std::integral_constant<int, 0> none{};
-  const std::integral_constant<int, LOADS / 2> some{};
-  const std::integral_constant<int, LOADS> all{};
   auto behind = [](const int unit, const int n) { return unit + n * UNIT >= kRing * UNIT ? unit + (n - kRing) * UNIT : unit + n * UNIT; };
 
+  const int lane_n = id.n0 + wn * (DUAL ? T / 4 : T / 2);
+  const auto cols = put_cols<DUAL, MI>(g.epi, lane_n, lane);  // on its way while the product is computed
   if (s0 < s1) {
 #pragma unroll
-    for (int x = 0; x < 4 * LOADS; ++x) {
-      if (x % (2 * LOADS) == 0) aim(s0 + x / (2 * LOADS));
-      if (x & LOADS) issue(s0 + x / (2 * LOADS), B, x % LOADS, (x / LOADS) * UNIT);
-      else issue(s0 + x / (2 * LOADS), A, x % LOADS, (x / LOADS) * UNIT);
+    for (int x = 0; x < 2; ++x) {
+      if (PEEL && x == 1 && s0 + 1 >= s1) break;
+      aim(s0 + x);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) issue(s0 + x, A, i, 2 * x * UNIT);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) issue(s0 + x, B, i, (2 * x + 1) * UNIT);
     }
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");  // step s0 has landed
+    if (!PEEL || s0 + 1 < s1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");  // step s0 has landed
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = 0; i < MI; ++i) a0[i] = SA::fragment(lds, 0, fa, i, 0), b0[i] = SB::fragment(lds, UNIT, fb, i, 0);
     int ua = 0;
-    for (int s = s0; s < s1; ++s) {
+    auto step = [&](const int s, auto more) __attribute__((always_inline)) {  // more: step s + 2 exists
+      constexpr bool MORE = decltype(more)::value;
+      const std::integral_constant<int, MORE ? LOADS / 2 : 0> some{};
+      const std::integral_constant<int, MORE ? LOADS : 0> all{};
       const int ub = behind(ua, 1), na = behind(ua, 2), nb = behind(ua, 3), next = behind(ua, 4);
-      aim(s + 2);
+      if constexpr (MORE) aim(s + 2);
       quarter(a0, b0, 1, ua, ub, a1, b1, some, A, s + 2, 0, next);
       quarter(a1, b1, 2, ua, ub, a0, b0, some, A, s + 2, LOADS / 2, next);
       quarter(a0, b0, 3, ua, ub, a1, b1, none, A, 0, 0, 0);
       // own loads of step s + 1 have landed (those of A of s + 2 may be under way), own reads of step s are done: after the barrier both hold
       // for every wavefront
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(MORE ? LOADS : 0) : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
-      quarter(a1, b1, 0, na, nb, a0, b0, all, B, s + 2, 0, ua);  // (the fragments behind the last step: zeros)
+      quarter(a1, b1, 0, na, nb, a0, b0, all, B, s + 2, 0, ua);  // (the fragments behind the last step are read and not used)
       ua = na;
+    };
+    int s = s0;
+    for (; s + (PEEL ? 2 : 0) < s1; ++s) step(s, std::true_type{});
+    if constexpr (PEEL) {
+      for (; s < s1; ++s) step(s, std::false_type{});
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may still be on its way into LDS
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may still be on its way into LDS
     __syncthreads();
   }
   static_assert(4 * Stage<MI>::bytes <= Unit<T>::ring, "the epilogue's pieces lie in the ring");
-  put_tile<DUAL, typename MM::el>(acc, g.epi, id.split, g.M, id.m0 + wm * (T / 2), id.n0 + wn * (DUAL ? T / 4 : T / 2), lane,
-                                  lds + wave * Stage<MI>::bytes);
+  put_tile<DUAL, typename MM::el>(acc, g.epi, cols, id.split, g.M, id.m0 + wm * (T / 2), lane_n, lane, lds + wave * Stage<MI>::bytes);
 }
 
 // ---- epilogues: one(split, m, n, v, cols, row): eight sums of row m from column n on; pair: of both projections.  n may lie beyond the
@@ -416,20 +430,20 @@ struct GatedEpi {
   NN_D void pair(int, const int64_t m, const int n, const float (&v)[8], const float (&u)[8], Nothing, Nothing) const {
     if (n >= F) return;
     float o[8];
-    if (fu) {
-      float p[8], q[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        act_both<DT != SDFNN_F32>(act, v[i], p[i], q[i]);
-        o[i] = p[i] * u[i];
-        q[i] *= u[i];
-      }
-      store8<SDFNN_F32>(fu + m * F + n, p);
+    for (int i = 0; i < 8; ++i) o[i] = v[i];
+    if (fu) {
+      float q[8];
+      act8<DT != SDFNN_F32>(act, o, q);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] *= u[i];
+      store8<SDFNN_F32>(fu + m * F + n, o);
       store8<SDFNN_F32>(fg + m * F + n, q);
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = act_only<DT != SDFNN_F32>(act, v[i]) * u[i];
+      act8<DT != SDFNN_F32>(act, o);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] *= u[i];
     if (DT == SDFNN_F32 && plane) store_parts((char*)a + (m * F + n) * 2, plane, o);
     else store8<DT>(a + m * F + n, o);
   }
@@ -481,11 +495,13 @@ struct Int8Epi {
   int N, act;
   NN_D Cols cols(const int n) const {
     Cols c;
+    const int left = N - n < 0 ? 0 : N - n;
+    const float* t = su ? su : bias;
+    load8_n<SDFNN_F32>(sw + n, left, c.s);
+    if (t) load8_n<SDFNN_F32>(t + n, left, c.t);
+    else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int k = n + i < N ? n + i : N - 1;
-      c.s[i] = sw[k];
-      c.t[i] = su ? su[k] : bias ? bias[k] : 0.0f;
+      for (int i = 0; i < 8; ++i) c.t[i] = 0.0f;
     }
     return c;
   }
@@ -501,7 +517,10 @@ struct Int8Epi {
     if (n >= N) return;
     float o[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = act_only<DT != SDFNN_F32>(act, (float)v[i] * s * c.s[i]) * ((float)u[i] * s * c.t[i]);
+    for (int i = 0; i < 8; ++i) o[i] = (float)v[i] * s * c.s[i];
+    act8<DT != SDFNN_F32>(act, o);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] *= (float)u[i] * s * c.t[i];
     store8_n<DT>(y + m * N + n, N - n, o);
   }
 };

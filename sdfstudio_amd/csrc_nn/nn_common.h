@@ -157,13 +157,13 @@ NN_D float nn_phi(const float z) {
   return z < 0.0f ? c : 1.0f - c;
 }
 // a = act(z), d = act'(z)
-template <bool FAST>
-NN_D void act_both(const int act, const float z, float& a, float& d) {
-  if (act == SDFNN_SILU) {
+template <bool FAST, int ACT>
+NN_D void act_both(const float z, float& a, float& d) {
+  if constexpr (ACT == SDFNN_SILU) {
     const float s = nn_recip<FAST>(1.0f + nn_exp<FAST>(-z));
     a = z * s;
     d = s * (1.0f + z * (1.0f - s));
-  } else if (act == SDFNN_GELU) {
+  } else if constexpr (ACT == SDFNN_GELU) {
     const float phi = nn_phi<FAST>(z);
     a = z * phi;
     d = fmaf(z * 0.39894228040143267794f, nn_exp<FAST>(-0.5f * z * z), phi);
@@ -172,11 +172,31 @@ NN_D void act_both(const int act, const float z, float& a, float& d) {
     d = z > 0.0f ? 1.0f : 0.0f;
   }
 }
+// of eight values: one branch on the activation for all of them
+template <bool FAST, int ACT>
+NN_D void act8_of(float (&z)[8], float (&d)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) act_both<FAST, ACT>(z[i], z[i], d[i]);
+}
 template <bool FAST>
-NN_D float act_only(const int act, const float z) {
-  float a, d;
-  act_both<FAST>(act, z, a, d);  // (what the derivative alone needs is dropped by the compiler)
-  return a;
+NN_D void act8(const int act, float (&z)[8], float (&d)[8]) {
+  if (act == SDFNN_SILU) act8_of<FAST, SDFNN_SILU>(z, d);
+  else if (act == SDFNN_GELU) act8_of<FAST, SDFNN_GELU>(z, d);
+  else act8_of<FAST, SDFNN_RELU>(z, d);
+}
+template <bool FAST, int ACT>
+NN_D void act8_of(float (&z)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float d;
+    act_both<FAST, ACT>(z[i], z[i], d);  // (what the derivative alone needs is dropped by the compiler)
+  }
+}
+template <bool FAST>
+NN_D void act8(const int act, float (&z)[8]) {
+  if (act == SDFNN_SILU) act8_of<FAST, SDFNN_SILU>(z);
+  else if (act == SDFNN_GELU) act8_of<FAST, SDFNN_GELU>(z);
+  else act8_of<FAST, SDFNN_RELU>(z);
 }
 
 // ---- host side
