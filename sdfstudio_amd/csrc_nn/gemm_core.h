@@ -418,7 +418,7 @@ struct StoreEpi {
 // (error against 64 bits at 8192 x 4096 x 16384 bf16: 0.0031 of the gradients' size, 0.0024 this way, 0.0017 their own last rounding).
 template <int DT>
 struct GatedEpi {
-  static constexpr int kCost = DT == SDFNN_F32 ? 500 : 400;
+  static constexpr int kCost = DT == SDFNN_F32 ? 370 : 300;
   static constexpr int kUnroll = 1;
   typedef Nothing Row;
   elem_t<DT>* a;
@@ -486,7 +486,7 @@ struct GatedBwdEpi {
 
 template <int DT>
 struct Int8Epi {
-  static constexpr int kCost = 250;  // (one for all result types: the workspace query does not know it)
+  static constexpr int kCost = 190;  // (one for all result types: the workspace query does not know it)
   static constexpr int kUnroll = 8;
   struct Cols { float s[8], t[8]; };  // scales of the columns; t: of the second projection, or the bias
   typedef float Row;

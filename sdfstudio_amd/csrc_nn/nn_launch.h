@@ -31,9 +31,9 @@ struct Tiling {
 };
 // Which of the two tile sizes (gemm_core.h), and how often k is split: the smallest estimate of
 //   256: rounds of workgroups x (steps x 1.3 us + 5 us + the epilogue)
-//   128: rounds of pairs    x (max(steps x 1.08 us, two epilogues) + 3 us): one's epilogue runs under the other's steps
+//   128: rounds of pairs    x (max(steps x 1.15 us, two epilogues) + 3 us): one's epilogue runs under the other's steps
 // and, where k is split, the join of the raw sums.  Both sides measured (us, 256 / 128): 8192 x 4096 x 16384 bf16, plain store 800 / 1105;
-// 524288 x 512 x 256 fp32 with the gated backward's epilogue 1845 / 1490; 524288 x 1024 x 256 int8 gated 886 / 650.
+// 524288 x 512 x 256 fp32 with the gated backward's epilogue 1900 / 1443, 524288 x 1024 x 256 with the forward's 1935 / 2140; the same int8 630 / 506.
 inline Tiling choose_tiling(const int64_t M, const int64_t N, const int nk, const int terms, const int cost) {
   Tiling best = {};
   double best_us = 1e30;
@@ -45,7 +45,7 @@ inline Tiling choose_tiling(const int64_t M, const int64_t N, const int nk, cons
     for (int s = 1; s <= most; s = s < 4 ? s + 1 : s + s / 4) {
       const int per = (int)ceil_div(std::max(steps, 1), s);
       const double epilogue = 65536e-6 * (s == 1 ? cost : PartialEpi::kCost);
-      const double one = tile == 256 ? per * 1.3 + 5.0 + epilogue : std::max(per * 1.08, epilogue / 2) + 3.0;
+      const double one = tile == 256 ? per * 1.3 + 5.0 + epilogue : std::max(per * 1.15, epilogue / 2) + 3.0;
       const double join = s == 1 ? 0.0 : 6.0 + (double)(s + 1) * (double)M * (double)N * 4.0 / 3e6;
       const double us = (double)ceil_div(tiles * s, slots) * one + join;
       if (us < best_us) best_us = us, best = {tile, (int)gm, (int)gn, (int)ceil_div(std::max(steps, 1), per), per};
