@@ -121,7 +121,7 @@ int int8_operand(Call& c, const int8_t* p, const int64_t ld, const int64_t rows,
 template <int DT, bool DUAL>
 int int8_products(Call& c, const int8_t* q, const int64_t ldq, const int8_t* w0, const int64_t ld0, const int8_t* w1, const int64_t ld1,
                   const int64_t rows, const int64_t n, const int64_t k, const Int8Epi<DT>& epi) {
-  if (rows <= kSkinnyRows) {
+  if (rows <= few_rows(2)) {
     const Operand a{(const char*)q, ldq, 0, rows, k}, b0{(const char*)w0, ld0, 0, n, k}, b1{(const char*)w1, ld1, 0, n, k};
     return skinny<2, DUAL>(c, a, b0, b1, rows, n, n, epi);
   }
@@ -142,7 +142,7 @@ int check_int8(const char* what, const int8_t* q, const int64_t ldq, const int8_
   NN_REQUIRE(k >= 1 && k <= 131072, "%s: k = %lld: the 32-bit sum is exact for 1 .. 131072", what, (long long)k);
   NN_REQUIRE(q && w0 && w1, "%s: null tensor", what);
   NN_REQUIRE(ldq >= k && ld0 >= k && ld1 >= k, "%s: a row stride is smaller than the row", what);
-  if (rows > kSkinnyRows && k % 16 == 0)
+  if (rows > few_rows(2) && k % 16 == 0)
     NN_REQUIRE(aligned16(q, ldq) && aligned16(w0, ld0) && aligned16(w1, ld1),
                "%s: with k a multiple of 16 rows have to start at 16-byte boundaries", what);
   return 0;
@@ -180,7 +180,7 @@ struct Saved {
   char* a;
   int64_t plane;
   Saved(void* p, const int64_t M, const int64_t Fp) : fu((float*)p), fg(fu + M * Fp), a((char*)(fg + M * Fp)), plane(parts(M) ? M * Fp * 2 : 0) {}
-  static bool parts(const int64_t M) { return Kind<DT>::f32 && M > kSkinnyRows; }
+  static bool parts(const int64_t M) { return Kind<DT>::f32 && M > few_rows(Kind<DT>::few); }
   static int64_t a_size(const int64_t M, const int64_t Fp) { return M * Fp * (parts(M) ? 6 : Kind<DT>::es); }
   static int64_t size(const int64_t M, const int64_t Fp) { return M * Fp * 8 + a_size(M, Fp); }
 };
@@ -195,7 +195,7 @@ int gated_forward(Call& c, const void* x, const int64_t ldx, const void* wg, con
   if (!saved) sv.fu = sv.fg = nullptr, sv.a = c.take(Saved<DT>::a_size(M, Fp));
   const GatedEpi<DT> ge{(T*)sv.a, sv.plane, sv.fu, sv.fg, (int)Fp, act};
   const StoreEpi<DT> se{(T*)y, nullptr, M, M, 0, O, (int)O};
-  if (M <= kSkinnyRows) {
+  if (M <= few_rows(K::few)) {
     const Operand xo{(const char*)x, ldx * es, 0, M, D * es}, g{(const char*)wg, D * es, 0, F, D * es}, u{(const char*)wu, D * es, 0, F, D * es};
     const Operand ao{sv.a, Fp * es, 0, M, F * es}, d{(const char*)wd, F * es, 0, O, F * es};
     NN_TRY((skinny<K::few, true>(c, xo, g, u, M, F, Fp, ge)));
@@ -397,7 +397,7 @@ int sdfnn_gated_forward(const void* x, int64_t ldx, const void* w_gate, const vo
   NN_REQUIRE(x && w_gate && w_up && w_down && y, "gated_forward: null tensor");
   NN_REQUIRE(ldx >= dim, "gated_forward: a row stride is smaller than the row");
   const int64_t es = elem_size(dtype);
-  if (rows > kSkinnyRows && es == 2) {
+  if (rows > few_rows(0) && es == 2) {
     NN_REQUIRE(dim % 8 || (aligned16(x, ldx * es) && aligned16(w_gate, 0) && aligned16(w_up, 0)),
                "gated_forward: with dim a multiple of 8 rows have to start at 16-byte boundaries");
     NN_REQUIRE(hidden % 8 || aligned16(w_down, 0), "gated_forward: with hidden a multiple of 8 w_down has to start at a 16-byte boundary");

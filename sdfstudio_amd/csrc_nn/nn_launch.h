@@ -100,16 +100,19 @@ int product(Call& c, const Operand& a, const Operand& b0, const Operand& b1, con
   return 0;
 }
 
-constexpr int64_t kSkinnyRows = 32;
+// Rows up to which a product streams its weights (skinny_kernels.h).  fp32, whose tiles first have to split the weights into parts, stays with it
+// longer: 64 x 4096 -> 2 x 16384 -> 4096 takes 714 us on tiles.
+constexpr int64_t few_rows(const int kind) { return kind == 3 ? 64 : 32; }
 
-// the same for at most kSkinnyRows rows.  cols: columns that the epilogue writes (>= N)
+// the same for at most few_rows(KIND) rows.  cols: columns that the epilogue writes (>= N)
 template <int KIND, bool DUAL, class EPI>
 int skinny(Call& c, const Operand& a, const Operand& b0, const Operand& b1, const int64_t M, const int64_t N, const int64_t cols, const EPI& epi) {
   if (c.dry() || M == 0 || N == 0) return 0;
   GemmArgs<EPI> g{a, {b0, b1}, M, (int)N, 0, 0, 0, 0, 0, 0, epi};
   const dim3 grid((unsigned)ceil_div(cols, 16)), block(kSkinnyWaves * 64);
   if (M <= 16) hipLaunchKernelGGL((skinny_kernel<KIND, 1, DUAL, EPI>), grid, block, 0, c.stream, g);
-  else hipLaunchKernelGGL((skinny_kernel<KIND, 2, DUAL, EPI>), grid, block, 0, c.stream, g);
+  else if (M <= 32) hipLaunchKernelGGL((skinny_kernel<KIND, 2, DUAL, EPI>), grid, block, 0, c.stream, g);
+  else if constexpr (few_rows(KIND) > 32) hipLaunchKernelGGL((skinny_kernel<KIND, 4, DUAL, EPI>), grid, block, 0, c.stream, g);
   NN_LAUNCHED("product of few rows");
   return 0;
 }

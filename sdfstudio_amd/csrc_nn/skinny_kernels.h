@@ -1,4 +1,4 @@
-// sdfnn — products of few rows (one token, a handful of rays): y[m, n] = sum_k x[m, k] w[n, k] for m <= 32.
+// sdfnn — products of few rows (one token, a handful of rays): y[m, n] = sum_k x[m, k] w[n, k] for m <= 32 (fp32: 64).
 //
 // Bound by reading the weights once.  They go from HBM straight into the operand registers of the matrix instruction (nothing is read twice,
 // so LDS would only add a trip): a wavefront owns 16 rows of w (DUAL: 16 of each projection), a lane 16 bytes of one row at a time; the
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void skinny_kernel(const GemmArg
       for (int r = 0; r < 4; ++r) part[wave][p * MT + i][r][lane] = acc[p][i][r];
   __syncthreads();
   // a lane (grp, col) of a wavefront holds rows n = 4 grp + r of column m = col; a thread joins the eight sums of 8 consecutive n
-  if (threadIdx.x < MT * 32) {
+  if (threadIdx.x < MT * 32) {  // (MT <= 4: 128 of 512 threads)
     const int i = threadIdx.x >> 5, half = (threadIdx.x >> 4) & 1, c = threadIdx.x & 15;
     const int64_t m = i * 16 + c;
     typename S_::el v[NP][8];
