@@ -109,27 +109,19 @@ int norm_backward(NormArgs a, elem_t<DT>* dw, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------------------------- 8-bit products
-// an operand that the tiles read where it lies, or its copy with rows of whole steps
-int int8_operand(Call& c, const int8_t* p, const int64_t ld, const int64_t rows, const int64_t k, const bool direct, Operand& o) {
-  if (direct) {
-    o = {(const char*)p, ld, 0, rows, k};
-    return 0;
-  }
-  return pack_rows<1>(c, p, ld, rows, k, round_up(k, 128), o);
-}
-
 template <int DT, bool DUAL>
 int int8_products(Call& c, const int8_t* q, const int64_t ldq, const int8_t* w0, const int64_t ld0, const int8_t* w1, const int64_t ld1,
                   const int64_t rows, const int64_t n, const int64_t k, const Int8Epi<DT>& epi) {
-  if (rows <= few_rows(2)) {
-    const Operand a{(const char*)q, ldq, 0, rows, k}, b0{(const char*)w0, ld0, 0, n, k}, b1{(const char*)w1, ld1, 0, n, k};
-    return skinny<2, DUAL>(c, a, b0, b1, rows, n, n, epi);
+  Operand a{(const char*)q, ldq, 0, rows, k}, b0{(const char*)w0, ld0, 0, n, k}, b1{(const char*)w1, ld1, 0, n, k};
+  if (rows <= few_rows(2)) return skinny<2, DUAL>(c, a, b0, b1, rows, n, n, epi);
+  if (k % 16) {  // the tiles read 16 bytes at a time
+    Packs<1> packs;
+    const int64_t pad = round_up(k, 128);
+    a = packs.add(c, q, ldq, rows, k, pad);
+    b0 = packs.add(c, w0, ld0, n, k, pad);
+    if (DUAL) b1 = packs.add(c, w1, ld1, n, k, pad);
+    NN_TRY(packs.launch(c));
   }
-  const bool direct = k % 16 == 0;
-  Operand a{}, b0{}, b1{};
-  NN_TRY(int8_operand(c, q, ldq, rows, k, direct, a));
-  NN_TRY(int8_operand(c, w0, ld0, n, k, direct, b0));
-  if (DUAL) NN_TRY(int8_operand(c, w1, ld1, n, k, direct, b1));
   const int64_t nk = ceil_div(k, 128);
   return product<2, 1, DUAL, kRows>(c, a, b0, b1, rows, n, nk, nk, epi);
 }
@@ -164,12 +156,9 @@ template <int DT> struct Kind {  // of the tile and of the few-row product
 
 // [rows, cols] where it lies if the tiles can read it there (16-bit rows of a multiple of 8), else a copy with rows of whole steps
 template <int DT>
-int operand(Call& c, const void* p, const int64_t ld, const int64_t rows, const int64_t cols, Operand& o) {
-  if (!Kind<DT>::f32 && cols % 8 == 0) {
-    o = {(const char*)p, ld * 2, 0, rows, cols * 2};
-    return 0;
-  }
-  return pack_rows<Kind<DT>::es>(c, p, ld, rows, cols, round_up(cols, 64), o);
+Operand operand(Call& c, Packs<Kind<DT>::es>& packs, const void* p, const int64_t ld, const int64_t rows, const int64_t cols) {
+  if (!Kind<DT>::f32 && cols % 8 == 0) return {(const char*)p, ld * 2, 0, rows, cols * 2};
+  return packs.add(c, p, ld, rows, cols, round_up(cols, 64));
 }
 
 // what a forward pass keeps: fu, fg [rows][Fp] fp32 (GatedEpi), then a [rows][Fp]: 16-bit types and few rows of fp32 as it is, else as the
@@ -201,13 +190,12 @@ int gated_forward(Call& c, const void* x, const int64_t ldx, const void* wg, con
     NN_TRY((skinny<K::few, true>(c, xo, g, u, M, F, Fp, ge)));
     return skinny<K::few, false>(c, ao, d, d, M, O, O, se);
   }
-  Operand xo, g, u, d;
-  NN_TRY(operand<DT>(c, x, ldx, M, D, xo));
-  NN_TRY(operand<DT>(c, wg, D, F, D, g));
-  NN_TRY(operand<DT>(c, wu, D, F, D, u));
+  Packs<K::es> packs;
+  const Operand xo = operand<DT>(c, packs, x, ldx, M, D), g = operand<DT>(c, packs, wg, D, F, D), u = operand<DT>(c, packs, wu, D, F, D);
+  const Operand d = operand<DT>(c, packs, wd, F, O, F);
+  NN_TRY(packs.launch(c));
   const int64_t nd = ceil_div(D, 64), nf = Fp / 64;
   NN_TRY((product<K::tile, K::terms, true, kRows>(c, xo, g, u, M, F, nd, nd, ge)));
-  NN_TRY(operand<DT>(c, wd, F, O, F, d));
   const Operand ao{sv.a, Fp * 2, sv.plane, M, Fp * 2};
   return product<K::tile, K::terms, false, kRows>(c, ao, d, d, M, O, nf, nf, se);
 }
@@ -224,37 +212,38 @@ int gated_backward(Call& c, const void* x, const int64_t ldx, const void* wg, co
   const int64_t dplane = M * 2 * Fp * 2;
   const Operand dgu{c.take((K::f32 ? 3 : 1) * dplane), 2 * Fp * 2, dplane, M, 2 * Fp * 2};
   const int64_t nm = ceil_div(M, 64), nf = Fp / 64;
-  Operand dyo;
-  NN_TRY(operand<DT>(c, dy, lddy, M, O, dyo));
-  const int64_t start = c.used;  // the operands of one product make room for those of the next
+  Packs<K::es> packs;
+  const Operand dyo = operand<DT>(c, packs, dy, lddy, M, O);
+  Operand d{}, g{}, u{}, xo{}, a{sv.a, Fp * 2, sv.plane, M, Fp * 2};
+  if (dx || dwg) d = operand<DT>(c, packs, wd, F, O, F);
+  if (dx) g = operand<DT>(c, packs, wg, D, F, D), u = operand<DT>(c, packs, wu, D, F, D);
+  if (dwg) xo = operand<DT>(c, packs, x, ldx, M, D);
+  NN_TRY(packs.launch(c));
+  if (dwd && K::f32 && !Saved<DT>::parts(M)) {
+    Packs<K::es> few;
+    a = few.add(c, sv.a, Fp, M, Fp, Fp);
+    NN_TRY(few.launch(c));
+  }
+  const int64_t start = c.used;  // the split sums of one product make room for those of the next
   int64_t most = start;
   auto next = [&]() { most = std::max(most, c.used), c.used = start; };
   if (dx || dwg) {
-    Operand w;
-    NN_TRY(operand<DT>(c, wd, F, O, F, w));
     const GatedBwdEpi<DT> be{sv.fu, sv.fg, const_cast<char*>(dgu.p), dgu.plane, (int)Fp};
     const int64_t no = ceil_div(O, 64);
-    NN_TRY((product<K::tile, K::terms, false, kRowsDown>(c, dyo, w, w, M, F, no, no, be)));
+    NN_TRY((product<K::tile, K::terms, false, kRowsDown>(c, dyo, d, d, M, F, no, no, be)));
     next();
   }
   if (dx) {
-    Operand g, u;
-    NN_TRY(operand<DT>(c, wg, D, F, D, g));
-    NN_TRY(operand<DT>(c, wu, D, F, D, u));
     const StoreEpi<DT> se{(T*)dx, nullptr, M, M, 0, D, (int)D};
     NN_TRY((product<K::tile, K::terms, false, kRowsDown>(c, dgu, g, u, M, D, 2 * nf, nf, se)));
     next();
   }
   if (dwd) {
-    Operand a{sv.a, Fp * 2, sv.plane, M, Fp * 2};
-    if (K::f32 && !Saved<DT>::parts(M)) NN_TRY(pack_rows<4>(c, sv.a, Fp, M, Fp, Fp, a));
     const StoreEpi<DT> se{(T*)dwd, nullptr, O, O, 0, F, (int)F};
     NN_TRY((product<K::tile, K::terms, false, kDown>(c, dyo, a, a, O, F, nm, nm, se)));
     next();
   }
   if (dwg) {
-    Operand xo;
-    NN_TRY(operand<DT>(c, x, ldx, M, D, xo));
     const StoreEpi<DT> se{(T*)dwg, (T*)dwu, Fp, F, F, D, (int)D};
     NN_TRY((product<K::tile, K::terms, false, kDown>(c, dgu, xo, xo, 2 * Fp, D, nm, nm, se)));
     next();

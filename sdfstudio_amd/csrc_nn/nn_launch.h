@@ -117,15 +117,26 @@ int skinny(Call& c, const Operand& a, const Operand& b0, const Operand& b1, cons
   return 0;
 }
 
-// a copy of src with rows of whole steps.  ES: bytes of an element (4: three bf16 parts)
+// Copies of operands with rows of whole steps, gathered and made in one launch.  ES: bytes of an element (4: three bf16 parts)
 template <int ES>
-int pack_rows(Call& c, const void* src, const int64_t ld, const int64_t rows, const int64_t cols, const int64_t pad, Operand& o) {
-  const int64_t es = ES == 1 ? 1 : 2, plane = rows * pad * 2;
-  char* dst = c.take(ES == 4 ? 3 * plane : rows * pad * es);
-  o = {dst, pad * es, plane, rows, pad * es};
-  if (c.dry() || rows == 0 || pad == 0) return 0;
-  const PackArgs a{src, ld, rows, cols, dst, pad, plane, pad};
-  hipLaunchKernelGGL((pack_rows_kernel<ES>), dim3((unsigned)ceil_div(rows * (pad / 8), 256)), dim3(256), 0, c.stream, a);
-  NN_LAUNCHED("operand copy");
-  return 0;
-}
+struct Packs {
+  PackBatch b{};
+  int64_t blocks = 0;
+  Operand add(Call& c, const void* src, const int64_t ld, const int64_t rows, const int64_t cols, const int64_t pad) {
+    const int64_t es = ES == 1 ? 1 : 2, plane = rows * pad * 2;
+    char* dst = c.take(ES == 4 ? 3 * plane : rows * pad * es);
+    if (rows > 0 && pad > 0) {
+      b.a[b.count] = {src, ld, rows, cols, dst, pad, plane, pad};
+      b.first[b.count++] = (unsigned)blocks;
+      blocks += ceil_div(rows * (pad / 8), 256);
+    }
+    return {dst, pad * es, plane, rows, pad * es};
+  }
+  int launch(Call& c) {
+    if (c.dry() || b.count == 0) return 0;
+    NN_REQUIRE(blocks < 0x7fffffff, "operands of more than 2^42 elements");
+    hipLaunchKernelGGL((pack_rows_kernel<ES>), dim3((unsigned)blocks), dim3(256), 0, c.stream, b);
+    NN_LAUNCHED("operand copy");
+    return 0;
+  }
+};

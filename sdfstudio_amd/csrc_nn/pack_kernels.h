@@ -13,10 +13,23 @@ struct PackArgs {
   int64_t pad;        // columns of dst that are written (>= cols), a multiple of 64
 };
 
-// rows as they are: one thread 8 elements.  ES: bytes of an element (4: fp32 into parts)
+// What a call needs copied, in one launch: matrix k has the workgroups [first[k], first[k + 1])
+constexpr int kPacks = 5;
+struct PackBatch {
+  PackArgs a[kPacks];
+  unsigned first[kPacks + 1];
+  int count;
+};
+
+// one thread 8 elements.  ES: bytes of an element (4: fp32 into parts)
 template <int ES>
-__global__ __launch_bounds__(256) void pack_rows_kernel(const PackArgs a) {
-  const int64_t groups = a.pad / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void pack_rows_kernel(const PackBatch b) {
+  int k = 0;
+#pragma unroll
+  for (int j = 1; j < kPacks; ++j)
+    if (j < b.count && blockIdx.x >= b.first[j]) k = j;
+  const PackArgs& a = b.a[k];
+  const int64_t groups = a.pad / 8, i = (int64_t)(blockIdx.x - b.first[k]) * 256 + threadIdx.x;
   if (i >= groups * a.rows) return;
   const int64_t row = i / groups, c = (i - row * groups) * 8;
   const int64_t left = a.cols - c;
