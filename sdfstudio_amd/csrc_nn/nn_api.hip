@@ -45,8 +45,7 @@ void pick_row(const int64_t dim, F&& f, W&& wide) {
 }
 // rows that a workgroup of that shape takes at a time
 constexpr int64_t rows_at_once(const int tpr, const int u) { return (tpr > 256 ? 1 : 256 / tpr) * u; }
-// workgroups that walk the rows of a forward pass: no more than are resident at the kernels' registers (four of 256 threads a CU and up)
-int64_t row_groups(const int64_t rows, const int tpr, const int u) { return std::min<int64_t>(ceil_div(rows, rows_at_once(tpr, u)), 256 * 8); }
+dim3 row_grid(const int64_t rows, const int tpr, const int u) { return dim3((unsigned)ceil_div(rows, rows_at_once(tpr, u))); }
 
 int check_norm(const char* what, const void* x, const int64_t ldx, const void* residual, const int64_t ldr, const int32_t dtype,
                const int64_t rows, const int64_t dim) {
@@ -63,8 +62,8 @@ template <int DT>
 int norm_forward(const NormArgs& a, hipStream_t s) {
   pick_row(a.dim, [&](auto tpr, auto nv, auto u) {
     NN_ROW_SHAPE;
-    hipLaunchKernelGGL((rms_norm_fwd_kernel<DT, TPR, NV, U>), dim3((unsigned)row_groups(a.rows, TPR, U)), dim3(256), 0, s, a);
-  }, [&] { hipLaunchKernelGGL((rms_norm_fwd_wide_kernel<DT>), dim3((unsigned)row_groups(a.rows, kWide, 1)), dim3(kWide), 0, s, a); });
+    hipLaunchKernelGGL((rms_norm_fwd_kernel<DT, TPR, NV, U>), row_grid(a.rows, TPR, U), dim3(256), 0, s, a);
+  }, [&] { hipLaunchKernelGGL((rms_norm_fwd_wide_kernel<DT>), row_grid(a.rows, kWide, 1), dim3(kWide), 0, s, a); });
   NN_LAUNCHED("rms_norm_forward");
   return 0;
 }
@@ -72,8 +71,10 @@ template <int DT>
 int norm_quantize(const NormArgs& a, hipStream_t s) {
   pick_row(a.dim, [&](auto tpr, auto nv, auto u) {
     NN_ROW_SHAPE;
-    hipLaunchKernelGGL((rms_norm_quant_kernel<DT, TPR, NV, U>), dim3((unsigned)row_groups(a.rows, TPR, U)), dim3(256), 0, s, a);
-  }, [&] { hipLaunchKernelGGL((rms_norm_quant_wide_kernel<DT>), dim3((unsigned)row_groups(a.rows, kWide, 1)), dim3(kWide), 0, s, a); });
+    const dim3 grid = row_grid(a.rows, TPR, U), block(256);
+    if (!a.w && !a.r) hipLaunchKernelGGL((rms_norm_quant_kernel<DT, TPR, NV, U, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((rms_norm_quant_kernel<DT, TPR, NV, U, false>), grid, block, 0, s, a);
+  }, [&] { hipLaunchKernelGGL((rms_norm_quant_wide_kernel<DT>), row_grid(a.rows, kWide, 1), dim3(kWide), 0, s, a); });
   NN_LAUNCHED("rms_norm_quantize");
   return 0;
 }
@@ -93,11 +94,10 @@ int norm_backward(NormArgs a, elem_t<DT>* dw, hipStream_t s) {
   if (a.rows > 0)
     pick_row(a.dim, [&](auto tpr, auto nv, auto u) {
       NN_ROW_SHAPE;
-      const dim3 grid((unsigned)groups), block(256);
-      if (dw) hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, TPR, NV, U, true>), grid, block, 0, s, a);
-      else hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, TPR, NV, U, false>), grid, block, 0, s, a);
+      if (dw) hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, TPR, NV, U, true>), dim3((unsigned)groups), dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, TPR, NV, U, false>), row_grid(a.rows, TPR, U), dim3(256), 0, s, a);
     }, [&] {
-      if (a.dx) hipLaunchKernelGGL((rms_norm_bwd_wide_kernel<DT>), dim3((unsigned)row_groups(a.rows, kWide, 1)), dim3(kWide), 0, s, a);
+      if (a.dx) hipLaunchKernelGGL((rms_norm_bwd_wide_kernel<DT>), row_grid(a.rows, kWide, 1), dim3(kWide), 0, s, a);
       if (dw) hipLaunchKernelGGL((rms_norm_dw_wide_kernel<DT>), dim3((unsigned)ceil_div(a.dim, 256), (unsigned)groups), dim3(256), 0, s, a);
     });
   NN_LAUNCHED("rms_norm_backward");

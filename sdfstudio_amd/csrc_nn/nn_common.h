@@ -66,11 +66,15 @@ template <int DT>
 NN_D void load8_n(const elem_t<DT>* p, const int n, float (&v)[8]) { widen8<DT>(raw8_n<DT>(p, n), v); }
 template <int DT>
 NN_D void store8(elem_t<DT>* p, const float (&v)[8]) {
-  elem_t<DT> t[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = (elem_t<DT>)v[i];
   Raw8<DT> raw;
-  __builtin_memcpy(&raw, t, sizeof(t));
+  if constexpr (DT == SDFNN_F32) {
+    __builtin_memcpy(&raw, v, 32);
+  } else {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef elem_t<DT> e2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw.w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{v[2 * i], v[2 * i + 1]}), e2));
+  }
   *reinterpret_cast<Raw8<DT>*>(p) = raw;
 }
 template <int DT>
@@ -130,7 +134,7 @@ NN_D float nn_phi(const float z) {
   const float x = fabsf(z);
   float p, c;
   if constexpr (FAST) {
-    const float y = fminf(x, 5.0f);
+    const float y = __builtin_amdgcn_fmed3f(x, 0.0f, 5.0f);
     p = -2.92766572e-07f;
     p = fmaf(p, y, 4.06725712e-06f);
     p = fmaf(p, y, 1.34747179e-05f);

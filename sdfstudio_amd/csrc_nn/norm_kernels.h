@@ -9,9 +9,10 @@
 // the stored one is rounded to the type.
 //
 // Eight to 64 lanes a row up to 2048 elements (no barrier and no LDS: the sums are joined by lane permutations), U rows of narrow ones at a
-// time; a workgroup of 256 threads a row above.  Workgroups walk the rows and keep the weight in registers.  (The next rows' loads under way
-// while these are worked on: no faster, the other wavefronts cover them.)  Rows beyond 8192 elements go through kernels of their own
-// that read them twice (the second time from L2).  bf16, 524288 x 256 with a residual: forward 202 us = 5.3 TB/s, backward 265 us = 5.1 TB/s.
+// time; a workgroup of 256 threads a row above.  Every workgroup of a forward pass takes its rows once: a loop over rows saves the loads of the weight
+// but waits for its own stores before the next rows' loads arrive (the counter of both is one), 202 us where the launch below takes 177.  The backward
+// pass has to walk: it keeps the sums of dw.  Rows beyond 8192 elements go through kernels of their own that read them twice (the second time
+// from L2).  bf16, 524288 x 256 with a residual: forward 177 us = 6.1 TB/s, backward 259 us = 5.2 TB/s; fp16 to codes 89 us = 4.5 TB/s.
 #pragma once
 #include "nn_common.h"
 
@@ -111,14 +112,13 @@ NN_D void load_h(const elem_t<DT>* x, const elem_t<DT>* r, const int64_t c, cons
   }
 }
 
-// Walks the rows: load(row, u) fetches a row into registers, work(first) handles U of them.  GRP rows of threads a workgroup.
-template <int U, int GRP, class LOAD, class WORK>
-NN_D void walk_rows(const int64_t rows, const int sub, LOAD&& load, WORK&& work) {
-  for (int64_t first = ((int64_t)blockIdx.x * GRP + sub) * U; first < rows; first += (int64_t)gridDim.x * GRP * U) {
+// U rows from `first` on: load(row, u) fetches a row into registers, work(first) handles them
+template <int U, class LOAD, class WORK>
+NN_D void take_rows(const int64_t rows, const int64_t first, LOAD&& load, WORK&& work) {
+  if (first >= rows) return;
 #pragma unroll
-    for (int u = 0; u < U; ++u) load(first + u < rows ? first + u : rows - 1, u);
-    work(first);
-  }
+  for (int u = 0; u < U; ++u) load(first + u < rows ? first + u : rows - 1, u);
+  work(first);
 }
 
 // ---- forward.  TPR threads a row, GRP rows of them a workgroup, U such rows at a time
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(256) void rms_norm_fwd_kernel(const NormArgs a) {
   const T *x = (const T*)a.x, *r = (const T*)a.r, *w = (const T*)a.w;
   Raw8<DT> wr[NV], xr[U][NV], rr[U][NV];
   row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t c, const int n) { wr[i] = raw8_n<DT>(w + c, n); });
-  walk_rows<U, GRP>(a.rows, threadIdx.x / TPR, [&](const int64_t row, const int u) {
+  take_rows<U>(a.rows, ((int64_t)blockIdx.x * GRP + threadIdx.x / TPR) * U, [&](const int64_t row, const int u) {
     row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t c, const int n) {
       xr[u][i] = raw8_n<DT>(x + row * a.ldx + c, n);
       if (r) rr[u][i] = raw8_n<DT>(r + row * a.ldr + c, n);
@@ -174,33 +174,33 @@ template <int DT>
 __global__ __launch_bounds__(kWide) void rms_norm_fwd_wide_kernel(const NormArgs a) {
   typedef elem_t<DT> T;
   __shared__ float lds[16];
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T *x = (const T*)a.x + row * a.ldx, *r = a.r ? (const T*)a.r + row * a.ldr : nullptr;
-    float ss = 0.0f;
-    wide_loop(a.dim, [&](const int64_t c, const int n) {
-      float h[8];
-      load_h<DT>(x, r, c, n, h);
-      if (a.h) store8_n<DT>((T*)a.h + row * a.dim + c, n, h);
+  const int64_t row = blockIdx.x;
+  const T *x = (const T*)a.x + row * a.ldx, *r = a.r ? (const T*)a.r + row * a.ldr : nullptr;
+  float ss = 0.0f;
+  wide_loop(a.dim, [&](const int64_t c, const int n) {
+    float h[8];
+    load_h<DT>(x, r, c, n, h);
+    if (a.h) store8_n<DT>((T*)a.h + row * a.dim + c, n, h);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(h[e], h[e], ss);
-    });
-    const float inv = 1.0f / sqrtf(row_join<kWide>(ss, AddF{}, lds) / (float)a.dim + a.eps);
-    if (threadIdx.x == 0 && a.inv) a.inv[row] = inv;
-    wide_loop(a.dim, [&](const int64_t c, const int n) {
-      float h[8], o[8];
-      load_h<DT>(x, r, c, n, h);
-      load8_n<DT>((const T*)a.w + c, n, o);
+    for (int e = 0; e < 8; ++e) ss = fmaf(h[e], h[e], ss);
+  });
+  const float inv = 1.0f / sqrtf(row_join<kWide>(ss, AddF{}, lds) / (float)a.dim + a.eps);
+  if (threadIdx.x == 0 && a.inv) a.inv[row] = inv;
+  wide_loop(a.dim, [&](const int64_t c, const int n) {
+    float h[8], o[8];
+    load_h<DT>(x, r, c, n, h);
+    load8_n<DT>((const T*)a.w + c, n, o);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] *= h[e] * inv;
-      store8_n<DT>((T*)a.y + row * a.dim + c, n, o);
-    });
-  }
+    for (int e = 0; e < 8; ++e) o[e] *= h[e] * inv;
+    store8_n<DT>((T*)a.y + row * a.dim + c, n, o);
+  });
 }
 
-// ---- 8-bit output.  The code of v is round(127 v / top) with v = (x + r) w and top = max|v| exact.  In fp32 the quotient is off by at most six
-// half steps of 127 (4.6e-5), so only a value within 5e-5 of the border between two codes - one in ten thousand - can go wrong: a row that
-// holds one finds its largest magnitude in 64 bits (among the few values next to the largest in fp32) and decides such values there.  Ties
-// exist (half the largest value is one) and are decided by the quotient of exact numbers, so that they go to even.
+// ---- 8-bit output.  The code of v is round(127 v / top) with v = (x + r) w and top = max|v| exact.  In fp32 the quotient is off by two half steps
+// (7.6e-6 each, of 127), two more where there is a residual and two more where there is a weight, so only a value that close to the border between
+// two codes - one in ten thousand - can go wrong: a row that holds one finds its largest magnitude in 64 bits (among the few values next to the
+// largest in fp32; without residual and weight it is known) and decides such values there, each alone.  Ties exist (half the largest value is
+// one) and are decided by the quotient of exact numbers, so that they go to even.
 NN_D int code_of(const double v, const double top) {
   double c = __builtin_rint(v * 127.0 / top);
   c = c > 127.0 ? 127.0 : c;
@@ -243,6 +243,16 @@ struct Eight {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = ((double)a[e] + (double)b[e]) * (double)k[e];
   }
+  // the codes of those among v that fp32 cannot decide
+  NN_D void decide(const bool has_r, const bool has_w, const float (&v)[8], const float per, const float edge, const double top, int (&q)[8]) const {
+    double d[8];
+    exact(has_r, has_w, d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float k = v[e] * per;
+      if (!(fabsf(k - __builtin_rintf(k)) <= edge)) q[e] = code_of(d[e], top);
+    }
+  }
 };
 NN_D void largest(const float (&v)[8], uint32_t& big) {
 #pragma unroll
@@ -251,11 +261,12 @@ NN_D void largest(const float (&v)[8], uint32_t& big) {
     big = b > big ? b : big;
   }
 }
-// the largest magnitude exactly: the fp32 values are off by two half steps (2^-23), so it is among those from top (1 - 2^-21) on
+// the largest magnitude exactly: the fp32 values are off by two half steps (2^-23, or some of the smallest steps there are), so it is among those
+// from top (1 - 2^-21) on
 NN_D void largest_exact(const float (&v)[8], const double (&d)[8], const float top, unsigned long long& big) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    if (fabsf(v[e]) < top * (1.0f - 0x1p-21f)) continue;
+    if (fabsf(v[e]) < top * (1.0f - 0x1p-21f) - 0x1p-146f) continue;
     const unsigned long long b = (unsigned long long)__double_as_longlong(d[e]) & 0x7fffffffffffffffull;
     big = b > big ? b : big;
   }
@@ -268,10 +279,6 @@ NN_D void codes8(const float (&v)[8], const float per, int (&q)[8], float& off) 
     off = fmaxf(off, fabsf(k - z));
     q[e] = (int)z;
   }
-}
-NN_D void codes8_exact(const double (&d)[8], const double top, int (&q)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) q[e] = code_of(d[e], top);
 }
 NN_D void store_codes(int8_t* out, const int n, const int (&q)[8]) {
   if (n >= 8) {
@@ -289,12 +296,17 @@ NN_D void store_codes(int8_t* out, const int n, const int (&q)[8]) {
 // 127 / top (0: a row of zeros, or one that is not finite: codes 0), and how far from its code a value may lie for fp32 to decide (where 127 / top
 // may overflow: nowhere)
 NN_D float codes_per(const float top) { return top > 0.0f && top < INFINITY ? 127.0f / top : 0.0f; }
-NN_D float codes_edge(const float top) { return top > 0.0f && top < 1e-30f ? -1.0f : 0.49995f; }
+NN_D float codes_edge(const float top, const NormArgs& a) {
+  return top > 0.0f && top < 1e-30f ? -1.0f : 0.5f - 2e-5f - (a.r ? 1.55e-5f : 0.0f) - (a.w ? 1.55e-5f : 0.0f);
+}
+// inv in fp32 as the forward pass has it (every wavefront computes a row's scale in one lane: 64-bit roots and quotients took as long as the codes)
 NN_D float scale_of(const float top, const float ss, const NormArgs& a) {
-  return (float)((double)top / 127.0 * (a.w ? 1.0 / sqrt((double)ss / (double)a.dim + (double)a.eps) : 1.0));
+  if (!a.w) return top / 127.0f;
+  return (float)((double)top * (double)(1.0f / sqrtf(ss / (float)a.dim + a.eps)) * (1.0 / 127.0));
 }
 
-template <int DT, int TPR, int NV, int U>
+// PLAIN: neither weight nor residual
+template <int DT, int TPR, int NV, int U, bool PLAIN>
 __global__ __launch_bounds__(256) void rms_norm_quant_kernel(const NormArgs a) {
   typedef elem_t<DT> T;
   constexpr int GRP = 256 / TPR;
@@ -302,14 +314,14 @@ __global__ __launch_bounds__(256) void rms_norm_quant_kernel(const NormArgs a) {
   __shared__ uint32_t ldsb[16];
   __shared__ unsigned long long ldsd[16];
   const int t = threadIdx.x % TPR;
-  const T *x = (const T*)a.x, *r = (const T*)a.r, *w = (const T*)a.w;
+  const T *x = (const T*)a.x, *r = PLAIN ? nullptr : (const T*)a.r, *w = PLAIN ? nullptr : (const T*)a.w;
   Raw8<DT> wr[NV];
   Eight<DT> in[U][NV];
   if (w) row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t c, const int n) { wr[i] = raw8_n<DT>(w + c, n); });
-  walk_rows<U, GRP>(a.rows, threadIdx.x / TPR, [&](const int64_t row, const int u) {
+  take_rows<U>(a.rows, ((int64_t)blockIdx.x * GRP + threadIdx.x / TPR) * U, [&](const int64_t row, const int u) {
     row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t c, const int n) {
       in[u][i].load(x + row * a.ldx, r ? r + row * a.ldr : nullptr, nullptr, c, n);
-      in[u][i].w = wr[i];
+      if (!PLAIN) in[u][i].w = wr[i];
     });
   }, [&](const int64_t first) {
     float v[U][NV][8], ss[U];
@@ -319,7 +331,7 @@ __global__ __launch_bounds__(256) void rms_norm_quant_kernel(const NormArgs a) {
       ss[u] = 0.0f, big[u] = 0;
       row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t c, const int n) {
         in[u][i].sum(r != nullptr, v[u][i]);
-        if (a.h && first + u < a.rows) store8_n<DT>((T*)a.h + (first + u) * a.dim + c, n, v[u][i]);
+        if (!PLAIN && a.h && first + u < a.rows) store8_n<DT>((T*)a.h + (first + u) * a.dim + c, n, v[u][i]);
         if (w) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) ss[u] = fmaf(v[u][i][e], v[u][i][e], ss[u]);
@@ -335,25 +347,23 @@ __global__ __launch_bounds__(256) void rms_norm_quant_kernel(const NormArgs a) {
       int q[NV][8];
       float off = 0.0f;
       row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t, const int) { codes8(v[u][i], per, q[i], off); });
-      off = row_join<TPR>(off, MaxF{}, ldso);
-      if (off > codes_edge(top)) {  // (all threads of the row alike)
-        unsigned long long b = 0;
-        row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t, const int) {
-          double d[8];
-          in[u][i].exact(r != nullptr, w != nullptr, d);
-          largest_exact(v[u][i], d, top, b);
-        });
-        const double exact = __longlong_as_double((long long)row_join<TPR>(b, MaxBits{}, ldsd));
-        row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t, const int) {
-          float mine = 0.0f;
-          int z[8];
-          codes8(v[u][i], per, z, mine);
-          if (mine <= codes_edge(top)) return;
-          double d[8];
-          in[u][i].exact(r != nullptr, w != nullptr, d);
-          codes8_exact(d, exact, q[i]);
-        });
+      const float edge = codes_edge(top, a);
+      double exact = top;
+      if (r || w) {
+        if (row_join<TPR>(off, MaxF{}, ldso) > edge) {  // (all threads of the row alike)
+          unsigned long long b = 0;
+          row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t, const int) {
+            double d[8];
+            in[u][i].exact(r != nullptr, w != nullptr, d);
+            largest_exact(v[u][i], d, top, b);
+          });
+          exact = __longlong_as_double((long long)row_join<TPR>(b, MaxBits{}, ldsd));
+        }
       }
+      if (off > edge)
+        row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t, const int) {
+          in[u][i].decide(r != nullptr, w != nullptr, v[u][i], per, edge, exact, q[i]);
+        });
       const int64_t row = first + u;
       if (row >= a.rows) continue;  // (U > 1: the threads of a row leave together, and no barrier follows)
       if (t == 0) a.scales[row] = scale_of(top, sum, a);
@@ -368,28 +378,31 @@ __global__ __launch_bounds__(kWide) void rms_norm_quant_wide_kernel(const NormAr
   __shared__ uint32_t ldsb[16];
   __shared__ unsigned long long ldsd[16];
   const bool has_r = a.r != nullptr, has_w = a.w != nullptr;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T *x = (const T*)a.x + row * a.ldx, *r = has_r ? (const T*)a.r + row * a.ldr : nullptr, *w = (const T*)a.w;
-    auto take = [&](const int64_t c, const int n, Eight<DT>& in, float (&h)[8], float (&v)[8]) {
-      in.load(x, r, w, c, n);
-      in.sum(has_r, h);
+  const int64_t row = blockIdx.x;
+  const T *x = (const T*)a.x + row * a.ldx, *r = has_r ? (const T*)a.r + row * a.ldr : nullptr, *w = (const T*)a.w;
+  auto take = [&](const int64_t c, const int n, Eight<DT>& in, float (&h)[8], float (&v)[8]) {
+    in.load(x, r, w, c, n);
+    in.sum(has_r, h);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = h[e];
-      in.values(has_w, v);
-    };
-    float ss = 0.0f;
-    uint32_t big = 0;
-    wide_loop(a.dim, [&](const int64_t c, const int n) {
-      Eight<DT> in;
-      float h[8], v[8];
-      take(c, n, in, h, v);
+    for (int e = 0; e < 8; ++e) v[e] = h[e];
+    in.values(has_w, v);
+  };
+  float ss = 0.0f;
+  uint32_t big = 0;
+  wide_loop(a.dim, [&](const int64_t c, const int n) {
+    Eight<DT> in;
+    float h[8], v[8];
+    take(c, n, in, h, v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(h[e], h[e], ss);
-      largest(v, big);
-      if (a.h) store8_n<DT>((T*)a.h + row * a.dim + c, n, h);
-    });
-    ss = row_join<kWide>(ss, AddF{}, ldss);
-    const float top = __builtin_bit_cast(float, row_join<kWide>(big, MaxBits{}, ldsb)), per = codes_per(top);
+    for (int e = 0; e < 8; ++e) ss = fmaf(h[e], h[e], ss);
+    largest(v, big);
+    if (a.h) store8_n<DT>((T*)a.h + row * a.dim + c, n, h);
+  });
+  ss = row_join<kWide>(ss, AddF{}, ldss);
+  const float top = __builtin_bit_cast(float, row_join<kWide>(big, MaxBits{}, ldsb)), per = codes_per(top);
+  const float edge = codes_edge(top, a);
+  double exact = top;
+  if (has_r || has_w) {
     unsigned long long b = 0;
     wide_loop(a.dim, [&](const int64_t c, const int n) {
       Eight<DT> in;
@@ -399,22 +412,18 @@ __global__ __launch_bounds__(kWide) void rms_norm_quant_wide_kernel(const NormAr
       in.exact(has_r, has_w, d);
       largest_exact(v, d, top, b);
     });
-    const double exact = __longlong_as_double((long long)row_join<kWide>(b, MaxBits{}, ldsd));
-    if (threadIdx.x == 0) a.scales[row] = scale_of(top, ss, a);
-    wide_loop(a.dim, [&](const int64_t c, const int n) {
-      Eight<DT> in;
-      float h[8], v[8], off = 0.0f;
-      int q[8];
-      take(c, n, in, h, v);
-      codes8(v, per, q, off);
-      if (off > codes_edge(top)) {
-        double d[8];
-        in.exact(has_r, has_w, d);
-        codes8_exact(d, exact, q);
-      }
-      store_codes(a.q + row * a.dim + c, n, q);
-    });
+    exact = __longlong_as_double((long long)row_join<kWide>(b, MaxBits{}, ldsd));
   }
+  if (threadIdx.x == 0) a.scales[row] = scale_of(top, ss, a);
+  wide_loop(a.dim, [&](const int64_t c, const int n) {
+    Eight<DT> in;
+    float h[8], v[8], off = 0.0f;
+    int q[8];
+    take(c, n, in, h, v);
+    codes8(v, per, q, off);
+    if (off > edge) in.decide(has_r, has_w, v, per, edge, exact, q);
+    store_codes(a.q + row * a.dim + c, n, q);
+  });
 }
 
 // ---- backward.  The workgroups walk the rows and keep their threads' columns of dw in registers; their partial sums are added in a fixed order by the
@@ -432,56 +441,57 @@ __global__ __launch_bounds__(256) void rms_norm_bwd_kernel(const NormArgs a) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) fill8(dw[i], 0.0f);
   row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t c, const int n) { wr[i] = raw8_n<DT>(w + c, n); });
-  walk_rows<U, GRP>(a.rows, sub, [&](const int64_t row, const int u) {
-    inv[u] = a.inv[row];
-    row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t c, const int n) {
-      xr[u][i] = raw8_n<DT>(x + row * a.ldx + c, n);
-      if (r) rr[u][i] = raw8_n<DT>(r + row * a.ldr + c, n);
-      if (dy) yr[u][i] = raw8_n<DT>(dy + row * a.lddy + c, n);
-      if (dh) hr[u][i] = raw8_n<DT>(dh + row * a.lddh + c, n);
-    });
-  }, [&](const int64_t first) {
-    float nn[U][NV][8], g[U][NV][8], un[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      un[u] = 0.0f;
-      const bool there = first + u < a.rows;
-      row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t, const int) {
-        float b[8], k[8];
-        widen8<DT>(xr[u][i], nn[u][i]);
-        if (r) {
-          widen8<DT>(rr[u][i], b);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) nn[u][i][e] += b[e];
-        }
-        if (dy) widen8<DT>(yr[u][i], g[u][i]);
-        else fill8(g[u][i], 0.0f);
-        widen8<DT>(wr[i], k);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          nn[u][i][e] *= inv[u];
-          if constexpr (DW) dw[i][e] = fmaf(there ? g[u][i][e] : 0.0f, nn[u][i][e], dw[i][e]);
-          g[u][i][e] *= k[e];
-          un[u] = fmaf(g[u][i][e], nn[u][i][e], un[u]);
-        }
-      });
-    }
-    if (!a.dx) return;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const float mean = row_join<TPR>(un[u], AddF{}, lds) / (float)a.dim;
-      const int64_t row = first + u;
-      if (row >= a.rows) continue;  // (U > 1: the threads of a row leave together, and no barrier follows)
+  for (int64_t at = ((int64_t)blockIdx.x * GRP + sub) * U; at < a.rows; at += (int64_t)gridDim.x * GRP * U)
+    take_rows<U>(a.rows, at, [&](const int64_t row, const int u) {
+      inv[u] = a.inv[row];
       row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t c, const int n) {
-        float d[8];
-        if (dh) widen8<DT>(hr[u][i], d);
-        else fill8(d, 0.0f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = fmaf(inv[u], g[u][i][e] - nn[u][i][e] * mean, d[e]);
-        store8_n<DT>((T*)a.dx + row * a.dim + c, n, d);
+        xr[u][i] = raw8_n<DT>(x + row * a.ldx + c, n);
+        if (r) rr[u][i] = raw8_n<DT>(r + row * a.ldr + c, n);
+        if (dy) yr[u][i] = raw8_n<DT>(dy + row * a.lddy + c, n);
+        if (dh) hr[u][i] = raw8_n<DT>(dh + row * a.lddh + c, n);
       });
-    }
-  });
+    }, [&](const int64_t first) {
+      float nn[U][NV][8], g[U][NV][8], un[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        un[u] = 0.0f;
+        const bool there = first + u < a.rows;
+        row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t, const int) {
+          float b[8], k[8];
+          widen8<DT>(xr[u][i], nn[u][i]);
+          if (r) {
+            widen8<DT>(rr[u][i], b);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) nn[u][i][e] += b[e];
+          }
+          if (dy) widen8<DT>(yr[u][i], g[u][i]);
+          else fill8(g[u][i], 0.0f);
+          widen8<DT>(wr[i], k);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            nn[u][i][e] *= inv[u];
+            if constexpr (DW) dw[i][e] = fmaf(there ? g[u][i][e] : 0.0f, nn[u][i][e], dw[i][e]);
+            g[u][i][e] *= k[e];
+            un[u] = fmaf(g[u][i][e], nn[u][i][e], un[u]);
+          }
+        });
+      }
+      if (!a.dx) return;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float mean = row_join<TPR>(un[u], AddF{}, lds) / (float)a.dim;
+        const int64_t row = first + u;
+        if (row >= a.rows) continue;  // (U > 1: the threads of a row leave together, and no barrier follows)
+        row_loop<TPR, NV>(a.dim, t, [&](const int i, const int64_t c, const int n) {
+          float d[8];
+          if (dh) widen8<DT>(hr[u][i], d);
+          else fill8(d, 0.0f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[e] = fmaf(inv[u], g[u][i][e] - nn[u][i][e] * mean, d[e]);
+          store8_n<DT>((T*)a.dx + row * a.dim + c, n, d);
+        });
+      }
+    });
   if constexpr (DW) {
     float* out = a.partial + (int64_t)blockIdx.x * a.dim;
 #pragma unroll
@@ -513,36 +523,35 @@ template <int DT>
 __global__ __launch_bounds__(kWide) void rms_norm_bwd_wide_kernel(const NormArgs a) {
   typedef elem_t<DT> T;
   __shared__ float lds[16];
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T *x = (const T*)a.x + row * a.ldx, *r = a.r ? (const T*)a.r + row * a.ldr : nullptr;
-    const float inv = a.inv[row];
-    auto load = [&](const int64_t c, const int n, float (&nn)[8], float (&u)[8]) {
-      float k[8];
-      load_h<DT>(x, r, c, n, nn);
-      if (a.dy) load8_n<DT>((const T*)a.dy + row * a.lddy + c, n, u);
-      else fill8(u, 0.0f);
-      load8_n<DT>((const T*)a.w + c, n, k);
+  const int64_t row = blockIdx.x;
+  const T *x = (const T*)a.x + row * a.ldx, *r = a.r ? (const T*)a.r + row * a.ldr : nullptr;
+  const float inv = a.inv[row];
+  auto load = [&](const int64_t c, const int n, float (&nn)[8], float (&u)[8]) {
+    float k[8];
+    load_h<DT>(x, r, c, n, nn);
+    if (a.dy) load8_n<DT>((const T*)a.dy + row * a.lddy + c, n, u);
+    else fill8(u, 0.0f);
+    load8_n<DT>((const T*)a.w + c, n, k);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) nn[e] *= inv, u[e] *= k[e];
-    };
-    float un = 0.0f;
-    wide_loop(a.dim, [&](const int64_t c, const int n) {
-      float nn[8], u[8];
-      load(c, n, nn, u);
+    for (int e = 0; e < 8; ++e) nn[e] *= inv, u[e] *= k[e];
+  };
+  float un = 0.0f;
+  wide_loop(a.dim, [&](const int64_t c, const int n) {
+    float nn[8], u[8];
+    load(c, n, nn, u);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) un = fmaf(u[e], nn[e], un);
-    });
-    const float mean = row_join<kWide>(un, AddF{}, lds) / (float)a.dim;
-    wide_loop(a.dim, [&](const int64_t c, const int n) {
-      float nn[8], u[8], d[8];
-      load(c, n, nn, u);
-      if (a.dh) load8_n<DT>((const T*)a.dh + row * a.lddh + c, n, d);
-      else fill8(d, 0.0f);
+    for (int e = 0; e < 8; ++e) un = fmaf(u[e], nn[e], un);
+  });
+  const float mean = row_join<kWide>(un, AddF{}, lds) / (float)a.dim;
+  wide_loop(a.dim, [&](const int64_t c, const int n) {
+    float nn[8], u[8], d[8];
+    load(c, n, nn, u);
+    if (a.dh) load8_n<DT>((const T*)a.dh + row * a.lddh + c, n, d);
+    else fill8(d, 0.0f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d[e] = fmaf(inv, u[e] - nn[e] * mean, d[e]);
-      store8_n<DT>((T*)a.dx + row * a.dim + c, n, d);
-    });
-  }
+    for (int e = 0; e < 8; ++e) d[e] = fmaf(inv, u[e] - nn[e] * mean, d[e]);
+    store8_n<DT>((T*)a.dx + row * a.dim + c, n, d);
+  });
 }
 
 // rows too wide for the registers of a workgroup: dw by columns.  One thread a column, the rows split over blockIdx.y
