@@ -11,8 +11,9 @@
  * uses atomics: results do not change from run to run.
  *
  * Matrices are row-major; a row stride (ld*, in elements) may exceed the row's width, elements of a row are adjacent.  Tensors need their
- * element's alignment only (16-byte aligned rows are read without a copy).  Rows beyond the last one and the gap between rows of an
- * output are left as they were.
+ * element's alignment; where a product of more than 32 rows (or a backward pass) reads its operands in place - 16-bit rows of a multiple of
+ * 8 elements, codes of a multiple of 16 - every row has to start at a 16-byte boundary, else the call is refused.  Rows of 8 MiB and more
+ * are refused there too.  Outputs are contiguous; what lies behind their last row is left as it was.
  */
 #ifndef SDFNN_H_
 #define SDFNN_H_
@@ -65,9 +66,12 @@ int sdfnn_int8_gated_linear(const int8_t* q, int64_t ldq, const float* sq, const
 /* ---- gated MLP
  * g = x Wg^T, u = x Wu^T, a = act(g) u, y = a Wd^T.  x [rows, dim] (stride ldx), w_gate / w_up [hidden, dim], w_down [out, hidden], all
  * contiguous, y [rows, out] contiguous.  16-bit types: products of those types with fp32 sums; a is rounded to the type before the second
- * product.  fp32: every operand as three bf16 parts that hold its 24 bits, six products, fp32 sums (a non-finite input gives NaN).
- * saved: sdfnn_gated_saved_size bytes, what the backward needs (act(g) and u act'(g) in fp32, a in the type); NULL when none will follow. */
-int64_t sdfnn_gated_saved_size(int32_t dtype, int64_t rows, int64_t hidden);
+ * product, and so are the gradients of g and u before theirs (fp16: a hidden value beyond 65504 becomes infinite and gradients below 6e-8
+ * vanish, as everywhere in that type: scale the loss).  fp32: every operand as three bf16 parts that hold its 24 bits, six products, fp32
+ * sums (magnitudes below 2^-110 hold fewer bits).  A row with an input that is not finite gives NaN.
+ * saved: sdfnn_gated_saved_size bytes, what the backward needs (act(g) and u act'(g) in fp32, a in the type; fp32 above 64 rows: a and x as
+ * their three parts); NULL when none will follow. */
+int64_t sdfnn_gated_saved_size(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden);
 int64_t sdfnn_gated_workspace_size(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden, int64_t out, int32_t backward);
 int sdfnn_gated_forward(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* w_down, int32_t dtype, int32_t act,
                         int64_t rows, int64_t dim, int64_t hidden, int64_t out, void* saved, void* y, void* workspace,

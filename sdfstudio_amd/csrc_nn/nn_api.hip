@@ -156,22 +156,26 @@ template <int DT> struct Kind {  // of the tile and of the few-row product
 
 // [rows, cols] where it lies if the tiles can read it there (16-bit rows of a multiple of 8), else a copy with rows of whole steps
 template <int DT>
-Operand operand(Call& c, Packs<Kind<DT>::es>& packs, const void* p, const int64_t ld, const int64_t rows, const int64_t cols) {
+Operand operand(Call& c, Packs<Kind<DT>::es>& packs, const void* p, const int64_t ld, const int64_t rows, const int64_t cols, char* to = nullptr) {
   if (!Kind<DT>::f32 && cols % 8 == 0) return {(const char*)p, ld * 2, 0, rows, cols * 2};
-  return packs.add(c, p, ld, rows, cols, round_up(cols, 64));
+  return packs.add(c, p, ld, rows, cols, round_up(cols, 64), to);
 }
 
 // what a forward pass keeps: fu, fg [rows][Fp] fp32 (GatedEpi), then a [rows][Fp]: 16-bit types and few rows of fp32 as it is, else as the
-// three bf16 parts that the products read
+// three bf16 parts that the products read; behind them the parts of x, which the backward reads again (to split x once more takes 223 us of
+// 8.4 ms at 524288 x 256 x 512)
 template <int DT>
 struct Saved {
   float *fu, *fg;
-  char* a;
+  char *a, *x;
   int64_t plane;
-  Saved(void* p, const int64_t M, const int64_t Fp) : fu((float*)p), fg(fu + M * Fp), a((char*)(fg + M * Fp)), plane(parts(M) ? M * Fp * 2 : 0) {}
+  Saved(void* p, const int64_t M, const int64_t Fp)
+      : fu((float*)p), fg(fu + M * Fp), a((char*)(fg + M * Fp)), x(a + a_size(M, Fp)), plane(parts(M) ? M * Fp * 2 : 0) {}
   static bool parts(const int64_t M) { return Kind<DT>::f32 && M > few_rows(Kind<DT>::few); }
   static int64_t a_size(const int64_t M, const int64_t Fp) { return M * Fp * (parts(M) ? 6 : Kind<DT>::es); }
-  static int64_t size(const int64_t M, const int64_t Fp) { return M * Fp * 8 + a_size(M, Fp); }
+  static int64_t size(const int64_t M, const int64_t D, const int64_t Fp) {
+    return M * Fp * 8 + a_size(M, Fp) + (parts(M) ? M * round_up(D, 64) * 6 : 0);
+  }
 };
 
 template <int DT>
@@ -191,7 +195,7 @@ int gated_forward(Call& c, const void* x, const int64_t ldx, const void* wg, con
     return skinny<K::few, false>(c, ao, d, d, M, O, O, se);
   }
   Packs<K::es> packs;
-  const Operand xo = operand<DT>(c, packs, x, ldx, M, D), g = operand<DT>(c, packs, wg, D, F, D), u = operand<DT>(c, packs, wu, D, F, D);
+  const Operand xo = operand<DT>(c, packs, x, ldx, M, D, saved && K::f32 ? sv.x : nullptr), g = operand<DT>(c, packs, wg, D, F, D), u = operand<DT>(c, packs, wu, D, F, D);
   const Operand d = operand<DT>(c, packs, wd, F, O, F);
   NN_TRY(packs.launch(c));
   const int64_t nd = ceil_div(D, 64), nf = Fp / 64;
@@ -217,7 +221,8 @@ int gated_backward(Call& c, const void* x, const int64_t ldx, const void* wg, co
   Operand d{}, g{}, u{}, xo{}, a{sv.a, Fp * 2, sv.plane, M, Fp * 2};
   if (dx || dwg) d = operand<DT>(c, packs, wd, F, O, F);
   if (dx) g = operand<DT>(c, packs, wg, D, F, D), u = operand<DT>(c, packs, wu, D, F, D);
-  if (dwg) xo = operand<DT>(c, packs, x, ldx, M, D);
+  const int64_t Dp = round_up(D, 64);
+  if (dwg) xo = Saved<DT>::parts(M) ? Operand{sv.x, Dp * 2, M * Dp * 2, M, Dp * 2} : operand<DT>(c, packs, x, ldx, M, D);
   NN_TRY(packs.launch(c));
   if (dwd && K::f32 && !Saved<DT>::parts(M)) {
     Packs<K::es> few;
@@ -361,10 +366,10 @@ int sdfnn_int8_gated_linear(const int8_t* q, int64_t ldq, const float* sq, const
   });
 }
 
-int64_t sdfnn_gated_saved_size(int32_t dtype, int64_t rows, int64_t hidden) {
-  if (dtype < SDFNN_F32 || dtype > SDFNN_F16 || rows < 0 || rows > kMaxRows || hidden < 1 || hidden > 1 << 20) return -1;
+int64_t sdfnn_gated_saved_size(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden) {
+  if (check_gated("gated_saved_size", dtype, 0, rows, dim, hidden, 1)) return -1;
   const int64_t Fp = round_up(hidden, 64);
-  return dtype == SDFNN_F32 ? Saved<SDFNN_F32>::size(rows, Fp) : Saved<SDFNN_BF16>::size(rows, Fp);
+  return dtype == SDFNN_F32 ? Saved<SDFNN_F32>::size(rows, dim, Fp) : Saved<SDFNN_BF16>::size(rows, dim, Fp);
 }
 
 int64_t sdfnn_gated_workspace_size(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden, int64_t out, int32_t backward) {

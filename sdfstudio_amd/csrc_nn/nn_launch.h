@@ -122,9 +122,10 @@ template <int ES>
 struct Packs {
   PackBatch b{};
   int64_t blocks = 0;
-  Operand add(Call& c, const void* src, const int64_t ld, const int64_t rows, const int64_t cols, const int64_t pad) {
+  // to: where the copy goes; NULL: into the workspace
+  Operand add(Call& c, const void* src, const int64_t ld, const int64_t rows, const int64_t cols, const int64_t pad, char* to = nullptr) {
     const int64_t es = ES == 1 ? 1 : 2, plane = rows * pad * 2;
-    char* dst = c.take(ES == 4 ? 3 * plane : rows * pad * es);
+    char* dst = to ? to : c.take(ES == 4 ? 3 * plane : rows * pad * es);
     if (rows > 0 && pad > 0) {
       b.a[b.count] = {src, ld, rows, cols, dst, pad, plane, pad};
       b.first[b.count++] = (unsigned)blocks;

@@ -30,7 +30,7 @@ class _GatedMLP(torch.autograd.Function):
             wg, wu, wd = _nn.aligned(w_gate), _nn.aligned(w_up), _nn.aligned(w_down)
             dim = x.shape[-1]
             y = torch.empty((*x.shape[:-1], out), dtype=x.dtype, device=dev)
-            saved = _nn.workspace(_nn.size("sdfnn_gated_saved_size", code, rows, hidden), dev) if save else None
+            saved = _nn.workspace(_nn.size("sdfnn_gated_saved_size", code, rows, dim, hidden), dev) if save else None
             if rows:
                 size = _nn.size("sdfnn_gated_workspace_size", code, rows, dim, hidden, out, 0)
                 ws = _nn.workspace(size, dev)

@@ -96,7 +96,7 @@ def test_c_abi_refuses_bad_calls():
     refused(call(gb, ok, _7=63), "stride")
     refused(call(gb, ok, _6=P + 2), "16-byte")
     refused(call(gb, ok, _18=64), "workspace")
-    assert lib.sdfnn_gated_workspace_size(1, -1, 64, 64, 64, 0) == -1 and lib.sdfnn_gated_saved_size(7, 1, 1) == -1
+    assert lib.sdfnn_gated_workspace_size(1, -1, 64, 64, 64, 0) == -1 and lib.sdfnn_gated_saved_size(7, 1, 1, 1) == -1
     assert lib.sdfnn_int8_linear_workspace_size(1, 1, 131073, 1) == -1 and lib.sdfnn_rms_norm_backward_workspace_size(1, 0) == -1
 
 
@@ -110,8 +110,8 @@ def test_workspaces_are_sized_by_the_call():
         a = lib.sdfnn_gated_workspace_size(dt, 1000, 64, 100, 64, 0)
         assert a >= 1000 * 128 * es
         assert lib.sdfnn_gated_workspace_size(dt, 1000, 64, 100, 64, 1) >= 1000 * 256 * es
-        assert lib.sdfnn_gated_saved_size(dt, 1000, 100) == 1000 * 128 * (8 + (6 if dt == 0 else 2))
-        assert lib.sdfnn_gated_saved_size(dt, 20, 100) == 20 * 128 * (8 + es)
+        assert lib.sdfnn_gated_saved_size(dt, 1000, 60, 100) == 1000 * 128 * (8 + (6 if dt == 0 else 2)) + (1000 * 64 * 6 if dt == 0 else 0)
+        assert lib.sdfnn_gated_saved_size(dt, 20, 60, 100) == 20 * 128 * (8 + es)
 
 
 def test_cpu_tensors_are_refused():
