@@ -157,11 +157,12 @@ def build_nn(verbose: bool = True) -> str:
 
 
 def build(verbose: bool = True) -> str:
-    build_mesh(verbose)
-    build_nn(verbose)
     os.makedirs(BUILD, exist_ok=True)
     with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, min(len(SOURCES), os.cpu_count() or 1))) as ex:
+        others = [ex.submit(f, verbose) for f in (build_nn, build_mesh)]
         objs = list(ex.map(_compile, SOURCES))
+        for f in others:
+            f.result()
     stamp = os.path.join(BUILD, "link.stamp")
     key = " ".join(os.path.basename(o) for o in objs)
     prev = open(stamp).read() if os.path.exists(stamp) else ""
