@@ -383,3 +383,93 @@ def test_beyond_32_bit_offsets(device):
     assert int((grads[0].abs().sum(-1) > 0).sum()) == 5
     for g, v in zip(grads[1:], want[1:]):
         near("dw", g, v, 2.0 ** -6)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,dim", [(70001, 24), (33333, 200), (20001, 333), (3001, 1500)])
+def test_norm_of_many_rows_with_a_frozen_weight(device, dtype, rows, dim):
+    """More rows than one turn of the chip and an odd number of them; the weight has no gradient; rows that start off every boundary."""
+    from sdfstudio_amd.field_components.normalization import rms_norm, rms_norm_quantized
+
+    wide = torch.randn(rows, dim + 3, device="cuda").to(dtype)
+    x, r = wide[:, 1:1 + dim], torch.randn(rows, dim, device="cuda").to(dtype)
+    w = (1 + 0.2 * torch.randn(dim, device="cuda")).to(dtype)
+    dy, dh = torch.randn(rows, dim, device="cuda").to(dtype), torch.randn(rows, dim, device="cuda").to(dtype)
+    xl, wl = x.detach().requires_grad_(True), w.clone().requires_grad_(True)
+    (frozen,) = torch.autograd.grad(rms_norm(xl, w, residual=r), xl, (dy, dh))
+    both = torch.autograd.grad(rms_norm(xl, wl, residual=r), (xl, wl), (dy, dh))
+    assert torch.equal(frozen, both[0])
+    hd = x.double() + r.double()
+    inv = 1.0 / torch.sqrt(hd.square().mean(-1, keepdim=True) + 1e-6)
+    u, n = dy.double() * w.double(), hd * inv
+    want = inv * (u - n * (u * n).mean(-1, keepdim=True)) + dh.double()
+    # dx: half a step of the type, and eight of fp32 (inv, n, u, the mean, products and sums) on terms of up to twice the result
+    near("dx", frozen, want, torch.finfo(dtype).eps / 2 + 2.0 ** -20)
+    # dw: a sum of `rows` fp32 products in chains of at most 100 (a workgroup's turns, its rows, 32 + 32 of the parts): 100 half steps of 2^-24 on the
+    # sum of the magnitudes at the worst, a third of that (2^-19) with room for rounding either way
+    terms = dy.double() * n
+    assert ((both[1].double() - terms.sum(0)).abs() <= 2.0 ** -19 * terms.abs().sum(0) + torch.finfo(dtype).eps / 2 * terms.sum(0).abs()).all()
+    q, s, h = rms_norm_quantized(x, w, residual=r)
+    v = hd * w.double()
+    top = v.abs().amax(-1, keepdim=True)
+    assert torch.equal(q.double(), torch.round(127 * v / top))
+    near("scales", s, (top * inv / 127).squeeze(-1), 2.0 ** -21)
+    near("h", h, hd, torch.finfo(dtype).eps)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_codes_of_the_smallest_rows(device, dtype):
+    """Rows whose largest value lies among the smallest numbers of the type, where 127 over it exceeds every number: the codes are exact still."""
+    from sdfstudio_amd.field_components.quantization import quantize_rows
+
+    x = torch.randn(40, 300, device="cuda", dtype=torch.float64) * torch.logspace(-44, -34, 40, device="cuda", dtype=torch.float64)[:, None]
+    x = (x * (1e30 if dtype == F16 else 1.0)).to(dtype)
+    q, s = quantize_rows(x)
+    v = x.double()
+    top = v.abs().amax(-1, keepdim=True)
+    assert torch.equal(q.double(), torch.where(top > 0, torch.round(127 * v / torch.where(top > 0, top, 1.0)), 0.0))
+    # half a step of fp32, whose smallest is 2^-149
+    assert ((s.double() - top[:, 0] / 127).abs() <= 2.0 ** -24 * top[:, 0] / 127 + 2.0 ** -150).all()
+
+
+def test_model_with_a_background_of_blocks_trains_and_serves(device):
+    """background_feature_blocks of a surface model: one optimiser step of the method's own optimisers on flat parameters moves the blocks, and the
+    rendered image of the served form stays near the trained one (5 % as in test_stack_serves_in_8_bits; the background is a part of it)."""
+    import copy
+
+    import bench as B
+    from sdfstudio_amd.cameras.rays import RayBundle
+    from sdfstudio_amd.configs.method_configs import method_configs
+    from sdfstudio_amd.engine.optimizers import Optimizers
+    from sdfstudio_amd.models.neus_facto import SceneBox
+
+    m = method_configs["neus-facto"]
+    cfg = copy.deepcopy(m.model)
+    cfg.background_model, cfg.background_feature_blocks = "mlp", 2
+    torch.manual_seed(0)
+    model = cfg.setup(scene_box=SceneBox(aabb=torch.tensor([[-1.0, -1, -1], [1, 1, 1]]), near=0.5, far=4.5), num_train_data=49).to(device).train()
+    groups = {k: v for k, v in model.get_param_groups().items() if v}
+    opts = Optimizers({k: m.optimizers[k] for k in groups}, groups)
+    blocks = model.field_background.feature_blocks
+    before = {k: v.detach().clone() for k, v in blocks.named_parameters()}
+    gen = torch.Generator(device=device)
+    gen.manual_seed(1)
+    centers, rot = B.synthetic_cameras(device)
+    for step in range(2):
+        o, d, norm, cam = B.draw_rays(centers, rot, 256, gen)
+        bundle = RayBundle(origins=o, directions=d, directions_norm=norm, camera_indices=cam[:, None])
+        loss = model.get_loss_dict(model(bundle), {"image": torch.rand(256, 3, device=device, generator=gen)})
+        opts.zero_grad_all()
+        sum(loss.values()).backward()
+        for k, v in blocks.named_parameters():
+            assert torch.isfinite(v.grad).all() and v.grad.any(), k
+        opts.optimizer_scaler_step_all(torch.amp.GradScaler("cuda", enabled=False))
+        opts.scheduler_step_all(step)  # (the warm-up starts at a rate of zero)
+    for k, v in blocks.named_parameters():
+        assert torch.isfinite(v).all() and not torch.equal(v, before[k]), k
+    model.eval()
+    with torch.no_grad():
+        plain = model(bundle)["rgb"]
+        blocks.quantize()
+        served = model(bundle)["rgb"]
+    assert torch.isfinite(served).all() and float((served - plain).norm() / plain.norm()) < 0.05
