@@ -402,13 +402,25 @@ struct StoreEpi {
   int N;
   NN_D Nothing cols(int) const { return {}; }
   NN_D Nothing fetch(int64_t, int64_t, int) const { return {}; }
+  NN_D elem_t<DT>* row(const int64_t m) const {
+    return m < rows0 ? c0 + m * ld : m >= split_row && m < split_row + rows1 ? c1 + (m - split_row) * ld : nullptr;
+  }
   NN_D void one(int, const int64_t m, const int n, const float (&v)[8], Nothing, Nothing) const {
-    if (n >= N) return;
-    elem_t<DT>* q;
-    if (m < rows0) q = c0 + m * ld;
-    else if (m >= split_row && m < split_row + rows1) q = c1 + (m - split_row) * ld;
-    else return;
-    store8_n<DT>(q + n, N - n, v);
+    elem_t<DT>* q = row(m);
+    if (q && n < N) store8_n<DT>(q + n, N - n, v);
+  }
+  NN_D void four(const int64_t m, const int64_t n, const float (&v)[4]) const {
+    elem_t<DT>* q = row(m);
+    if (!q || n >= N) return;
+    if (n + 4 <= N) {
+      Bytes<4, 4> raw;
+      __builtin_memcpy(&raw, v, 16);
+      *reinterpret_cast<Bytes<4, 4>*>(q + n) = raw;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < N) q[n + e] = v[e];
+    }
   }
 };
 
@@ -449,7 +461,7 @@ struct GatedEpi {
   }
 };
 
-// the gradient of a in, those of g and u out: [M][2 F], dg | du (fp32: as three bf16 parts)
+// the gradient of a in, those of g and u out: [M][2 F], dg | du (fp32 with a plane: as three bf16 parts)
 template <int DT>
 struct GatedBwdEpi {
   static constexpr int kCost = DT == SDFNN_F32 ? 1250 : 750;
@@ -474,7 +486,7 @@ struct GatedBwdEpi {
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = r.p[i] * v[i], q[i] = r.q[i] * v[i];
     const int64_t at = m * 2 * F + n;
-    if constexpr (DT == SDFNN_F32) {
+    if (DT == SDFNN_F32 && plane) {
       store_parts(d + at * 2, plane, q);
       store_parts(d + (at + F) * 2, plane, p);
     } else {

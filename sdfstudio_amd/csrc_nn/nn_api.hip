@@ -204,6 +204,27 @@ int gated_forward(Call& c, const void* x, const int64_t ldx, const void* wg, con
   return product<K::tile, K::terms, false, kRows>(c, ao, d, d, M, O, nf, nf, se);
 }
 
+// up to few_rows fp32 rows: no operand is copied or split
+int gated_backward_few(Call& c, const char* x, const int64_t ldx, const char* wg, const char* wu, const char* wd, const Saved<SDFNN_F32>& sv,
+                       const char* dy, const int64_t lddy, const int64_t M, const int64_t D, const int64_t F, const int64_t O, float* dx, float* dwg,
+                       float* dwu, float* dwd) {
+  const int64_t Fp = round_up(F, 64);
+  const Operand dgu{c.take(M * Fp * 8), Fp * 8, 0, M, Fp * 8}, dyo{dy, lddy * 4, 0, M, O * 4};
+  if (dx || dwg) {
+    const Operand d{wd, F * 4, 0, O, F * 4};
+    const GatedBwdEpi<SDFNN_F32> be{sv.fu, sv.fg, const_cast<char*>(dgu.p), 0, (int)Fp};
+    NN_TRY(skinny_down(c, dyo, d, d, M, F, O, round_up(O, 16), be));
+  }
+  if (dx) {
+    const Operand g{wg, D * 4, 0, F, D * 4}, u{wu, D * 4, 0, F, D * 4};
+    const StoreEpi<SDFNN_F32> se{dx, nullptr, M, M, 0, D, (int)D};
+    NN_TRY(skinny_down(c, dgu, g, u, M, D, 2 * Fp, Fp, se));
+  }
+  if (dwd) NN_TRY(outer(c, dyo, {sv.a, Fp * 4, 0, M, F * 4}, M, O, {dwd, nullptr, O, O, 0, F, (int)F}));
+  if (dwg) NN_TRY(outer(c, dgu, {x, ldx * 4, 0, M, D * 4}, M, 2 * Fp, {dwg, dwu, Fp, F, F, D, (int)D}));
+  return 0;
+}
+
 template <int DT>
 int gated_backward(Call& c, const void* x, const int64_t ldx, const void* wg, const void* wu, const void* wd, const void* saved, const void* dy,
                    const int64_t lddy, const int64_t M, const int64_t D, const int64_t F, const int64_t O, void* dx, void* dwg, void* dwu,
@@ -212,23 +233,22 @@ int gated_backward(Call& c, const void* x, const int64_t ldx, const void* wg, co
   typedef Kind<DT> K;
   const int64_t Fp = round_up(F, 64);
   const Saved<DT> sv(const_cast<void*>(saved), M, Fp);
+  if constexpr (K::f32)
+    if (!Saved<DT>::parts(M)) return gated_backward_few(c, (const char*)x, ldx, (const char*)wg, (const char*)wu, (const char*)wd, sv, (const char*)dy, lddy, M, D, F, O, (float*)dx,
+                                                        (float*)dwg, (float*)dwu, (float*)dwd);
   // gradients of g and u, side by side
   const int64_t dplane = M * 2 * Fp * 2;
   const Operand dgu{c.take((K::f32 ? 3 : 1) * dplane), 2 * Fp * 2, dplane, M, 2 * Fp * 2};
   const int64_t nm = ceil_div(M, 64), nf = Fp / 64;
   Packs<K::es> packs;
   const Operand dyo = operand<DT>(c, packs, dy, lddy, M, O);
-  Operand d{}, g{}, u{}, xo{}, a{sv.a, Fp * 2, sv.plane, M, Fp * 2};
+  Operand d{}, g{}, u{}, xo{};
+  const Operand a{sv.a, Fp * 2, sv.plane, M, Fp * 2};
   if (dx || dwg) d = operand<DT>(c, packs, wd, F, O, F);
   if (dx) g = operand<DT>(c, packs, wg, D, F, D), u = operand<DT>(c, packs, wu, D, F, D);
   const int64_t Dp = round_up(D, 64);
   if (dwg) xo = Saved<DT>::parts(M) ? Operand{sv.x, Dp * 2, M * Dp * 2, M, Dp * 2} : operand<DT>(c, packs, x, ldx, M, D);
   NN_TRY(packs.launch(c));
-  if (dwd && K::f32 && !Saved<DT>::parts(M)) {
-    Packs<K::es> few;
-    a = few.add(c, sv.a, Fp, M, Fp, Fp);
-    NN_TRY(few.launch(c));
-  }
   const int64_t start = c.used;  // the split sums of one product make room for those of the next
   int64_t most = start;
   auto next = [&]() { most = std::max(most, c.used), c.used = start; };

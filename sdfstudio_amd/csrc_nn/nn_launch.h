@@ -101,7 +101,7 @@ int product(Call& c, const Operand& a, const Operand& b0, const Operand& b1, con
 }
 
 // Rows up to which a product streams its weights (skinny_kernels.h).  fp32, whose tiles first have to split the weights into parts, stays with it
-// longer: 64 x 4096 -> 2 x 16384 -> 4096 takes 714 us on tiles.
+// longer: 64 x 4096 -> 2 x 16384 -> 4096 takes 714 us on tiles and 391 here, its backward pass 1076 and 710 (16 rows: 1045 and 435).
 constexpr int64_t few_rows(const int kind) { return kind == 3 ? 64 : 32; }
 
 // the same for at most few_rows(KIND) rows.  cols: columns that the epilogue writes (>= N)
@@ -114,6 +114,44 @@ int skinny(Call& c, const Operand& a, const Operand& b0, const Operand& b1, cons
   else if (M <= 32) hipLaunchKernelGGL((skinny_kernel<KIND, 2, DUAL, EPI>), grid, block, 0, c.stream, g);
   else if constexpr (few_rows(KIND) > 32) hipLaunchKernelGGL((skinny_kernel<KIND, 4, DUAL, EPI>), grid, block, 0, c.stream, g);
   NN_LAUNCHED("product of few rows");
+  return 0;
+}
+
+// y[m, n] = sum_k a[m, k] b[k, n] of at most few_rows(3) fp32 rows; b1 follows b0 along k from row `turn` on, K: all rows of k
+template <class EPI>
+int skinny_down(Call& c, const Operand& a, const Operand& b0, const Operand& b1, const int64_t M, const int64_t N, const int64_t K, const int64_t turn,
+                const EPI& epi) {
+  const int64_t cols = ceil_div(N, 64), units = ceil_div(K, 16);
+  // four workgroups a CU, each with two turns of its wavefronts or more
+  const int64_t want = std::max<int64_t>(1, std::min(units / (2 * kDownWaves), 1024 / cols)), per = ceil_div(units, want), splits = ceil_div(units, per);
+  const int64_t ld = round_up(N, 64);
+  char* part = splits > 1 ? c.take(splits * M * ld * 4) : nullptr;
+  if (c.dry() || M == 0) return 0;
+  auto start = [&](const auto& e) {
+    typedef std::remove_cv_t<std::remove_reference_t<decltype(e)>> E;
+    const GemmArgs<E> g{a, {b0, b1}, M, (int)N, (int)units, (int)turn, (int)per, 0, 0, 0, e};
+    const dim3 grid((unsigned)cols, (unsigned)splits), block(kDownWaves * 64);
+    if (M <= 16) hipLaunchKernelGGL((skinny_down_kernel<1, E>), grid, block, 0, c.stream, g);
+    else if (M <= 32) hipLaunchKernelGGL((skinny_down_kernel<2, E>), grid, block, 0, c.stream, g);
+    else hipLaunchKernelGGL((skinny_down_kernel<4, E>), grid, block, 0, c.stream, g);
+  };
+  if (splits == 1) {
+    start(epi);
+    NN_LAUNCHED("product of few rows");
+    return 0;
+  }
+  start(PartialEpi{(uint32_t*)part, M, ld});
+  NN_LAUNCHED("product of few rows");
+  hipLaunchKernelGGL((split_reduce_kernel<float, false, EPI>), dim3((unsigned)ceil_div(ld / 8 * M, 256)), dim3(256), 0, c.stream, (const float*)part,
+                     (int)splits, M, ld, epi);
+  NN_LAUNCHED("split sum");
+  return 0;
+}
+// w[r, c] = sum_m p[m, r] x[m, c] of few fp32 rows into `to`; R rows r (both halves of `to` with what lies between)
+inline int outer(Call& c, const Operand& p, const Operand& x, const int64_t M, const int64_t R, const StoreEpi<SDFNN_F32>& to) {
+  if (c.dry() || R == 0) return 0;
+  hipLaunchKernelGGL(outer_kernel, dim3((unsigned)ceil_div(to.N, 256), (unsigned)ceil_div(R, 64)), dim3(256), 0, c.stream, OuterArgs{p, x, M, to});
+  NN_LAUNCHED("outer product");
   return 0;
 }
 

@@ -157,3 +157,132 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void skinny_kernel(const GemmArg
     }
   }
 }
+
+// ---- the backward pass of few fp32 rows, on the same instruction: the tiles would have to split all weights into parts first.
+// y[m, n] = sum_k x[m, k] w[k, n], the weights' k down the rows.  A workgroup owns 64 columns (256 bytes of a row), its four wavefronts take turns
+// of 16 rows: a lane loads 16 bytes of four of them, and its four elements are operands of four instructions (columns 4 c + e of instruction e), so that
+// a lane ends up with 16 consecutive columns of one m.  b[1] follows b[0] along k from row `turn` (a multiple of 16) on; g.nk, g.per: in units of 16
+// rows; where columns are few k is split over blockIdx.y.  16 x 4096 x 16384: the gradient of a 43 us (6.3 TB/s, a part
+// from the last-level cache), dx 103 us (5.2 TB/s); 64 rows, where the instructions take as long as the loads, 114 and 221 us.
+constexpr int kDownWaves = 4;
+
+template <int MT, class EPI>
+__global__ __launch_bounds__(kDownWaves * 64) void skinny_down_kernel(const GemmArgs<EPI> g) {
+  __shared__ float part[kDownWaves][MT][16][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int n0 = blockIdx.x * 64, n = n0 + col * 4;
+  const int64_t left_n = ((int64_t)g.N - n) * 4;
+  const char* x[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {  // lanes beyond the last row read the last one; their sums are not stored
+    const int64_t m = i * 16 + col < g.M ? i * 16 + col : g.M - 1;
+    x[i] = g.a.p + m * g.a.ld;
+  }
+  f32x4 acc[MT][4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[i][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 wv[2][4], xv[2][MT];
+  auto load = [&](const int s, auto set) __attribute__((always_inline)) {
+    constexpr int S = decltype(set)::value;
+    const int64_t k0 = (int64_t)s * 16;
+    const bool after = k0 >= g.turn;
+    const char* p = after ? g.b[1].p : g.b[0].p;
+    const int64_t ld = after ? g.b[1].ld : g.b[0].ld, rows = after ? g.b[1].rows : g.b[0].rows, at = k0 - (after ? g.turn : 0);
+    const int64_t k = k0 + grp * 4, row = at + grp * 4;
+    if (at + 16 <= rows && n0 + 64 <= g.N && (k0 + 16) * 4 <= g.a.width) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) wv[S][j] = __builtin_bit_cast(f32x4, load16<4>(p + (row + j) * ld + (int64_t)n * 4, 16));
+#pragma unroll
+      for (int i = 0; i < MT; ++i) xv[S][i] = __builtin_bit_cast(f32x4, load16<4>(x[i] + k * 4, 16));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        wv[S][j] = __builtin_bit_cast(f32x4, load16<4>(p + (row + j) * ld + (int64_t)n * 4, row + j < rows ? left_n : 0));
+#pragma unroll
+      for (int i = 0; i < MT; ++i) xv[S][i] = __builtin_bit_cast(f32x4, load16<4>(x[i] + k * 4, g.a.width - k * 4));
+    }
+  };
+  auto multiply = [&](auto set) __attribute__((always_inline)) {
+    constexpr int S = decltype(set)::value;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[S][j][e], xv[S][i][j], acc[i][e], 0, 0, 0);
+  };
+  const std::integral_constant<int, 0> s0{};
+  const std::integral_constant<int, 1> s1{};
+  const int first = blockIdx.y * g.per, last = first + g.per < g.nk ? first + g.per : g.nk;
+  int s = first + wave;
+  if (s < last) load(s, s0);
+  for (; s < last; s += 2 * kDownWaves) {
+    if (s + kDownWaves < last) load(s + kDownWaves, s1);
+    multiply(s0);
+    if (s + kDownWaves >= last) break;
+    if (s + 2 * kDownWaves < last) load(s + 2 * kDownWaves, s0);
+    multiply(s1);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[wave][i][4 * r + e][lane] = acc[i][e][r];
+  __syncthreads();
+  for (int id = threadIdx.x; id < MT * 128; id += kDownWaves * 64) {
+    const int i = id >> 7, half = (id >> 6) & 1, from = id & 63;
+    const int64_t m = i * 16 + (from & 15);
+    const int c = n0 + (from >> 4) * 16 + half * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kDownWaves; ++k) v[e] += part[k][i][half * 8 + e][from];
+    }
+    if (m < g.M) g.epi.one((int)blockIdx.y, m, c, v, g.epi.cols(c), g.epi.fetch(m, g.M, c));
+  }
+}
+
+// w[r, c] = sum_m p[m, r] x[m, c] of few rows m: bound by writing w.  64 x 64 results a wavefront, four wavefronts side by side along c; both operands are
+// read 16 bytes a lane (rows 4 i + a, columns 4 i + e of instruction (a, e)), so that a lane ends up with runs of four columns.  The operands are small
+// and come from L2.  16 x 4096 x 16384: 805 MB of gradients in 220 us (3.7 TB/s).
+struct OuterArgs {
+  Operand p, x;  // rows m; width: bytes of a row that exist
+  int64_t M;
+  StoreEpi<SDFNN_F32> to;
+};
+__global__ __launch_bounds__(256) void outer_kernel(const OuterArgs g) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = ((int64_t)blockIdx.x * 4 + wave) * 64;
+  const int64_t left_p = g.p.width - (r0 + col * 4) * 4, left_x = g.x.width - (c0 + col * 4) * 4;
+  const char *p = g.p.p + (r0 + col * 4) * 4, *x = g.x.p + (c0 + col * 4) * 4;
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[a][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int64_t k = 0; k < g.M; k += 4) {
+    const int64_t m = k + grp;
+    const bool there = m < g.M;
+    const f32x4 pv = __builtin_bit_cast(f32x4, load16<4>(p + m * g.p.ld, there ? left_p : 0));
+    const f32x4 xv = __builtin_bit_cast(f32x4, load16<4>(x + m * g.x.ld, there ? left_x : 0));
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[a][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[a], xv[e], acc[a][e], 0, 0, 0);
+  }
+  const int64_t c = c0 + col * 4;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const float v[4] = {acc[a][0][r], acc[a][1][r], acc[a][2][r], acc[a][3][r]};
+      g.to.four(r0 + grp * 16 + r * 4 + a, c, v);
+    }
+}

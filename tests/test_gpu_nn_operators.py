@@ -234,6 +234,7 @@ def gated_ref(x, wg, wu, wd, dy, act):
 
 
 GATED_SHAPES = [(1, 1, 1, 1), (1, 64, 128, 64), (2, 7, 13, 5), (16, 100, 40, 36), (17, 64, 64, 64), (32, 33, 65, 31), (33, 64, 128, 64), (49, 100, 70, 52), (64, 31, 129, 65), (65, 63, 127, 61),
+                (5, 700, 33, 900), (40, 90, 1500, 1003), (64, 513, 300, 257),
                 (128, 128, 256, 128), (200, 72, 136, 40), (300, 256, 512, 264), (515, 40, 24, 8), (1025, 200, 72, 300)]
 
 
