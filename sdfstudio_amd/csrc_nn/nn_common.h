@@ -64,16 +64,21 @@ template <int DT>
 NN_D void load8(const elem_t<DT>* p, float (&v)[8]) { widen8<DT>(raw8<DT>(p), v); }
 template <int DT>
 NN_D void load8_n(const elem_t<DT>* p, const int n, float (&v)[8]) { widen8<DT>(raw8_n<DT>(p, n), v); }
+// two values rounded to a 16-bit type, as one word
+template <class E>
+NN_D uint32_t pack2(const float a, const float b) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef E e2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), e2));
+}
 template <int DT>
 NN_D void store8(elem_t<DT>* p, const float (&v)[8]) {
   Raw8<DT> raw;
   if constexpr (DT == SDFNN_F32) {
     __builtin_memcpy(&raw, v, 32);
   } else {
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    typedef elem_t<DT> e2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) raw.w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{v[2 * i], v[2 * i + 1]}), e2));
+    for (int i = 0; i < 4; ++i) raw.w[i] = pack2<elem_t<DT>>(v[2 * i], v[2 * i + 1]);
   }
   *reinterpret_cast<Raw8<DT>*>(p) = raw;
 }
@@ -85,23 +90,21 @@ NN_D void store8_n(elem_t<DT>* p, const int n, const float (&v)[8]) {
     if (i < n) p[i] = (elem_t<DT>)v[i];
 }
 
-// x = p0 + p1 + p2, each a bf16.  The largest finite values round to infinity as bf16: they are cut instead.  A value that is not finite is
-// its first part alone.
-NN_D void split3(const float x, uint16_t& p0, uint16_t& p1, uint16_t& p2) {
-  const uint32_t bits = __builtin_bit_cast(uint32_t, x);
-  uint16_t h = __builtin_bit_cast(uint16_t, (__bf16)x);
-  const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
-  if ((h & 0x7fffu) == 0x7f80u && finite) h = (uint16_t)(bits >> 16);
-  const float r = finite ? x - __builtin_bit_cast(float, (uint32_t)h << 16) : 0.0f;
-  p0 = h;
-  p1 = __builtin_bit_cast(uint16_t, (__bf16)r);
-  p2 = __builtin_bit_cast(uint16_t, (__bf16)(r - __builtin_bit_cast(float, (uint32_t)p1 << 16)));
-}
-// eight values as their three parts, `plane` bytes apart
+// x = p0 + p1 + p2, each a bf16, of eight values: three rows of 16 bytes, `plane` bytes apart.  The largest finite values would round to infinity as
+// bf16: p0 is held at the largest bf16, the rest goes to p1.  Of a value that is not finite p2 at least is NaN.
 NN_D void store_parts(char* p, const int64_t plane, const float (&v)[8]) {
-  alignas(16) uint16_t h[3][8];
+  uint32_t h[3][4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) split3(v[e], h[0][e], h[1][e], h[2][e]);
+  for (int i = 0; i < 4; ++i) {
+    constexpr float top = 0x1.fep127f;
+    float a = v[2 * i], b = v[2 * i + 1];
+    h[0][i] = pack2<__bf16>(__builtin_amdgcn_fmed3f(a, -top, top), __builtin_amdgcn_fmed3f(b, -top, top));
+#pragma unroll
+    for (int k = 1; k < 3; ++k) {
+      a -= __builtin_bit_cast(float, h[k - 1][i] << 16), b -= __builtin_bit_cast(float, h[k - 1][i] & 0xffff0000u);
+      h[k][i] = pack2<__bf16>(a, b);
+    }
+  }
 #pragma unroll
   for (int k = 0; k < 3; ++k) *(uint4*)(p + k * plane) = *(const uint4*)h[k];
 }
