@@ -33,7 +33,8 @@ struct Tiling {
 //   256: rounds of workgroups x (steps x 1.3 us + 5 us + the epilogue)
 //   128: rounds of pairs    x (max(steps x 1.15 us, two epilogues) + 3 us): one's epilogue runs under the other's steps
 // and, where k is split, the join of the raw sums.  Both sides measured (us, 256 / 128): 8192 x 4096 x 16384 bf16, plain store 800 / 1105;
-// 524288 x 512 x 256 fp32 with the gated backward's epilogue 1810 / 1450, 524288 x 1024 x 256 with the forward's 2020 / 2180; the same int8 600 / 460.
+// 524288 x 512 x 256 fp32 with the gated backward's epilogue 1420 / 1420 (bound by HBM), 524288 x 1024 x 256 with the forward's 1950 / 2120; the same
+// int8 600 / 460.
 inline Tiling choose_tiling(const int64_t M, const int64_t N, const int nk, const int terms, const int cost) {
   Tiling best = {};
   double best_us = 1e30;
