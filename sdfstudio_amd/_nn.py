@@ -125,6 +125,12 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def differentiated(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a call on these is recorded for a backward pass.  (Inside an autograd function it cannot be told: its needs_input_grad does not
+    know about torch.no_grad().)"""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _NotTwice(torch.autograd.Function):
     """The gradients of a backward pass whose graph is recorded, tied to what they depend on: differentiating them is an error, not zero."""
 

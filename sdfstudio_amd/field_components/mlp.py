@@ -18,26 +18,30 @@ from sdfstudio_amd.field_components.normalization import RMSNorm
 from sdfstudio_amd.field_components.quantization import Int8Linear, int8_gated_linear, quantize_rows
 
 
+def _forward(x, w_gate, w_up, w_down, act, save):
+    """y, and with `save` what a backward pass reads (else None)."""
+    lib, code = _nn.load(), _nn.dtype_code(x, "gated_mlp")
+    dev = _nn.on_device("gated_mlp", x, w_gate, w_up, w_down)
+    hidden, out = w_gate.shape[0], w_down.shape[0]
+    with _nn.on(dev) as cur:
+        x2, px, rows, ldx = _nn.rows_of(x, align=True)
+        wg, wu, wd = _nn.aligned(w_gate), _nn.aligned(w_up), _nn.aligned(w_down)
+        dim = x.shape[-1]
+        y = torch.empty((*x.shape[:-1], out), dtype=x.dtype, device=dev)
+        saved = _nn.workspace(_nn.size("sdfnn_gated_saved_size", code, rows, dim, hidden), dev) if save else None
+        if rows:
+            size = _nn.size("sdfnn_gated_workspace_size", code, rows, dim, hidden, out, 0)
+            ws = _nn.workspace(size, dev)
+            _nn.check(lib.sdfnn_gated_forward(px, ldx, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), code, act, rows, dim, hidden, out,
+                                              _nn.ptr(saved), y.data_ptr(), ws.data_ptr(), size, cur.stream), "sdfnn_gated_forward")
+    return y, saved
+
+
 class _GatedMLP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, act):
-        lib, code = _nn.load(), _nn.dtype_code(x, "gated_mlp")
-        dev = _nn.on_device("gated_mlp", x, w_gate, w_up, w_down)
-        hidden, out = w_gate.shape[0], w_down.shape[0]
-        save = any(ctx.needs_input_grad)
-        with _nn.on(dev) as cur:
-            x2, px, rows, ldx = _nn.rows_of(x, align=True)
-            wg, wu, wd = _nn.aligned(w_gate), _nn.aligned(w_up), _nn.aligned(w_down)
-            dim = x.shape[-1]
-            y = torch.empty((*x.shape[:-1], out), dtype=x.dtype, device=dev)
-            saved = _nn.workspace(_nn.size("sdfnn_gated_saved_size", code, rows, dim, hidden), dev) if save else None
-            if rows:
-                size = _nn.size("sdfnn_gated_workspace_size", code, rows, dim, hidden, out, 0)
-                ws = _nn.workspace(size, dev)
-                _nn.check(lib.sdfnn_gated_forward(px, ldx, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), code, act, rows, dim, hidden, out,
-                                                  _nn.ptr(saved), y.data_ptr(), ws.data_ptr(), size, cur.stream), "sdfnn_gated_forward")
-        if save:
-            ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
+        y, saved = _forward(x, w_gate, w_up, w_down, act, True)
+        ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
         return y
 
     @staticmethod
@@ -78,6 +82,8 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         raise ValueError(f"{what}: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_down {tuple(w_down.shape)} do not chain")
     if not (x.dtype == w_gate.dtype == w_up.dtype == w_down.dtype):
         raise TypeError(f"{what}: x {x.dtype}, weights {w_gate.dtype}, {w_up.dtype}, {w_down.dtype}: one type")
+    if not _nn.differentiated(x, w_gate, w_up, w_down):
+        return _forward(x, w_gate, w_up, w_down, act, False)[0]
     return _GatedMLP.apply(x, w_gate, w_up, w_down, act)
 
 

@@ -21,21 +21,27 @@ def _check(what: str, x: torch.Tensor, weight: Optional[torch.Tensor], residual:
         raise ValueError(f"{what}: residual {tuple(residual.shape)} {residual.dtype} for x {tuple(x.shape)} {x.dtype}")
 
 
+def _forward(x, weight, residual, eps, save):
+    """y, h (None without a residual) and, with `save`, inv (else None)."""
+    lib, code = _nn.load(), _nn.dtype_code(x, "rms_norm")
+    dev = _nn.on_device("rms_norm", x, weight, residual)
+    with _nn.on(dev) as cur:
+        x2, px, rows, ldx = _nn.rows_of(x)
+        r2, pr, _, ldr = _nn.rows_of(residual) if residual is not None else (None, None, 0, 0)
+        w = weight.contiguous()
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        h = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
+        inv = torch.empty(rows, dtype=torch.float32, device=dev) if save else None
+        if rows:
+            _nn.check(lib.sdfnn_rms_norm_forward(px, ldx, pr, ldr, w.data_ptr(), code, rows, x.shape[-1], eps, y.data_ptr(), _nn.ptr(h),
+                                                 _nn.ptr(inv), cur.stream), "sdfnn_rms_norm_forward")
+    return y, h, inv
+
+
 class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        lib, code = _nn.load(), _nn.dtype_code(x, "rms_norm")
-        dev = _nn.on_device("rms_norm", x, weight, residual)
-        with _nn.on(dev) as cur:
-            x2, px, rows, ldx = _nn.rows_of(x)
-            r2, pr, _, ldr = _nn.rows_of(residual) if residual is not None else (None, None, 0, 0)
-            w = weight.contiguous()
-            y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-            h = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
-            inv = torch.empty(rows, dtype=torch.float32, device=dev)
-            if rows:
-                _nn.check(lib.sdfnn_rms_norm_forward(px, ldx, pr, ldr, w.data_ptr(), code, rows, x.shape[-1], eps, y.data_ptr(), _nn.ptr(h),
-                                                     inv.data_ptr(), cur.stream), "sdfnn_rms_norm_forward")
+        y, h, inv = _forward(x, weight, residual, eps, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, weight, residual, inv)
         return y if residual is None else (y, h)
@@ -73,6 +79,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     Returns y, with a residual (y, h).  x [..., dim] in float32 / bfloat16 / float16, weight [dim] and residual of the same type; gradients
     for x, weight and residual (one pass; not differentiable twice)."""
     _check("rms_norm", x, weight, residual)
+    if not _nn.differentiated(x, weight, residual):
+        y, h, _ = _forward(x, weight, residual, float(eps), False)
+        return y if residual is None else (y, h)
     return _RMSNorm.apply(x, weight, residual, float(eps))
 
 

@@ -473,3 +473,30 @@ def test_model_with_a_background_of_blocks_trains_and_serves(device):
         blocks.quantize()
         served = model(bundle)["rgb"]
     assert torch.isfinite(served).all() and float((served - plain).norm() / plain.norm()) < 0.05
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_no_grad_keeps_nothing(device, dtype):
+    """Under torch.no_grad() a module, whose parameters require gradients, neither writes nor holds what a backward pass would read, and gives the same
+    values."""
+    from sdfstudio_amd.field_components.mlp import GatedMLP, GatedStack
+
+    mlp = GatedMLP(64, 512).to("cuda", dtype)
+    x = torch.randn(40000, 64, device="cuda").to(dtype)
+    want = mlp(x)
+    assert want.requires_grad
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        y = mlp(x)
+    # the hidden rows in the type (fp32: three parts) and x's and the weights' parts; act(g) and u act'(g) would be 40000 x 512 x 8 bytes more
+    assert torch.cuda.max_memory_allocated() - before < 40000 * 512 * (6 if dtype == F32 else 2) + 40000 * 64 * 16 + (4 << 20)
+    assert torch.equal(y, want) and not y.requires_grad
+    stack = GatedStack(64, 128, 2).to("cuda", dtype)
+    want = stack(x)
+    with torch.inference_mode():
+        assert torch.equal(stack(x), want)
+    for p in stack.parameters():
+        p.requires_grad_(False)
+    assert torch.equal(stack(x), want) and not stack(x).requires_grad
