@@ -56,10 +56,10 @@ class _GatedMLP(torch.autograd.Function):
             g2, pg, _, ldg = _nn.rows_of(dy, align=True)
             wg, wu, wd = _nn.aligned(w_gate), _nn.aligned(w_up), _nn.aligned(w_down)
             dim = x.shape[-1]
-            dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-            dwg = torch.empty(hidden, dim, dtype=x.dtype, device=dev) if need_g or need_u else None
-            dwu = torch.empty(hidden, dim, dtype=x.dtype, device=dev) if need_g or need_u else None
-            dwd = torch.empty(out, hidden, dtype=x.dtype, device=dev) if need_d else None
+            dx = _nn.like(x) if need_x else None
+            dwg = _nn.like(w_gate) if need_g or need_u else None
+            dwu = _nn.like(w_up) if need_g or need_u else None
+            dwd = _nn.like(w_down) if need_d else None
             if rows == 0:
                 return dx, *(None if t is None else t.zero_() for t in (dwg, dwu, dwd)), None
             size = _nn.size("sdfnn_gated_workspace_size", code, rows, dim, hidden, out, 1)

@@ -29,8 +29,8 @@ def _forward(x, weight, residual, eps, save):
         x2, px, rows, ldx = _nn.rows_of(x)
         r2, pr, _, ldr = _nn.rows_of(residual) if residual is not None else (None, None, 0, 0)
         w = weight.contiguous()
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        h = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
+        y = _nn.like(x)
+        h = _nn.like(x) if residual is not None else None
         inv = torch.empty(rows, dtype=torch.float32, device=dev) if save else None
         if rows:
             _nn.check(lib.sdfnn_rms_norm_forward(px, ldx, pr, ldr, w.data_ptr(), code, rows, x.shape[-1], eps, y.data_ptr(), _nn.ptr(h),
@@ -62,8 +62,8 @@ class _RMSNorm(torch.autograd.Function):
             w = weight.contiguous()
             g2, pg, _, ldg = _nn.rows_of(dy) if dy is not None else (None, None, 0, 0)
             k2, pk, _, ldk = _nn.rows_of(dh) if dh is not None else (None, None, 0, 0)
-            dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-            dw = torch.empty(dim, dtype=x.dtype, device=dev) if need_w else None
+            dx = _nn.like(x) if need_x else None
+            dw = _nn.like(weight) if need_w else None
             if rows == 0:
                 return dx, dw.zero_() if need_w else None, dx if residual is not None else None, None
             size = _nn.size("sdfnn_rms_norm_backward_workspace_size", rows, dim) if need_w else 0
@@ -99,9 +99,9 @@ def _quantize(what: str, x: torch.Tensor, weight: Optional[torch.Tensor], residu
         x2, px, rows, ldx = _nn.rows_of(x)
         r2, pr, _, ldr = _nn.rows_of(residual) if residual is not None else (None, None, 0, 0)
         w = weight.contiguous() if weight is not None else None
-        q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+        q = _nn.like(x, torch.int8)
         scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-        h = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
+        h = _nn.like(x) if residual is not None else None
         if rows:
             _nn.check(lib.sdfnn_rms_norm_quantize(px, ldx, pr, ldr, _nn.ptr(w), code, rows, x.shape[-1], eps, q.data_ptr(), scales.data_ptr(),
                                                   _nn.ptr(h), cur.stream), "sdfnn_rms_norm_quantize")

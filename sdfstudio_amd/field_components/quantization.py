@@ -20,6 +20,9 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 
 def _check_operand(what: str, name: str, q: torch.Tensor, scales: torch.Tensor, k: Optional[int] = None) -> None:
+    if q.dtype == torch.int8 and scales.dtype == torch.float32 and q.dim() == 2 and scales.dim() == 1 and scales.size(0) == q.size(0) and \
+            (k is None or q.size(1) == k):
+        return  # (as nearly always)
     if q.dtype != torch.int8 or q.dim() < 1:
         raise TypeError(f"{what}: {name} {tuple(q.shape)} {q.dtype}: int8 rows expected")
     if k is not None and (q.dim() != 2 or q.shape[1] != k):
@@ -55,7 +58,7 @@ def int8_linear(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, w
         sq, sw = scales.contiguous(), weight_scales.contiguous()
         b = bias.contiguous() if bias is not None else None
         k = q.shape[-1]
-        y = torch.empty((*q.shape[:-1], n), dtype=out_dtype, device=dev)
+        y = torch.empty((rows, n) if q.dim() == 2 else (*q.shape[:-1], n), dtype=out_dtype, device=dev)
         if rows and n:
             size = _nn.size("sdfnn_int8_linear_workspace_size", rows, n, k, 1)
             ws = _nn.workspace(size, dev) if size else None
@@ -80,7 +83,7 @@ def int8_gated_linear(q: torch.Tensor, scales: torch.Tensor, gate_q: torch.Tenso
         u2, pu, _, ldu = _nn.rows_of(up_q, align=True)
         sq, sg, su = scales.contiguous(), gate_scales.contiguous(), up_scales.contiguous()
         k = q.shape[-1]
-        y = torch.empty((*q.shape[:-1], n), dtype=out_dtype, device=dev)
+        y = torch.empty((rows, n) if q.dim() == 2 else (*q.shape[:-1], n), dtype=out_dtype, device=dev)
         if rows and n:
             size = _nn.size("sdfnn_int8_linear_workspace_size", rows, n, k, 2)
             ws = _nn.workspace(size, dev) if size else None
