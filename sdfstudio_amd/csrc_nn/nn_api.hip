@@ -46,6 +46,27 @@ void pick_row(const int64_t dim, F&& f, W&& wide) {
 // rows that a workgroup of that shape takes at a time
 constexpr int64_t rows_at_once(const int tpr, const int u) { return (tpr > 256 ? 1 : 256 / tpr) * u; }
 dim3 row_grid(const int64_t rows, const int tpr, const int u) { return dim3((unsigned)ceil_div(rows, rows_at_once(tpr, u))); }
+// f(arguments) for pieces of the rows, each of less than the 2^32 threads that a launch may have
+template <int DT, class F>
+void row_pieces(const NormArgs& a, const int tpr, const int u, F&& f) {
+  typedef elem_t<DT> T;
+  const int64_t most = tpr > 256 ? (int64_t)1 << 21 : rows_at_once(tpr, u) << 23;
+  for (int64_t at = 0; at < a.rows; at += most) {
+    NormArgs b = a;
+    b.rows = std::min(most, a.rows - at);
+    b.x = (const T*)a.x + at * a.ldx;
+    if (a.r) b.r = (const T*)a.r + at * a.ldr;
+    if (a.dy) b.dy = (const T*)a.dy + at * a.lddy;
+    if (a.dh) b.dh = (const T*)a.dh + at * a.lddh;
+    if (a.y) b.y = (T*)a.y + at * a.dim;
+    if (a.h) b.h = (T*)a.h + at * a.dim;
+    if (a.dx) b.dx = (T*)a.dx + at * a.dim;
+    if (a.inv) b.inv = a.inv + at;
+    if (a.q) b.q = a.q + at * a.dim;
+    if (a.scales) b.scales = a.scales + at;
+    f(b);
+  }
+}
 
 int check_norm(const char* what, const void* x, const int64_t ldx, const void* residual, const int64_t ldr, const int32_t dtype,
                const int64_t rows, const int64_t dim) {
@@ -62,8 +83,14 @@ template <int DT>
 int norm_forward(const NormArgs& a, hipStream_t s) {
   pick_row(a.dim, [&](auto tpr, auto nv, auto u) {
     NN_ROW_SHAPE;
-    hipLaunchKernelGGL((rms_norm_fwd_kernel<DT, TPR, NV, U>), row_grid(a.rows, TPR, U), dim3(256), 0, s, a);
-  }, [&] { hipLaunchKernelGGL((rms_norm_fwd_wide_kernel<DT>), row_grid(a.rows, kWide, 1), dim3(kWide), 0, s, a); });
+    row_pieces<DT>(a, TPR, U, [&](const NormArgs& b) {
+      hipLaunchKernelGGL((rms_norm_fwd_kernel<DT, TPR, NV, U>), row_grid(b.rows, TPR, U), dim3(256), 0, s, b);
+    });
+  }, [&] {
+    row_pieces<DT>(a, kWide, 1, [&](const NormArgs& b) {
+      hipLaunchKernelGGL((rms_norm_fwd_wide_kernel<DT>), row_grid(b.rows, kWide, 1), dim3(kWide), 0, s, b);
+    });
+  });
   NN_LAUNCHED("rms_norm_forward");
   return 0;
 }
@@ -71,10 +98,16 @@ template <int DT>
 int norm_quantize(const NormArgs& a, hipStream_t s) {
   pick_row(a.dim, [&](auto tpr, auto nv, auto u) {
     NN_ROW_SHAPE;
-    const dim3 grid = row_grid(a.rows, TPR, U), block(256);
-    if (!a.w && !a.r) hipLaunchKernelGGL((rms_norm_quant_kernel<DT, TPR, NV, U, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((rms_norm_quant_kernel<DT, TPR, NV, U, false>), grid, block, 0, s, a);
-  }, [&] { hipLaunchKernelGGL((rms_norm_quant_wide_kernel<DT>), row_grid(a.rows, kWide, 1), dim3(kWide), 0, s, a); });
+    row_pieces<DT>(a, TPR, U, [&](const NormArgs& b) {
+      const dim3 grid = row_grid(b.rows, TPR, U), block(256);
+      if (!b.w && !b.r) hipLaunchKernelGGL((rms_norm_quant_kernel<DT, TPR, NV, U, true>), grid, block, 0, s, b);
+      else hipLaunchKernelGGL((rms_norm_quant_kernel<DT, TPR, NV, U, false>), grid, block, 0, s, b);
+    });
+  }, [&] {
+    row_pieces<DT>(a, kWide, 1, [&](const NormArgs& b) {
+      hipLaunchKernelGGL((rms_norm_quant_wide_kernel<DT>), row_grid(b.rows, kWide, 1), dim3(kWide), 0, s, b);
+    });
+  });
   NN_LAUNCHED("rms_norm_quantize");
   return 0;
 }
@@ -95,9 +128,13 @@ int norm_backward(NormArgs a, elem_t<DT>* dw, hipStream_t s) {
     pick_row(a.dim, [&](auto tpr, auto nv, auto u) {
       NN_ROW_SHAPE;
       if (dw) hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, TPR, NV, U, true>), dim3((unsigned)groups), dim3(256), 0, s, a);
-      else hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, TPR, NV, U, false>), row_grid(a.rows, TPR, U), dim3(256), 0, s, a);
+      else row_pieces<DT>(a, TPR, U, [&](const NormArgs& b) {
+        hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, TPR, NV, U, false>), row_grid(b.rows, TPR, U), dim3(256), 0, s, b);
+      });
     }, [&] {
-      if (a.dx) hipLaunchKernelGGL((rms_norm_bwd_wide_kernel<DT>), row_grid(a.rows, kWide, 1), dim3(kWide), 0, s, a);
+      if (a.dx) row_pieces<DT>(a, kWide, 1, [&](const NormArgs& b) {
+        hipLaunchKernelGGL((rms_norm_bwd_wide_kernel<DT>), row_grid(b.rows, kWide, 1), dim3(kWide), 0, s, b);
+      });
       if (dw) hipLaunchKernelGGL((rms_norm_dw_wide_kernel<DT>), dim3((unsigned)ceil_div(a.dim, 256), (unsigned)groups), dim3(256), 0, s, a);
     });
   NN_LAUNCHED("rms_norm_backward");

@@ -41,6 +41,7 @@ inline Tiling choose_tiling(const int64_t M, const int64_t N, const int nk, cons
   const int steps = nk * terms;
   for (int tile : {256, 128}) {
     const int64_t gm = ceil_div(M, tile), gn = ceil_div(N, tile), tiles = gm * gn;
+    if (tile == 128 && tiles >= (int64_t)1 << 24) break;  // a launch has less than 2^32 threads (256 x 256 tiles that would not fit exceed the memory)
     const int64_t slots = tile == 256 ? 256 : 512;
     const int most = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 4, 2 * slots / std::max<int64_t>(tiles, 1)));
     for (int s = 1; s <= most; s = s < 4 ? s + 1 : s + s / 4) {
@@ -86,7 +87,7 @@ int product(Call& c, const Operand& a, const Operand& b0, const Operand& b1, con
   char* part = t.splits > 1 ? c.take((int64_t)t.splits * M * ld * 4) : nullptr;
   if (c.dry() || M == 0 || N == 0) return 0;
   NN_REQUIRE(256 * std::max(a.ld, std::max(b0.ld, b1.ld)) < 0x7fffffff, "rows of more than 8 MiB are not supported");
-  NN_REQUIRE((int64_t)t.gm * t.gn * t.splits < 0x7fffffff && nk * TERMS < 0x7fffffff, "too many tiles");
+  NN_REQUIRE((int64_t)t.gm * t.gn * t.splits < (int64_t)1 << 24 && nk * TERMS < 0x7fffffff, "too many tiles");
   if (t.splits == 1) {
     GemmArgs<EPI> g{a, {b0, b1}, M, (int)N, (int)nk, (int)turn, 0, 0, 0, 0, epi};
     return launch_gemm<KIND, TERMS, DUAL, SIDES>(c, t, g);
@@ -168,13 +169,13 @@ struct Packs {
     if (rows > 0 && pad > 0) {
       b.a[b.count] = {src, ld, rows, cols, dst, pad, plane, pad};
       b.first[b.count++] = (unsigned)blocks;
-      blocks += ceil_div(rows * (pad / 8), 256);
+      blocks += std::min<int64_t>(ceil_div(rows * (pad / 8), 256), 1 << 21);
     }
     return {dst, pad * es, plane, rows, pad * es};
   }
   int launch(Call& c) {
     if (c.dry() || b.count == 0) return 0;
-    NN_REQUIRE(blocks < 0x7fffffff, "operands of more than 2^42 elements");
+    b.first[b.count] = (unsigned)blocks;
     hipLaunchKernelGGL((pack_rows_kernel<ES>), dim3((unsigned)blocks), dim3(256), 0, c.stream, b);
     NN_LAUNCHED("operand copy");
     return 0;

@@ -29,29 +29,30 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const PackBatch b) {
   for (int j = 1; j < kPacks; ++j)
     if (j < b.count && blockIdx.x >= b.first[j]) k = j;
   const PackArgs& a = b.a[k];
-  const int64_t groups = a.pad / 8, i = (int64_t)(blockIdx.x - b.first[k]) * 256 + threadIdx.x;
-  if (i >= groups * a.rows) return;
-  const int64_t row = i / groups, c = (i - row * groups) * 8;
-  const int64_t left = a.cols - c;
-  if constexpr (ES == 4) {
-    float v[8];
-    load8_n<SDFNN_F32>((const float*)a.src + row * a.ld + c, (int)(left < 0 ? 0 : left < 8 ? left : 8), v);
-    store_parts(a.dst + (row * a.dst_ld + c) * 2, a.plane, v);
-  } else {
-    const char* s = (const char*)a.src + (row * a.ld + c) * ES;
-    char b[8 * ES];
-    if (left >= 8) {
-      const Bytes<2 * ES, ES> raw = *reinterpret_cast<const Bytes<2 * ES, ES>*>(s);
-      __builtin_memcpy(b, &raw, 8 * ES);
+  const int64_t groups = a.pad / 8, total = groups * a.rows, threads = (int64_t)(b.first[k + 1] - b.first[k]) * 256;
+  for (int64_t i = (int64_t)(blockIdx.x - b.first[k]) * 256 + threadIdx.x; i < total; i += threads) {  // (more than one turn: beyond 2^32 elements)
+    const int64_t row = i / groups, c = (i - row * groups) * 8;
+    const int64_t left = a.cols - c;
+    if constexpr (ES == 4) {
+      float v[8];
+      load8_n<SDFNN_F32>((const float*)a.src + row * a.ld + c, (int)(left < 0 ? 0 : left < 8 ? left : 8), v);
+      store_parts(a.dst + (row * a.dst_ld + c) * 2, a.plane, v);
     } else {
+      const char* s = (const char*)a.src + (row * a.ld + c) * ES;
+      char b[8 * ES];
+      if (left >= 8) {
+        const Bytes<2 * ES, ES> raw = *reinterpret_cast<const Bytes<2 * ES, ES>*>(s);
+        __builtin_memcpy(b, &raw, 8 * ES);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (e < left) __builtin_memcpy(b + e * ES, s + e * ES, ES);
-        else __builtin_memset(b + e * ES, 0, ES);
+        for (int e = 0; e < 8; ++e) {
+          if (e < left) __builtin_memcpy(b + e * ES, s + e * ES, ES);
+          else __builtin_memset(b + e * ES, 0, ES);
+        }
       }
+      Bytes<2 * ES, 8> raw;
+      __builtin_memcpy(&raw, b, 8 * ES);
+      *reinterpret_cast<Bytes<2 * ES, 8>*>(a.dst + (row * a.dst_ld + c) * ES) = raw;
     }
-    Bytes<2 * ES, 8> raw;
-    __builtin_memcpy(&raw, b, 8 * ES);
-    *reinterpret_cast<Bytes<2 * ES, 8>*>(a.dst + (row * a.dst_ld + c) * ES) = raw;
   }
 }

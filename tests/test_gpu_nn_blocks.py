@@ -500,3 +500,60 @@ def test_no_grad_keeps_nothing(device, dtype):
     for p in stack.parameters():
         p.requires_grad_(False)
     assert torch.equal(stack(x), want) and not stack(x).requires_grad
+
+
+def test_more_rows_than_one_launch_has_threads(device):
+    """A launch has less than 2^32 threads: norms of narrow rows beyond 2^29 and of wide ones beyond 2^21, operand copies of more than 2^35 elements
+    and products of 2^31 - 1 rows come in pieces; rows at every border are right."""
+    from sdfstudio_amd.field_components.normalization import rms_norm
+    from sdfstudio_amd.field_components.quantization import int8_linear, quantize_rows
+
+    def rows_at(*borders):
+        return torch.tensor([b + i for b in borders for i in range(-3, 3)], device="cuda")
+
+    rows = (1 << 29) + 70
+    pick = rows_at(3, 1 << 28, 1 << 29, rows - 3)
+    x = torch.zeros(rows, 2, device="cuda", dtype=BF16)
+    x[pick] = torch.randn(len(pick), 2, device="cuda").to(BF16)
+    w = torch.tensor([1.0, 2.0], device="cuda", dtype=BF16)
+    h = x[pick].double().requires_grad_(True)
+    want = rms(h, w.double())
+    leaf = x.requires_grad_(True)
+    y = rms_norm(leaf, w)
+    near("y", y[pick], want, 2.0 ** -8)
+    (dx,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    (dh,) = torch.autograd.grad(want, h, torch.ones_like(want))
+    # dx is a difference of terms: half a step of bf16, and 2^-20 of inv times the largest weight, each
+    inv = 1.0 / torch.sqrt(h.detach().square().mean(-1, keepdim=True) + 1e-6)
+    assert ((dx[pick].double() - dh).abs() <= 2.0 ** -8 * dh.abs() + 2.0 ** -19 * 2.0 * inv).all()
+    del y, dx
+    q, s = quantize_rows(leaf)
+    top = h.detach().abs().amax(-1, keepdim=True)
+    assert torch.equal(q[pick].double(), torch.round(127 * h.detach() / top)) and not q[10:1000].any() and not s[10:1000].any()
+    del q, s, x, leaf
+    rows = (1 << 28) + 100
+    q = torch.randint(-127, 128, (rows, 1), device="cuda", dtype=torch.int8)
+    s, wq, sw = torch.rand(rows, device="cuda"), torch.tensor([[5], [-7]], device="cuda", dtype=torch.int8), torch.tensor([0.5, 0.25], device="cuda")
+    y = int8_linear(q, s, wq, sw)
+    for i in range(2):
+        assert torch.equal(y[:, i], q[:, 0] * wq[i].float() * s * sw[i])
+    del q, s, y
+    torch.cuda.empty_cache()
+    rows = (1 << 31) - 1
+    pick = rows_at(3, 1 << 30, rows - 3)
+    q = torch.zeros(rows, 16, device="cuda", dtype=torch.int8)
+    q[pick] = torch.randint(-127, 128, (len(pick), 16), device="cuda", dtype=torch.int8)
+    wq = torch.randint(-127, 128, (1, 16), device="cuda", dtype=torch.int8)
+    y = int8_linear(q, torch.ones(rows, device="cuda"), wq, torch.ones(1, device="cuda"))
+    assert torch.equal(y[pick].double(), q[pick].double() @ wq.double().t()) and not y[10:1000].any()
+    del q, y
+    torch.cuda.empty_cache()
+    rows = (1 << 21) + 5
+    pick = rows_at(3, 1 << 20, 1 << 21, rows - 3)
+    x = torch.zeros(rows, 8200, device="cuda", dtype=F16)
+    x[pick] = torch.randn(len(pick), 8200, device="cuda").to(F16)
+    q, s = quantize_rows(x)
+    v = x[pick].double()
+    assert torch.equal(q[pick].double(), torch.round(127 * v / v.abs().amax(-1, keepdim=True))) and not s[10:1000].any()
+    del x, q, s
+    torch.cuda.empty_cache()
