@@ -66,7 +66,8 @@ int sdfnn_int8_gated_linear(const int8_t* q, int64_t ldq, const float* sq, const
 /* ---- gated MLP
  * g = x Wg^T, u = x Wu^T, a = act(g) u, y = a Wd^T.  x [rows, dim] (stride ldx), w_gate / w_up [hidden, dim], w_down [out, hidden], all
  * contiguous, y [rows, out] contiguous.  16-bit types: products of those types with fp32 sums; a is rounded to the type before the second
- * product, and so are the gradients of g and u before theirs (fp16: a hidden value beyond 65504 becomes infinite and gradients below 6e-8
+ * product (up to 16 rows it goes there as two numbers of the type that hold twice its bits), and so are the gradients of g
+ * and u before theirs (fp16: a hidden value beyond 65504 becomes infinite - up to 16 rows of a forward pass: beyond 131008 - and gradients below 6e-8
  * vanish, as everywhere in that type: scale the loss).  fp32: every operand as three bf16 parts that hold its 24 bits, six products, fp32
  * sums (magnitudes below 2^-110 hold fewer bits).  A row with an input that is not finite gives NaN.
  * saved: sdfnn_gated_saved_size bytes, what the backward needs (act(g) and u act'(g) in fp32, a in the type; fp32 above 64 rows: a and x as

@@ -428,7 +428,10 @@ struct StoreEpi {
 // there were read as zeros).  Where a backward pass will follow, the two factors it needs beside it: act(g) and u act'(g), formed from the
 // sums as they are and kept in fp32 - rounded to 16 bits, g and u alone cost the gradients as much as all their other roundings together
 // (error against 64 bits at 8192 x 4096 x 16384 bf16: 0.0031 of the gradients' size, 0.0024 this way, 0.0017 their own last rounding).
-template <int DT>
+// a itself is one number of the type where tiles read it, and so are the gradients of g and u below: each as two numbers would be a third more matrix
+// instructions forward and five sixths more backward.  TWO (few rows of 16 bits): two numbers, the rounding of a and what it leaves, which hold a to
+// 2^-16 (bf16) and 2^-22.
+template <int DT, bool TWO = false>
 struct GatedEpi {
   static constexpr int kCost = DT == SDFNN_F32 ? 370 : 300;
   static constexpr int kUnroll = 1;
@@ -437,6 +440,8 @@ struct GatedEpi {
   int64_t plane;   // fp32: 0: a as it is; else its three bf16 parts, as the second product reads them, this many bytes apart
   float *fu, *fg;  // factors of du and dg; NULL: inference
   int F, act;
+  elem_t<DT>* two = nullptr;  // TWO: [2 M][F], the second numbers `rest` elements behind the first; a: NULL unless a backward pass will follow
+  int64_t rest = 0;
   NN_D Nothing cols(int) const { return {}; }
   NN_D Nothing fetch(int64_t, int64_t, int) const { return {}; }
   NN_D void pair(int, const int64_t m, const int n, const float (&v)[8], const float (&u)[8], Nothing, Nothing) const {
@@ -456,6 +461,18 @@ struct GatedEpi {
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] *= u[i];
+    if constexpr (TWO) {
+      float p[8], q[8];
+      constexpr float top = DT == SDFNN_F16 ? 65504.0f : 0x1.fep127f;  // the first is held there, so that only what is infinite becomes so
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = (float)(elem_t<DT>)__builtin_amdgcn_fmed3f(o[i], -top, top);
+        q[i] = o[i] - p[i];
+      }
+      store8<DT>(two + m * F + n, p);
+      store8<DT>(two + rest + m * F + n, q);
+      if (!a) return;
+    }
     if (DT == SDFNN_F32 && plane) store_parts((char*)a + (m * F + n) * 2, plane, o);
     else store8<DT>(a + m * F + n, o);
   }

@@ -222,15 +222,27 @@ int gated_forward(Call& c, const void* x, const int64_t ldx, const void* wg, con
   typedef Kind<DT> K;
   const int64_t Fp = round_up(F, 64), es = K::es;
   Saved<DT> sv(saved, M, Fp);
-  if (!saved) sv.fu = sv.fg = nullptr, sv.a = c.take(Saved<DT>::a_size(M, Fp));
-  const GatedEpi<DT> ge{(T*)sv.a, sv.plane, sv.fu, sv.fg, (int)Fp, act};
+  // Up to 16 rows of 16 bits the hidden row goes into the second product as two numbers (GatedEpi): they fit the few-row product's 32 rows, which is bound
+  // by the weights.  4096 x 16384 bf16, one number / two: 1 row 84 / 84 us, 8 rows 88 / 90, 16 rows 90 / 103; 17 rows 97 / 111, 32 rows 114 / 140
+  // (the operand rows, read by every workgroup, are the time by then).
+  const bool few = M <= few_rows(K::few), two = !K::f32 && 2 * M <= few_rows(K::few);
+  if (!saved) sv.fu = sv.fg = nullptr, sv.a = two ? nullptr : c.take(Saved<DT>::a_size(M, Fp));
   const StoreEpi<DT> se{(T*)y, nullptr, M, M, 0, O, (int)O};
-  if (M <= few_rows(K::few)) {
+  if (few) {
     const Operand xo{(const char*)x, ldx * es, 0, M, D * es}, g{(const char*)wg, D * es, 0, F, D * es}, u{(const char*)wu, D * es, 0, F, D * es};
-    const Operand ao{sv.a, Fp * es, 0, M, F * es}, d{(const char*)wd, F * es, 0, O, F * es};
+    const Operand d{(const char*)wd, F * es, 0, O, F * es};
+    if constexpr (!K::f32)
+      if (two) {
+        char* a2 = c.take(2 * M * Fp * es);
+        const GatedEpi<DT, true> ge{(T*)sv.a, 0, sv.fu, sv.fg, (int)Fp, act, (T*)a2, M * Fp};
+        NN_TRY((skinny<K::few, true>(c, xo, g, u, M, F, Fp, ge)));
+        return skinny<K::few, false, true>(c, {a2, Fp * es, 0, 2 * M, F * es}, d, d, 2 * M, O, O, se);
+      }
+    const GatedEpi<DT> ge{(T*)sv.a, 0, sv.fu, sv.fg, (int)Fp, act};
     NN_TRY((skinny<K::few, true>(c, xo, g, u, M, F, Fp, ge)));
-    return skinny<K::few, false>(c, ao, d, d, M, O, O, se);
+    return skinny<K::few, false>(c, {sv.a, Fp * es, 0, M, F * es}, d, d, M, O, O, se);
   }
+  const GatedEpi<DT> ge{(T*)sv.a, sv.plane, sv.fu, sv.fg, (int)Fp, act};
   Packs<K::es> packs;
   const Operand xo = operand<DT>(c, packs, x, ldx, M, D, saved && K::f32 ? sv.x : nullptr), g = operand<DT>(c, packs, wg, D, F, D), u = operand<DT>(c, packs, wu, D, F, D);
   const Operand d = operand<DT>(c, packs, wd, F, O, F);

@@ -106,15 +106,15 @@ int product(Call& c, const Operand& a, const Operand& b0, const Operand& b1, con
 // longer: 64 x 4096 -> 2 x 16384 -> 4096 takes 714 us on tiles and 391 here, its backward pass 1076 and 710 (16 rows: 1045 and 435).
 constexpr int64_t few_rows(const int kind) { return kind == 3 ? 64 : 32; }
 
-// the same for at most few_rows(KIND) rows.  cols: columns that the epilogue writes (>= N)
-template <int KIND, bool DUAL, class EPI>
+// the same for at most few_rows(KIND) rows.  cols: columns that the epilogue writes (>= N).  PAIR: M rows of a, each result the sum of two
+template <int KIND, bool DUAL, bool PAIR = false, class EPI>
 int skinny(Call& c, const Operand& a, const Operand& b0, const Operand& b1, const int64_t M, const int64_t N, const int64_t cols, const EPI& epi) {
   if (c.dry() || M == 0 || N == 0) return 0;
   GemmArgs<EPI> g{a, {b0, b1}, M, (int)N, 0, 0, 0, 0, 0, 0, epi};
   const dim3 grid((unsigned)ceil_div(cols, 16)), block(kSkinnyWaves * 64);
-  if (M <= 16) hipLaunchKernelGGL((skinny_kernel<KIND, 1, DUAL, EPI>), grid, block, 0, c.stream, g);
-  else if (M <= 32) hipLaunchKernelGGL((skinny_kernel<KIND, 2, DUAL, EPI>), grid, block, 0, c.stream, g);
-  else if constexpr (few_rows(KIND) > 32) hipLaunchKernelGGL((skinny_kernel<KIND, 4, DUAL, EPI>), grid, block, 0, c.stream, g);
+  if (M <= 16) hipLaunchKernelGGL((skinny_kernel<KIND, 1, DUAL, PAIR, EPI>), grid, block, 0, c.stream, g);
+  else if (M <= 32) hipLaunchKernelGGL((skinny_kernel<KIND, 2, DUAL, PAIR, EPI>), grid, block, 0, c.stream, g);
+  else if constexpr (few_rows(KIND) > 32) hipLaunchKernelGGL((skinny_kernel<KIND, 4, DUAL, PAIR, EPI>), grid, block, 0, c.stream, g);
   NN_LAUNCHED("product of few rows");
   return 0;
 }

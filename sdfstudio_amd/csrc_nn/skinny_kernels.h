@@ -2,7 +2,8 @@
 //
 // Bound by reading the weights once.  They go from HBM straight into the operand registers of the matrix instruction (nothing is read twice,
 // so LDS would only add a trip): a wavefront owns 16 rows of w (DUAL: 16 of each projection), a lane 16 bytes of one row at a time; the
-// eight wavefronts of a workgroup take turns of 8 KiB along k and join their sums in LDS.  x comes from L2.  fp32 runs on
+// eight wavefronts of a workgroup take turns of 8 KiB along k and join their sums in LDS.  x comes from L2.  PAIR: a row of x is the sum of two rows of
+// the operand, m and m + M / 2 (a value in two 16-bit numbers): both are multiplied, the join adds them.  fp32 runs on
 // v_mfma_f32_16x16x4_f32 as it is - at so few rows its rate suffices - and needs no splitting pass over the weights.  Rows need their element's
 // alignment only.  One row, 4096 -> 2 x 16384 -> 4096 bf16: 49 us (5.4 TB/s) and 32 us (4.1 TB/s, of which ~5 us are start and end).
 #pragma once
@@ -57,7 +58,7 @@ NN_D i32x4 load16(const char* p, const int64_t left) {  // 16 bytes, `left` of t
 
 constexpr int kSkinnyWaves = 8;
 
-template <int KIND, int MT, bool DUAL, class EPI>
+template <int KIND, int MT, bool DUAL, bool PAIR, class EPI>
 __global__ __launch_bounds__(kSkinnyWaves * 64) void skinny_kernel(const GemmArgs<EPI> g) {
   typedef Small<KIND> S_;
   const int64_t kb = g.b[0].width;
@@ -139,7 +140,9 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void skinny_kernel(const GemmArg
   // a lane (grp, col) of a wavefront holds rows n = 4 grp + r of column m = col; a thread joins the eight sums of 8 consecutive n
   if (threadIdx.x < MT * 32) {  // (MT <= 4: 128 of 512 threads)
     const int i = threadIdx.x >> 5, half = (threadIdx.x >> 4) & 1, c = threadIdx.x & 15;
-    const int64_t m = i * 16 + c;
+    const int64_t m = i * 16 + c, M = PAIR ? g.M / 2 : g.M;
+    if (m >= M) return;
+    const int j = PAIR ? (int)(m + M) >> 4 : 0, d = PAIR ? (int)(m + M) & 15 : 0;  // (m + M < 16 MT)
     typename S_::el v[NP][8];
 #pragma unroll
     for (int p = 0; p < NP; ++p)
@@ -148,13 +151,15 @@ __global__ __launch_bounds__(kSkinnyWaves * 64) void skinny_kernel(const GemmArg
         typename S_::el s = 0;
 #pragma unroll
         for (int k = 0; k < kSkinnyWaves; ++k) s += part[k][p * MT + i][e & 3][(half * 2 + (e >> 2)) * 16 + c];
+        if constexpr (PAIR) {
+#pragma unroll
+          for (int k = 0; k < kSkinnyWaves; ++k) s += part[k][p * MT + j][e & 3][(half * 2 + (e >> 2)) * 16 + d];
+        }
         v[p][e] = n0 + half * 8 + e < g.N ? s : (typename S_::el)0;  // the padding columns of a workspace are zeros
       }
-    if (m < g.M) {
-      const int c = n0 + half * 8;
-      if constexpr (DUAL) g.epi.pair(0, m, c, v[0], v[1], g.epi.cols(c), g.epi.fetch(m, g.M, c));
-      else g.epi.one(0, m, c, v[0], g.epi.cols(c), g.epi.fetch(m, g.M, c));
-    }
+    const int n8 = n0 + half * 8;
+    if constexpr (DUAL) g.epi.pair(0, m, n8, v[0], v[1], g.epi.cols(n8), g.epi.fetch(m, M, n8));
+    else g.epi.one(0, m, n8, v[0], g.epi.cols(n8), g.epi.fetch(m, M, n8));
   }
 }
 

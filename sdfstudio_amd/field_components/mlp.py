@@ -73,7 +73,9 @@ class _GatedMLP(torch.autograd.Function):
 def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str = "silu") -> torch.Tensor:
     """(activation(x w_gate^T) * (x w_up^T)) w_down^T: x [..., dim], w_gate / w_up [hidden, dim], w_down [out, hidden], all float32, bfloat16
     or float16; activation "silu", "gelu" (with the error function) or "relu".  Gradients for all four (not differentiable twice); under
-    torch.no_grad() nothing is kept for them.  float32 runs at float32 accuracy."""
+    torch.no_grad() nothing is kept for them.  float32 runs at float32 accuracy.  In the 16-bit types sums are float32, and the hidden row and the
+    gradients of the two projections are rounded to the type, as a chain of linear layers of that type rounds them; up to 16 rows the hidden row of the
+    forward pass keeps twice the type's bits."""
     what = "gated_mlp"
     act = _nn.activation_code(activation, what)
     if x.dim() < 1 or w_gate.dim() != 2 or w_down.dim() != 2 or w_gate.shape != w_up.shape:
