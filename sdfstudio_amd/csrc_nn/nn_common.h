@@ -111,11 +111,12 @@ NN_D void store_parts(char* p, const int64_t plane, const float (&v)[8]) {
 
 // ---- activations of the gated block and their derivatives.  FAST (16-bit results): the hardware's exponential and reciprocal, one ulp of
 // fp32 each, the exponent rounded to fp32 before it.  fp32 results: the part of x log2(e) that this rounding loses goes back in to first
-// order, and one Newton step follows the reciprocal.  |x| is cut at 87, where the exponential leaves the normal numbers.
+// order, and one Newton step follows the reciprocal; x <= 0 there, cut at -128, where the exponential has long been 0 (it ends with the normal numbers,
+// below -87.3), so that nothing is left to multiply a large z with.
 template <bool FAST>
 NN_D float nn_exp(float x) {
   if constexpr (FAST) return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
-  x = __builtin_amdgcn_fmed3f(x, -87.0f, 87.0f);
+  x = __builtin_amdgcn_fmed3f(x, -128.0f, 0.0f);
   const float t = x * 1.44269504088896340736f;
   const float lost = fmaf(x, 1.44269504088896340736f, -t) + x * 1.92596299112661746887e-8f;
   const float e = __builtin_amdgcn_exp2f(t);
@@ -166,10 +167,15 @@ NN_D float nn_phi(const float z) {
 // a = act(z), d = act'(z)
 template <bool FAST, int ACT>
 NN_D void act_both(const float z, float& a, float& d) {
-  if constexpr (ACT == SDFNN_SILU) {
+  if constexpr (ACT == SDFNN_SILU && FAST) {
     const float s = nn_recip<FAST>(1.0f + nn_exp<FAST>(-z));
     a = z * s;
     d = s * (1.0f + z * (1.0f - s));
+  } else if constexpr (ACT == SDFNN_SILU) {  // the sigmoid of |z| and of -|z| from exp(-|z|), which does not overflow
+    const float e = nn_exp<FAST>(-fabsf(z)), r = nn_recip<FAST>(1.0f + e), q = e * r;
+    const float s = z < 0.0f ? q : r;
+    a = z * s;
+    d = s * (1.0f + z * (z < 0.0f ? r : q));
   } else if constexpr (ACT == SDFNN_GELU) {
     const float phi = nn_phi<FAST>(z);
     a = z * phi;
