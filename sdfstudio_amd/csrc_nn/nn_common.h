@@ -129,8 +129,9 @@ NN_D float nn_recip(const float x) {  // 1 <= x < 2^127
   return fmaf(fmaf(-x, r, 1.0f), r, r);
 }
 // Phi(z), the normal distribution function.  For x = |z|:
-//   16-bit results: Phi(-x) = 2^(P(x) - x^2 / (2 ln 2)), P of degree 8 fitted to log2(erfcx(x / sqrt 2) / 2) on [0, 5] and held constant behind
-//   (Phi < 3e-7 there): off by 7e-7 at most, one exponential and no reciprocal.  The epilogues that call it are bound by such instructions.
+//   16-bit results: Phi(-x) = 2^(P(x) - x^2 / (2 ln 2)), P of degree 10 fitted to log2(erfcx(x / sqrt 2) / 2) on [0, 13.2], behind which Phi lies
+//   below the normal numbers: off by 6e-7 at most and by 1.3e-4 (2^-13) of its value, one exponential and no reciprocal.  The epilogues that call it are
+//   bound by such instructions.
 //   fp32 results: Phi(-x) = exp(-x^2 / 2) t P(t) / 2 with t = 1 / (1 + 0.4 x / sqrt 2), P of degree 8 fitted for the smallest relative error over
 //   x >= 0 (1.3e-7).
 template <bool FAST>
@@ -138,16 +139,18 @@ NN_D float nn_phi(const float z) {
   const float x = fabsf(z);
   float p, c;
   if constexpr (FAST) {
-    const float y = __builtin_amdgcn_fmed3f(x, 0.0f, 5.0f);
-    p = -2.92766572e-07f;
-    p = fmaf(p, y, 4.06725712e-06f);
-    p = fmaf(p, y, 1.34747179e-05f);
-    p = fmaf(p, y, -0.000727434061f);
-    p = fmaf(p, y, 0.0080369357f);
-    p = fmaf(p, y, -0.0533734821f);
-    p = fmaf(p, y, 0.262529612f);
-    p = fmaf(p, y, -1.15117145f);
-    p = fmaf(p, y, -0.999998152f);
+    const float y = __builtin_amdgcn_fmed3f(x, 0.0f, 13.2f);
+    p = -1.88042928e-10f;
+    p = fmaf(p, y, 9.56122825e-09f);
+    p = fmaf(p, y, -1.5210604e-07f);
+    p = fmaf(p, y, -4.91635603e-07f);
+    p = fmaf(p, y, 5.22080772e-05f);
+    p = fmaf(p, y, -0.000877389451f);
+    p = fmaf(p, y, 0.0083174957f);
+    p = fmaf(p, y, -0.0536075197f);
+    p = fmaf(p, y, 0.262596905f);
+    p = fmaf(p, y, -1.15117240f);
+    p = fmaf(p, y, -0.999998510f);
     c = __builtin_amdgcn_exp2f(fmaf(z * z, -0.72134752044448170368f, p));
   } else {
     const float t = nn_recip<FAST>(fmaf(0.28284271247461900976f, x, 1.0f));

@@ -64,3 +64,19 @@ def test_fp32_activations_far_from_zero(device, act, rows):
     s = z.abs() / 2.0 ** 20
     y = int8_gated_linear(q, s, one, torch.full((1,), 2.0 ** 20, device="cuda"), one, torch.full((1,), 2.0 ** -20, device="cuda"), activation=act)
     close("8 bits", y[:, 0], a * (z.double() * 2.0 ** -40), 2.0 ** -126 * 256, rel + 2.0 ** -20)
+
+
+@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("rows", [30, 8192])
+def test_16_bit_gelu_holds_its_relative_accuracy(device, t, rows):
+    """gelu of values far left of zero, where it is small but not nothing: z Phi(z) to the type's own step."""
+    from sdfstudio_amd.field_components.quantization import int8_gated_linear
+
+    x = torch.linspace(0.0, 12.5, rows, device="cuda")
+    q = torch.full((rows, 1), -1, device="cuda", dtype=torch.int8)
+    one = torch.ones(1, 1, device="cuda", dtype=torch.int8)
+    su = 1.0 if t == BF16 else 4096.0
+    y = int8_gated_linear(q, x, one, torch.ones(1, device="cuda"), one, torch.full((1,), su, device="cuda"), activation="gelu", out_dtype=t)
+    z = -x.double()
+    # 2^-12 for log2 of the tail's polynomial (1.3e-4), its exponent of up to 113 rounded twice (1e-5) and the exponential (2^-23)
+    close("gelu", y[:, 0], ACTS["gelu"](z) * (z * su), 2.0 ** -126 * 256, half(t) + 2.0 ** -12)
