@@ -12,8 +12,8 @@
  *
  * Matrices are row-major; a row stride (ld*, in elements) may exceed the row's width, elements of a row are adjacent.  Tensors need their
  * element's alignment; where a product of more than 32 rows (or a backward pass) reads its operands in place - 16-bit rows of a multiple of
- * 8 elements, codes of a multiple of 16 - every row has to start at a 16-byte boundary, else the call is refused.  Rows of 8 MiB and more
- * are refused there too.  Outputs are contiguous; what lies behind their last row is left as it was.
+ * 8 elements, codes of a multiple of 16 - every row has to start at a 16-byte boundary, and rows have to be less than 8 MiB apart, else the
+ * call is refused.  Outputs are contiguous; what lies behind their last row is left as it was.
  */
 #ifndef SDFNN_H_
 #define SDFNN_H_

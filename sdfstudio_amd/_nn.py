@@ -30,6 +30,7 @@ _SIGNATURES = {
 }
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
+ROW_REACH = 1 << 23  # bytes between rows from which the products do not read them in place
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -88,8 +89,8 @@ def on_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -
 
 def rows_of(t: torch.Tensor, align: bool = False) -> Tuple[torch.Tensor, int, int, int]:
     """t [..., dim] as rows the kernels can walk: (tensor to keep alive, its address, rows, row stride in elements).  The tensor itself or a
-    view wherever that is possible; a copy for rows that are not adjacent in memory, overlap, or - with `align` - do not start at 16-byte
-    boundaries although their width would allow it."""
+    view wherever that is possible; a copy for rows that are not adjacent in memory, overlap, or - with `align`, for the products - do not start at
+    16-byte boundaries although their width would allow it or are 8 MiB and more apart."""
     dim = t.shape[-1]
     whole = align and dim * t.element_size() % 16 == 0
     if t.is_contiguous():
@@ -99,7 +100,8 @@ def rows_of(t: torch.Tensor, align: bool = False) -> Tuple[torch.Tensor, int, in
     rows = t.numel() // dim
     t2 = t.reshape(rows, dim)
     stride = t2.stride(0) if rows > 1 else dim
-    if (dim > 1 and t2.stride(1) != 1) or stride < dim or (whole and (t2.data_ptr() % 16 or stride * t2.element_size() % 16)):
+    if (dim > 1 and t2.stride(1) != 1) or stride < dim or (align and stride * t2.element_size() >= ROW_REACH) or \
+            (whole and (t2.data_ptr() % 16 or stride * t2.element_size() % 16)):
         t2, stride = t2.clone(memory_format=torch.contiguous_format), dim
     return t2, t2.data_ptr(), rows, stride
 

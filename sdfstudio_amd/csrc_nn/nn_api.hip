@@ -27,6 +27,9 @@ constexpr int64_t kMaxRows = 0x7fffffff, kMaxDim = (int64_t)1 << 24;
 
 bool aligned16(const void* p, const int64_t ld_bytes) { return ((uintptr_t)p & 15) == 0 && (ld_bytes & 15) == 0; }
 
+// Tiles reach the rows of an operand that they read in place through 31-bit offsets (gemm_core.h): 256 of them lie below 2^31 bytes
+#define NN_REACH(what, ld, es) NN_REQUIRE((ld) <= ((int64_t)1 << 23) / (es) - 1, "%s: rows %lld bytes apart: less than 8 MiB", what, (long long)((ld) * (es)))
+
 // ---------------------------------------------------------------------------------------------- norm
 // f(IC<TPR>, IC<NV>, IC<U>) for the row width: how many threads and registers hold a row, how many rows at a time (norm_kernels.h); wide()
 // for rows that they do not hold
@@ -171,9 +174,11 @@ int check_int8(const char* what, const int8_t* q, const int64_t ldq, const int8_
   NN_REQUIRE(k >= 1 && k <= 131072, "%s: k = %lld: the 32-bit sum is exact for 1 .. 131072", what, (long long)k);
   NN_REQUIRE(q && w0 && w1, "%s: null tensor", what);
   NN_REQUIRE(ldq >= k && ld0 >= k && ld1 >= k, "%s: a row stride is smaller than the row", what);
-  if (rows > few_rows(2) && k % 16 == 0)
+  if (rows > few_rows(2) && k % 16 == 0) {
+    for (const int64_t ld : {ldq, ld0, ld1}) NN_REACH(what, ld, 1);
     NN_REQUIRE(aligned16(q, ldq) && aligned16(w0, ld0) && aligned16(w1, ld1),
                "%s: with k a multiple of 16 rows have to start at 16-byte boundaries", what);
+  }
   return 0;
 }
 
@@ -464,6 +469,7 @@ int sdfnn_gated_forward(const void* x, int64_t ldx, const void* w_gate, const vo
     NN_REQUIRE(dim % 8 || (aligned16(x, ldx * es) && aligned16(w_gate, 0) && aligned16(w_up, 0)),
                "gated_forward: with dim a multiple of 8 rows have to start at 16-byte boundaries");
     NN_REQUIRE(hidden % 8 || aligned16(w_down, 0), "gated_forward: with hidden a multiple of 8 w_down has to start at a 16-byte boundary");
+    if (dim % 8 == 0) NN_REACH("gated_forward", ldx, es);
   }
   NN_REQUIRE(!saved || aligned16(saved, 0), "gated_forward: saved has to start at a 16-byte boundary");
   const int64_t need = sdfnn_gated_workspace_size(dtype, rows, dim, hidden, out, 0);
@@ -488,6 +494,8 @@ int sdfnn_gated_backward(const void* x, int64_t ldx, const void* w_gate, const v
   NN_REQUIRE(es == 4 || ((out % 8 || aligned16(dy, lddy * es)) && (hidden % 8 || aligned16(w_down, 0)) &&
                          (dim % 8 || (aligned16(x, ldx * es) && aligned16(w_gate, 0) && aligned16(w_up, 0)))),
              "gated_backward: rows of a multiple of 8 elements have to start at 16-byte boundaries");
+  if (es == 2 && dim % 8 == 0) NN_REACH("gated_backward", ldx, es);
+  if (es == 2 && out % 8 == 0) NN_REACH("gated_backward", lddy, es);
   NN_REQUIRE(aligned16(saved, 0), "gated_backward: saved has to start at a 16-byte boundary");
   const int64_t need = sdfnn_gated_workspace_size(dtype, rows, dim, hidden, out, 1);
   NN_REQUIRE(need == 0 || (workspace && aligned16(workspace, 0) && workspace_bytes >= need),

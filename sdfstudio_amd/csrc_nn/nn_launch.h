@@ -86,7 +86,6 @@ int product(Call& c, const Operand& a, const Operand& b0, const Operand& b1, con
   const int64_t ld = (DUAL ? 2 : 1) * round_up(N, 64);
   char* part = t.splits > 1 ? c.take((int64_t)t.splits * M * ld * 4) : nullptr;
   if (c.dry() || M == 0 || N == 0) return 0;
-  NN_REQUIRE(256 * std::max(a.ld, std::max(b0.ld, b1.ld)) < 0x7fffffff, "rows of more than 8 MiB are not supported");
   NN_REQUIRE((int64_t)t.gm * t.gn * t.splits < (int64_t)1 << 24 && nk * TERMS < 0x7fffffff, "too many tiles");
   if (t.splits == 1) {
     GemmArgs<EPI> g{a, {b0, b1}, M, (int)N, (int)nk, (int)turn, 0, 0, 0, 0, epi};

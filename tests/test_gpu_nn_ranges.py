@@ -80,3 +80,34 @@ def test_16_bit_gelu_holds_its_relative_accuracy(device, t, rows):
     z = -x.double()
     # 2^-12 for log2 of the tail's polynomial (1.3e-4), its exponent of up to 113 rounded twice (1e-5) and the exponential (2^-23)
     close("gelu", y[:, 0], ACTS["gelu"](z) * (z * su), 2.0 ** -126 * 256, half(t) + 2.0 ** -12)
+
+
+@pytest.mark.parametrize("rows", [20, 40])
+def test_rows_of_long_strides(device, rows):
+    """The last token of every sequence of a batch: rows 8 MiB apart and more give what their copies give, forward and backward."""
+    from sdfstudio_amd.field_components.mlp import gated_mlp
+    from sdfstudio_amd.field_components.normalization import rms_norm
+    from sdfstudio_amd.field_components.quantization import int8_gated_linear, int8_linear, quantize_rows
+
+    base = torch.empty(rows, 1025, 4096, device="cuda", dtype=BF16)
+    x = base[:, -1]
+    x.copy_(torch.randn(rows, 4096, device="cuda"))
+    c = x.contiguous()
+    ws = [torch.randn(72, 4096, device="cuda").div_(64).to(BF16), torch.randn(72, 4096, device="cuda").div_(64).to(BF16), torch.randn(4096, 72, device="cuda").to(BF16)]
+    dy = base[:, 1]  # as far apart
+    dy.copy_(torch.randn(rows, 4096, device="cuda"))
+    got, want = [], []
+    for a, d, out in ((x, dy, got), (c, dy.contiguous(), want)):
+        leaves = [v.detach().requires_grad_(True) for v in (a, *ws)]
+        y = gated_mlp(*leaves)
+        out += [y, *torch.autograd.grad(y, leaves, d), rms_norm(a, ws[0][0]), *quantize_rows(a)]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del base, x, dy
+    base = torch.empty(rows, 2050, 4096, device="cuda", dtype=torch.int8)
+    q, s = base[:, -1], torch.rand(rows, device="cuda")
+    q.copy_(torch.randint(-127, 128, (rows, 4096), device="cuda"))
+    w, sw = torch.randint(-127, 128, (40, 4096), device="cuda", dtype=torch.int8), torch.rand(40, device="cuda")
+    assert torch.equal(int8_linear(q, s, w, sw), int8_linear(q.contiguous(), s, w, sw))
+    assert torch.equal(int8_gated_linear(q, s, w, sw, w, sw), int8_gated_linear(q.contiguous(), s, w, sw, w, sw))
+    few = base[:3, -1]  # as weights
+    assert torch.equal(int8_linear(w, sw, few, s[:3]), int8_linear(w, sw, few.contiguous(), s[:3]))
