@@ -8,6 +8,7 @@ import os
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SDFNN_LIB", os.path.join(_HERE, "libsdfnn.so"))
@@ -136,6 +137,26 @@ def differentiated(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether a call on these is recorded for a backward pass.  (Inside an autograd function it cannot be told: its needs_input_grad does not
     know about torch.no_grad().)"""
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# whether torch.jit.trace is recording: it keeps autograd functions as calls, nothing else of these operators
+traced = torch._C._is_tracing
+_modes = torch._C._len_torch_dispatch_stack
+
+
+def check_modes(what: str, *tensors: Optional[torch.Tensor], function: bool = False) -> None:
+    """Refuses what torch would take further without knowing that a kernel was there: tangents of forward-mode differentiation, which the result
+    would have lost, and graphs recorded tensor operation by tensor operation (make_fx; torch.jit.trace, unless the call is an autograd `function`),
+    which would hold the allocation of the outputs alone."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+    if _modes():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode  # (takes a second; here it has been imported)
+
+        if get_proxy_mode() is not None:
+            raise SdfNnError(f"{what} runs on the sdfnn kernels, which a graph of torch operations (make_fx) cannot hold")
+    if not function and traced():
+        raise SdfNnError(f"{what} runs on the sdfnn kernels, which torch.jit.trace cannot record")
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device

@@ -84,7 +84,8 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         raise ValueError(f"{what}: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_down {tuple(w_down.shape)} do not chain")
     if not (x.dtype == w_gate.dtype == w_up.dtype == w_down.dtype):
         raise TypeError(f"{what}: x {x.dtype}, weights {w_gate.dtype}, {w_up.dtype}, {w_down.dtype}: one type")
-    if not _nn.differentiated(x, w_gate, w_up, w_down):
+    _nn.check_modes(what, x, w_gate, w_up, w_down, function=True)
+    if not _nn.differentiated(x, w_gate, w_up, w_down) and not _nn.traced():
         return _forward(x, w_gate, w_up, w_down, act, False)[0]
     return _GatedMLP.apply(x, w_gate, w_up, w_down, act)
 

@@ -79,7 +79,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     Returns y, with a residual (y, h).  x [..., dim] in float32 / bfloat16 / float16, weight [dim] and residual of the same type; gradients
     for x, weight and residual (one pass; not differentiable twice)."""
     _check("rms_norm", x, weight, residual)
-    if not _nn.differentiated(x, weight, residual):
+    _nn.check_modes("rms_norm", x, weight, residual, function=True)
+    if not _nn.differentiated(x, weight, residual) and not _nn.traced():
         y, h, _ = _forward(x, weight, residual, float(eps), False)
         return y if residual is None else (y, h)
     return _RMSNorm.apply(x, weight, residual, float(eps))
@@ -93,6 +94,7 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, residual: Optional
 
 
 def _quantize(what: str, x: torch.Tensor, weight: Optional[torch.Tensor], residual: Optional[torch.Tensor], eps: float):
+    _nn.check_modes(what, x, weight, residual)
     lib, code = _nn.load(), _nn.dtype_code(x, what)
     dev = _nn.on_device(what, x, weight, residual)
     with _nn.on(dev) as cur:

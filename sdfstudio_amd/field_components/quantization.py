@@ -48,6 +48,7 @@ def int8_linear(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, w
     float32 [...], weight_q int8 [n, k] with weight_scales float32 [n], bias float32 [n]."""
     what = "int8_linear"
     _prepare(what, q, scales, {"weight_q": (weight_q, weight_scales)}, out_dtype)
+    _nn.check_modes(what, scales, weight_scales, bias)
     n = weight_q.shape[0]
     if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (n,)):
         raise ValueError(f"{what}: bias {tuple(bias.shape)} {bias.dtype} for {n} channels: float32")
@@ -72,6 +73,7 @@ def int8_gated_linear(q: torch.Tensor, scales: torch.Tensor, gate_q: torch.Tenso
     """activation(gate) * up of two int8_linear products of the same rows, in one kernel: neither product is written out."""
     what = "int8_gated_linear"
     _prepare(what, q, scales, {"gate_q": (gate_q, gate_scales), "up_q": (up_q, up_scales)}, out_dtype)
+    _nn.check_modes(what, scales, gate_scales, up_scales)
     if gate_q.shape != up_q.shape:
         raise ValueError(f"{what}: gate_q {tuple(gate_q.shape)} and up_q {tuple(up_q.shape)}")
     act = _nn.activation_code(activation, what)

@@ -40,3 +40,83 @@ def test_c_abi_refuses_rows_far_apart_before_it_launches():
         for rows in (4, 40):
             refused(lib.sdfnn_gated_backward(P, far16, P, P, P, P, P, 64, 1, rows, 64, hidden, 64, P, P, P, P, P, big, None))
             refused(lib.sdfnn_gated_backward(P, 64, P, P, P, P, P, far16, 1, rows, 64, hidden, 64, P, P, P, P, P, big, None))
+
+
+def every_operator():
+    """name -> (call, its floating tensors), on the CPU: what is refused here is refused before the device is looked at."""
+    from sdfstudio_amd.field_components.mlp import gated_mlp
+    from sdfstudio_amd.field_components.normalization import rms_norm, rms_norm_quantized
+    from sdfstudio_amd.field_components.quantization import int8_gated_linear, int8_linear, quantize_rows
+
+    x, w, r = torch.randn(4, 8), torch.ones(8), torch.randn(4, 8)
+    q, s, sw, b = torch.ones(4, 8, dtype=torch.int8), torch.ones(4), torch.ones(4), torch.ones(4)
+    return {
+        "rms_norm": (lambda x, w, r: rms_norm(x, w, residual=r), (x, w, r)),
+        "rms_norm_quantized": (lambda x, w, r: rms_norm_quantized(x, w, residual=r), (x, w, r)),
+        "quantize_rows": (quantize_rows, (x,)),
+        "int8_linear": (lambda s, sw, b: int8_linear(q, s, q, sw, bias=b), (s, sw, b)),
+        "int8_gated_linear": (lambda s, sg, su: int8_gated_linear(q, s, q, sg, q, su), (s, sw, sw.clone())),
+        "gated_mlp": (lambda x, g, u, d: gated_mlp(x, g, u, d), (x, torch.randn(6, 8), torch.randn(6, 8), torch.randn(5, 6))),
+    }
+
+
+@pytest.mark.parametrize("name", list(every_operator()))
+def test_forward_mode_is_refused(name):
+    """A tangent of any input: there is no forward-mode derivative, and a result without a tangent would be a constant to what follows."""
+    from torch.autograd import forward_ad
+
+    call, tensors = every_operator()[name]
+    for i in range(len(tensors)):
+        with forward_ad.dual_level():
+            args = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(tensors)]
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(*args)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call(*args)
+    with forward_ad.dual_level(), pytest.raises(_nn.SdfNnError, match="no CPU"):
+        call(*tensors)  # no tangent: as ever
+
+
+@pytest.mark.parametrize("name", list(every_operator()))
+def test_graphs_of_operations_are_refused(name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+
+    call, tensors = every_operator()[name]
+    with pytest.raises(_nn.SdfNnError, match="make_fx"):
+        make_fx(call)(*tensors)
+    with FlopCounterMode(display=False), pytest.raises(_nn.SdfNnError, match="no CPU"):  # other modes see the call as ever
+        call(*tensors)
+
+
+@pytest.mark.parametrize("name", ["rms_norm_quantized", "quantize_rows", "int8_linear", "int8_gated_linear"])
+def test_traces_of_8_bit_calls_are_refused(name):
+    call, tensors = every_operator()[name]
+    with torch.no_grad(), pytest.raises(_nn.SdfNnError, match="jit.trace"):
+        torch.jit.trace(call, tensors, check_trace=False)
+
+
+def test_traces_keep_the_calls(monkeypatch):
+    """torch.jit.trace keeps rms_norm and gated_mlp as calls, also under torch.no_grad(): a replay on other values computes theirs.  The kernels are
+    replaced by their formulas here."""
+    from sdfstudio_amd.field_components import mlp, normalization
+
+    def norm(x, weight, residual, eps, save):
+        h = x.detach().numpy() + residual.detach().numpy()  # (numpy: as invisible to a trace as a kernel)
+        y = torch.from_numpy(h * weight.detach().numpy())
+        return y, torch.from_numpy(h), torch.ones(len(h)) if save else None
+
+    def gated(x, w_gate, w_up, w_down, act, save):
+        n = [t.detach().numpy() for t in (x, w_gate, w_up, w_down)]
+        return torch.from_numpy(((n[0] @ n[1].T) * (n[0] @ n[2].T)) @ n[3].T), torch.ones(1) if save else None
+
+    monkeypatch.setattr(normalization, "_forward", norm)
+    monkeypatch.setattr(mlp, "_forward", gated)
+    for name in ("rms_norm", "gated_mlp"):
+        call, tensors = every_operator()[name]
+        with torch.no_grad():
+            graph = torch.jit.trace(call, tensors, check_trace=False)
+            other = [torch.randn_like(t) for t in tensors]
+            got, want = graph(*other), call(*other)
+            for a, b in zip(got if isinstance(got, tuple) else [got], want if isinstance(want, tuple) else [want]):
+                assert torch.equal(a, b)
