@@ -159,6 +159,14 @@ def check_modes(what: str, *tensors: Optional[torch.Tensor], function: bool = Fa
         raise SdfNnError(f"{what} runs on the sdfnn kernels, which torch.jit.trace cannot record")
 
 
+def check_no_gradient(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses a call that would be recorded for a backward pass, by an operator that has none."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise SdfNnError(f"{what} has no gradient: call it under torch.no_grad() or on tensors that require none")
+
+
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 

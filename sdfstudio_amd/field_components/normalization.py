@@ -88,8 +88,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
 
 def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
     """rms_norm with its output in 8 bits: codes int8 [..., dim] in [-127, 127] and scales float32 [...], codes * scales = y to half a step
-    of max|y| / 127 a row.  Returns (codes, scales), with a residual (codes, scales, h).  For serving: no gradients."""
+    of max|y| / 127 a row.  Returns (codes, scales), with a residual (codes, scales, h).  For serving: it has no gradients, and a call that would
+    need them is refused."""
     _check("rms_norm_quantized", x, weight, residual)
+    _nn.check_no_gradient("rms_norm_quantized", x, weight, residual)
     return _quantize("rms_norm_quantized", x, weight, residual, float(eps))
 
 

@@ -14,7 +14,8 @@ MAX_K = 131072  # 127 * 127 * k stays below 2^31
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x [..., dim] -> (codes int8 [..., dim] in [-127, 127], scales float32 [...]): code = round(127 x / max|x|) half to even, scale =
-    max|x| / 127 of its row (a row of zeros: scale 0).  Serves activations (a scale a token) and weights [out, in] (a scale a channel)."""
+    max|x| / 127 of its row (a row of zeros: scale 0).  Serves activations (a scale a token) and weights [out, in] (a scale a channel).  Both results
+    are constants to autograd, as rounded values are."""
     _check("quantize_rows", x, None, None)
     return _quantize("quantize_rows", x, None, None, 0.0)
 
@@ -45,10 +46,11 @@ def _prepare(what, q, scales, weights, out_dtype):
 def int8_linear(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, weight_scales: torch.Tensor,
                 bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """y[..., n] = (sum_k q[..., k] weight_q[n, k]) scales[...] weight_scales[n] + bias[n] in out_dtype.  q int8 [..., k] with scales
-    float32 [...], weight_q int8 [n, k] with weight_scales float32 [n], bias float32 [n]."""
+    float32 [...], weight_q int8 [n, k] with weight_scales float32 [n], bias float32 [n].  No gradients: scales or a bias that would need one are refused."""
     what = "int8_linear"
     _prepare(what, q, scales, {"weight_q": (weight_q, weight_scales)}, out_dtype)
     _nn.check_modes(what, scales, weight_scales, bias)
+    _nn.check_no_gradient(what, scales, weight_scales, bias)
     n = weight_q.shape[0]
     if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (n,)):
         raise ValueError(f"{what}: bias {tuple(bias.shape)} {bias.dtype} for {n} channels: float32")
@@ -74,6 +76,7 @@ def int8_gated_linear(q: torch.Tensor, scales: torch.Tensor, gate_q: torch.Tenso
     what = "int8_gated_linear"
     _prepare(what, q, scales, {"gate_q": (gate_q, gate_scales), "up_q": (up_q, up_scales)}, out_dtype)
     _nn.check_modes(what, scales, gate_scales, up_scales)
+    _nn.check_no_gradient(what, scales, gate_scales, up_scales)
     if gate_q.shape != up_q.shape:
         raise ValueError(f"{what}: gate_q {tuple(gate_q.shape)} and up_q {tuple(up_q.shape)}")
     act = _nn.activation_code(activation, what)

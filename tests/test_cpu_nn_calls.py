@@ -120,3 +120,19 @@ def test_traces_keep_the_calls(monkeypatch):
             got, want = graph(*other), call(*other)
             for a, b in zip(got if isinstance(got, tuple) else [got], want if isinstance(want, tuple) else [want]):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("name", ["rms_norm_quantized", "int8_linear", "int8_gated_linear"])
+def test_calls_without_a_backward_refuse_what_needs_one(name):
+    """Each floating input in turn requires a gradient: refused, and served under torch.no_grad() (up to the device)."""
+    call, tensors = every_operator()[name]
+    for i in range(len(tensors)):
+        args = [t.clone().requires_grad_(i == j) for j, t in enumerate(tensors)]
+        with pytest.raises(_nn.SdfNnError, match="no gradient"):
+            call(*args)
+        with torch.no_grad(), pytest.raises(_nn.SdfNnError, match="no CPU"):
+            call(*args)
+    from sdfstudio_amd.field_components.normalization import RMSNorm
+
+    with pytest.raises(_nn.SdfNnError, match="no gradient"):
+        RMSNorm(8).quantized(torch.randn(4, 8))  # its weight is a parameter
