@@ -17,6 +17,7 @@ import torch
 
 from sdfstudio_amd import _lib
 from sdfstudio_amd.distributed import FlatGradients
+from sdfstudio_amd.grad_slots import WRITES_ATTR
 
 
 # ---------------------------------------------------------------------------------------------- schedulers (multiplicative factors)
@@ -80,6 +81,9 @@ class FlatParameters:
                 off, n = self.offset[id(p)], p.numel()
                 self.flat[off:off + n].copy_(p.data.reshape(-1))
                 p.data = self.flat[off:off + n].view_as(p)
+        self.writes = [0]  # steps taken on the buffer, as its parameters know them (grad_slots.parameter_state)
+        for p in self.params:
+            setattr(p, WRITES_ATTR, self.writes)
 
 
 class FusedAdam:
@@ -155,6 +159,7 @@ class FusedAdam:
         asynchronous: FlatGradients.wait_parameters) - so that the first chunks' parameters travel while the later chunks' gradients
         are still arriving."""
         self.step_count += 1
+        self.flat_params.writes[0] += 1
         self.last_elements_visited = 0
         self._gathered = None  # moments assembled for a checkpoint (gather_moments) are stale from here on
         fg = self.flat_grads

@@ -16,6 +16,7 @@ from torch import nn
 from sdfstudio_amd import _nn
 from sdfstudio_amd.field_components.normalization import RMSNorm
 from sdfstudio_amd.field_components.quantization import Int8Linear, int8_gated_linear, quantize_rows
+from sdfstudio_amd.grad_slots import parameter_state
 
 
 def _forward(x, w_gate, w_up, w_down, act, save):
@@ -126,8 +127,10 @@ class GatedStack(nn.Module):
     """num_blocks pre-norm residual blocks  h <- h + mlp(norm(h))  and a last norm.  Every addition happens inside the norm that follows it.
 
     quantize() makes the 8-bit serving form: from then on a call that needs no gradient (torch.no_grad()) runs the blocks on 8-bit products,
-    with weights quantised from the parameters as they are now; training calls are unaffected, and parameters that change afterwards need another
-    quantize().  dequantize() drops it.  Moving the module to another device or type makes the form anew there (on the CPU: drops it)."""
+    with weights quantised from the parameters as they are now; training calls are unaffected.  Parameters that have changed since - an optimiser's
+    step, load_state_dict - need another quantize(): until then such a call raises, since it would mix old blocks with new norms.  (Writes through
+    .data or a raw address, and replays of a captured graph, are not seen.)  dequantize() drops the form.  Moving the module to another device or type
+    makes it anew there (on the CPU: drops it)."""
 
     def __init__(self, dim: int, hidden_dim: int, num_blocks: int, activation: str = "silu", eps: float = 1e-6) -> None:
         super().__init__()
@@ -136,10 +139,21 @@ class GatedStack(nn.Module):
         self.norms = nn.ModuleList(RMSNorm(dim, eps) for _ in range(num_blocks + 1))
         self.mlps = nn.ModuleList(GatedMLP(dim, hidden_dim, dim, activation) for _ in range(num_blocks))
         self._served = None  # a plain list, not submodules: state_dict holds the parameters alone
+        self._served_from = None  # the weights' parameter_state then; None: not known yet, taken at the next call
+
+    def _weights_state(self) -> list:
+        return [parameter_state(p) for m in self.mlps for p in (m.w_gate, m.w_up, m.w_down)]
 
     def quantize(self) -> "GatedStack":
         self._served = [Int8GatedMLP(m) for m in self.mlps]
+        self._served_from = self._weights_state()
         return self
+
+    def __getstate__(self):
+        state = self.__dict__.copy()  # a copy's weights lie elsewhere: it knows only whether its form was up to date
+        if self._served is not None and self._served_from is not None:
+            state["_served_from"] = None if self._served_from == self._weights_state() else []
+        return state
 
     def dequantize(self) -> "GatedStack":
         self._served = None
@@ -156,6 +170,12 @@ class GatedStack(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         h, delta = x, None
         serve = self._served is not None and not torch.is_grad_enabled()
+        if serve:
+            now = self._weights_state()
+            if self._served_from is None:
+                self._served_from = now
+            elif self._served_from != now:
+                raise _nn.SdfNnError("GatedStack: the weights have changed or moved since quantize(): call it again, or dequantize()")
         for i, norm in enumerate(self.norms[:-1]):
             out = norm.quantized(h, delta) if serve else norm(h, delta)
             if delta is not None:

@@ -19,6 +19,13 @@ import torch
 
 SLOT_ATTR = "_sdfhip_grad_slot"        # callable() -> fresh view of the flat gradient buffer, set by FlatGradients
 CLAIM_ATTR = "_sdfhip_slot_claimed"    # True once a producer has written the slot in this backward pass
+WRITES_ATTR = "_sdfhip_writes"         # [count] of the writes of a fused optimiser, which autograd's version counters do not see
+
+
+def parameter_state(p: torch.Tensor) -> tuple:
+    """What tells whether a parameter is still what it was: where it lies, autograd's count of the writes to it, and the fused optimiser's.  (Writes
+    through p.data or a raw address leave no trace.)"""
+    return p.data_ptr(), 0 if p.is_inference() else p._version, getattr(p, WRITES_ATTR, (0,))[0]
 
 
 def grad_target(p: torch.Tensor, zero_init: bool = False) -> Tuple[torch.Tensor, bool]:

@@ -136,3 +136,63 @@ def test_calls_without_a_backward_refuse_what_needs_one(name):
 
     with pytest.raises(_nn.SdfNnError, match="no gradient"):
         RMSNorm(8).quantized(torch.randn(4, 8))  # its weight is a parameter
+
+
+def test_a_served_form_knows_its_weights(monkeypatch):
+    """After an optimiser's step, a load or a move the 8-bit form of a stack is refused until it is made again; training calls, copies and pickles are
+    unaffected.  (Kernels left out: the blocks are the identity.)"""
+    import copy
+    import pickle
+
+    from sdfstudio_amd.engine.optimizers import FlatParameters
+    from sdfstudio_amd.field_components import mlp
+
+    monkeypatch.setattr(mlp, "Int8GatedMLP", IdentityBlock)
+    monkeypatch.setattr(mlp.RMSNorm, "quantized", lambda self, x, r=None: (x, None) if r is None else (x, None, x))
+    monkeypatch.setattr(mlp.RMSNorm, "forward", lambda self, x, r=None: (x, x))
+    stack, x = mlp.GatedStack(8, 6, 2), torch.randn(3, 8)
+
+    def serve(s=stack):
+        with torch.no_grad():
+            return s(x)
+
+    def stale(s=stack):
+        with pytest.raises(_nn.SdfNnError, match="since quantize"):
+            serve(s)
+
+    stack.quantize()
+    serve(), serve()
+    for p in (stack.mlps[1].w_down, stack.mlps[0].w_gate):  # torch's optimisers write in place
+        with torch.no_grad():
+            p.add_(1.0)
+        stale()
+        stale(copy.deepcopy(stack)), stale(pickle.loads(pickle.dumps(stack)))
+        serve(copy.deepcopy(stack.quantize())), serve(pickle.loads(pickle.dumps(stack))), serve()
+    other = copy.deepcopy(stack)
+    serve(other)
+    with torch.no_grad():
+        other.mlps[0].w_up.zero_()
+    stale(other), serve()
+    stack.load_state_dict(other.state_dict())
+    stale()
+    stack.quantize().load_state_dict(other.state_dict(), assign=True)
+    stale()
+    with torch.no_grad():
+        stack.quantize().norms[0].weight.add_(1.0)  # read as it is
+    serve()
+    flat = FlatParameters(stack.parameters())  # (moves them)
+    stale()
+    serve(stack.quantize())
+    flat.writes[0] += 1  # what FusedAdam.step does
+    stale()
+    stack.dequantize()
+    monkeypatch.setattr(mlp.GatedMLP, "forward", lambda self, x: x)
+    serve()
+
+
+class IdentityBlock:
+    def __init__(self, m):
+        pass
+
+    def __call__(self, q, scales, t):
+        return q

@@ -22,3 +22,39 @@ def test_traces_replay_on_other_values(device):
             for _ in range(2):
                 other = draw()
                 assert torch.equal(graph(*other), block(*other))
+
+
+def test_a_served_stack_follows_its_weights(device):
+    """quantize(), then a step of the fused optimiser or load_state_dict: the next served call raises, and after another quantize() equals that of a
+    stack that has held these weights from the start."""
+    import copy
+
+    from sdfstudio_amd._nn import SdfNnError
+    from sdfstudio_amd.engine.optimizers import Optimizers
+    from sdfstudio_amd.field_components.mlp import GatedStack
+
+    stack, x = GatedStack(64, 96, 2).to(device), torch.randn(50, 64, device=device)
+    opts = Optimizers({"blocks": {"lr": 0.1}}, {"blocks": list(stack.parameters())})
+
+    def check():
+        with torch.no_grad():
+            with pytest.raises(SdfNnError, match="since quantize"):
+                stack(x)
+            y = stack.quantize()(x)
+            fresh = GatedStack(64, 96, 2).to(device)
+            fresh.load_state_dict(stack.state_dict())
+            assert torch.equal(y, fresh.quantize()(x)) and torch.equal(y, copy.deepcopy(stack)(x)) and torch.equal(y, stack(x))
+
+    before = copy.deepcopy(stack.state_dict())
+    stack.quantize()
+    for _ in range(2):
+        opts.zero_grad_all()
+        stack(x).square().sum().backward()
+        opts.optimizer_step_all()
+        check()
+    assert not torch.equal(before["mlps.0.w_up"], stack.mlps[0].w_up)
+    stack.load_state_dict(before)
+    check()
+    stack.to(torch.bfloat16)  # makes the form anew
+    with torch.no_grad():
+        assert stack(x.bfloat16()).dtype == torch.bfloat16
