@@ -55,6 +55,9 @@ int sdfnn_rms_norm_quantize(const void* x, int64_t ldx, const void* residual, in
  * of -128 are allowed up to k = 131071), the rest in fp32.  q [rows, k] (stride ldq), w [n, k] (stride ldw), bias [n] fp32 or NULL,
  * y [rows, n] contiguous in `dtype`.  workspace: sdfnn_int8_linear_workspace_size(rows, n, k, projections) bytes. */
 int64_t sdfnn_int8_linear_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t projections);
+/* Which kernel the product takes, for tests and traces: 256 or 128, the side of its tiles, or 0, the kernel of few rows (-1: refused); *splits (may be
+ * NULL): over how many workgroups k is split.  Nothing is launched. */
+int32_t sdfnn_int8_product(int64_t rows, int64_t n, int64_t k, int32_t projections, int32_t* splits);
 int sdfnn_int8_linear(const int8_t* q, int64_t ldq, const float* sq, const int8_t* w, int64_t ldw, const float* sw, const float* bias,
                       int32_t dtype, int64_t rows, int64_t n, int64_t k, void* y, void* workspace, int64_t workspace_bytes,
                       sdfnn_stream_t stream);
@@ -74,6 +77,9 @@ int sdfnn_int8_gated_linear(const int8_t* q, int64_t ldq, const float* sq, const
  * their three parts); NULL when none will follow. */
 int64_t sdfnn_gated_saved_size(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden);
 int64_t sdfnn_gated_workspace_size(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden, int64_t out, int32_t backward);
+/* As sdfnn_int8_product, of product `index` of a pass.  Forward: 0 gate and up, 1 down; backward: 0 the gradients of g and u, 1 dx, 2 dw_down,
+ * 3 dw_gate and dw_up. */
+int32_t sdfnn_gated_product(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden, int64_t out, int32_t backward, int32_t index, int32_t* splits);
 int sdfnn_gated_forward(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* w_down, int32_t dtype, int32_t act,
                         int64_t rows, int64_t dim, int64_t hidden, int64_t out, void* saved, void* y, void* workspace,
                         int64_t workspace_bytes, sdfnn_stream_t stream);

@@ -22,10 +22,12 @@ _SIGNATURES = {
     "sdfnn_rms_norm_backward": (ctypes.c_int, [_p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _i64, _i32, _i64, _i64, _p, _p, _p, _i64, _p]),
     "sdfnn_rms_norm_quantize": (ctypes.c_int, [_p, _i64, _p, _i64, _p, _i32, _i64, _i64, _f32, _p, _p, _p, _p]),
     "sdfnn_int8_linear_workspace_size": (_i64, [_i64, _i64, _i64, _i32]),
+    "sdfnn_int8_product": (_i32, [_i64, _i64, _i64, _i32, _p]),
     "sdfnn_int8_linear": (ctypes.c_int, [_p, _i64, _p, _p, _i64, _p, _p, _i32, _i64, _i64, _i64, _p, _p, _i64, _p]),
     "sdfnn_int8_gated_linear": (ctypes.c_int, [_p, _i64, _p, _p, _i64, _p, _p, _i64, _p, _i32, _i32, _i64, _i64, _i64, _p, _p, _i64, _p]),
     "sdfnn_gated_saved_size": (_i64, [_i32, _i64, _i64, _i64]),
     "sdfnn_gated_workspace_size": (_i64, [_i32, _i64, _i64, _i64, _i64, _i32]),
+    "sdfnn_gated_product": (_i32, [_i32, _i64, _i64, _i64, _i64, _i32, _i32, _p]),
     "sdfnn_gated_forward": (ctypes.c_int, [_p, _i64, _p, _p, _p, _i32, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p]),
     "sdfnn_gated_backward": (ctypes.c_int, [_p, _i64, _p, _p, _p, _p, _p, _i64, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p]),
 }

@@ -341,6 +341,29 @@ int check_gated(const char* what, const int32_t dtype, const int32_t act, const 
   return 0;
 }
 
+// What a call needs and which kernels it takes, without launching anything
+int plan_int8(Call& c, const int64_t rows, const int64_t n, const int64_t k, const int32_t projections) {
+  if (rows < 0 || rows > kMaxRows || n < 1 || n > kMaxDim || k < 1 || k > 131072 || projections < 1 || projections > 2) return -1;
+  const Int8Epi<SDFNN_F32> epi{};
+  if (projections == 1) return int8_products<SDFNN_F32, false>(c, nullptr, k, nullptr, k, nullptr, k, rows, n, k, epi);
+  return int8_products<SDFNN_F32, true>(c, nullptr, k, nullptr, k, nullptr, k, rows, n, k, epi);
+}
+int plan_gated(Call& c, const char* what, const int32_t dtype, const int64_t rows, const int64_t dim, const int64_t hidden, const int64_t out,
+               const int32_t backward) {
+  NN_TRY(check_gated(what, dtype, 0, rows, dim, hidden, out));
+  char some = 0;
+  return by_dtype(dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (backward) return gated_backward<DT>(c, nullptr, dim, nullptr, nullptr, nullptr, nullptr, nullptr, out, rows, dim, hidden, out, &some, &some, &some, &some);
+    return gated_forward<DT>(c, nullptr, dim, nullptr, nullptr, nullptr, 0, rows, dim, hidden, out, nullptr, nullptr);
+  });
+}
+int32_t product_of(const Call& c, const int32_t index, int32_t* splits) {
+  NN_REQUIRE(index >= 0 && index < c.products, "product %d of %d", (int)index, c.products);
+  if (splits) *splits = c.splits[index];
+  return c.tile[index];
+}
+
 }  // namespace
 
 extern "C" {
@@ -397,12 +420,13 @@ int sdfnn_rms_norm_quantize(const void* x, int64_t ldx, const void* residual, in
 }
 
 int64_t sdfnn_int8_linear_workspace_size(int64_t rows, int64_t n, int64_t k, int32_t projections) {
-  if (rows < 0 || rows > kMaxRows || n < 1 || n > kMaxDim || k < 1 || k > 131072 || projections < 1 || projections > 2) return -1;
-  Call c{nullptr, 0, nullptr};
-  const Int8Epi<SDFNN_F32> epi{};
-  if (projections == 1) int8_products<SDFNN_F32, false>(c, nullptr, k, nullptr, k, nullptr, k, rows, n, k, epi);
-  else int8_products<SDFNN_F32, true>(c, nullptr, k, nullptr, k, nullptr, k, rows, n, k, epi);
-  return c.used;
+  Call c{};
+  return plan_int8(c, rows, n, k, projections) ? -1 : c.used;
+}
+
+int32_t sdfnn_int8_product(int64_t rows, int64_t n, int64_t k, int32_t projections, int32_t* splits) {
+  Call c{};
+  return plan_int8(c, rows, n, k, projections) ? -1 : product_of(c, 0, splits);
 }
 
 int sdfnn_int8_linear(const int8_t* q, int64_t ldq, const float* sq, const int8_t* w, int64_t ldw, const float* sw, const float* bias,
@@ -447,15 +471,13 @@ int64_t sdfnn_gated_saved_size(int32_t dtype, int64_t rows, int64_t dim, int64_t
 }
 
 int64_t sdfnn_gated_workspace_size(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden, int64_t out, int32_t backward) {
-  if (check_gated("gated_workspace_size", dtype, 0, rows, dim, hidden, out)) return -1;
-  Call c{nullptr, 0, nullptr};
-  char some = 0;
-  by_dtype(dtype, [&](auto dt) {
-    constexpr int DT = decltype(dt)::value;
-    if (backward) return gated_backward<DT>(c, nullptr, dim, nullptr, nullptr, nullptr, nullptr, nullptr, out, rows, dim, hidden, out, &some, &some, &some, &some);
-    return gated_forward<DT>(c, nullptr, dim, nullptr, nullptr, nullptr, 0, rows, dim, hidden, out, nullptr, nullptr);
-  });
-  return c.used;
+  Call c{};
+  return plan_gated(c, "gated_workspace_size", dtype, rows, dim, hidden, out, backward) ? -1 : c.used;
+}
+
+int32_t sdfnn_gated_product(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden, int64_t out, int32_t backward, int32_t index, int32_t* splits) {
+  Call c{};
+  return plan_gated(c, "gated_product", dtype, rows, dim, hidden, out, backward) ? -1 : product_of(c, index, splits);
 }
 
 int sdfnn_gated_forward(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* w_down, int32_t dtype, int32_t act,

@@ -11,6 +11,8 @@ struct Call {
   char* base;
   int64_t used;
   hipStream_t stream;
+  int tile[4], splits[4], products;  // of its products in their order (tile 0: a kernel of few rows), for the queries
+  void note(const int t, const int s) { tile[products & 3] = t, splits[products++ & 3] = s; }
   bool dry() const { return base == nullptr; }
   char* take(const int64_t bytes) {
     char* p = base + used;  // dry: never dereferenced
@@ -83,6 +85,7 @@ template <int KIND, int TERMS, bool DUAL, int SIDES, class EPI>
 int product(Call& c, const Operand& a, const Operand& b0, const Operand& b1, const int64_t M, const int64_t N, const int64_t nk, const int64_t turn,
             const EPI& epi) {
   const Tiling t = choose_tiling(M, DUAL ? 2 * N : N, (int)nk, TERMS, EPI::kCost);
+  c.note(t.tile, t.splits);
   const int64_t ld = (DUAL ? 2 : 1) * round_up(N, 64);
   char* part = t.splits > 1 ? c.take((int64_t)t.splits * M * ld * 4) : nullptr;
   if (c.dry() || M == 0 || N == 0) return 0;
@@ -108,6 +111,7 @@ constexpr int64_t few_rows(const int kind) { return kind == 3 ? 64 : 32; }
 // the same for at most few_rows(KIND) rows.  cols: columns that the epilogue writes (>= N).  PAIR: M rows of a, each result the sum of two
 template <int KIND, bool DUAL, bool PAIR = false, class EPI>
 int skinny(Call& c, const Operand& a, const Operand& b0, const Operand& b1, const int64_t M, const int64_t N, const int64_t cols, const EPI& epi) {
+  c.note(0, 1);
   if (c.dry() || M == 0 || N == 0) return 0;
   GemmArgs<EPI> g{a, {b0, b1}, M, (int)N, 0, 0, 0, 0, 0, 0, epi};
   const dim3 grid((unsigned)ceil_div(cols, 16)), block(kSkinnyWaves * 64);
@@ -127,6 +131,7 @@ int skinny_down(Call& c, const Operand& a, const Operand& b0, const Operand& b1,
   const int64_t want = std::max<int64_t>(1, std::min(units / (2 * kDownWaves), 1024 / cols)), per = ceil_div(units, want), splits = ceil_div(units, per);
   const int64_t ld = round_up(N, 64);
   char* part = splits > 1 ? c.take(splits * M * ld * 4) : nullptr;
+  c.note(0, (int)splits);
   if (c.dry() || M == 0) return 0;
   auto start = [&](const auto& e) {
     typedef std::remove_cv_t<std::remove_reference_t<decltype(e)>> E;
@@ -150,6 +155,7 @@ int skinny_down(Call& c, const Operand& a, const Operand& b0, const Operand& b1,
 }
 // w[r, c] = sum_m p[m, r] x[m, c] of few fp32 rows into `to`; R rows r (both halves of `to` with what lies between)
 inline int outer(Call& c, const Operand& p, const Operand& x, const int64_t M, const int64_t R, const StoreEpi<SDFNN_F32>& to) {
+  c.note(0, 1);
   if (c.dry() || R == 0) return 0;
   hipLaunchKernelGGL(outer_kernel, dim3((unsigned)ceil_div(to.N, 256), (unsigned)ceil_div(R, 64)), dim3(256), 0, c.stream, OuterArgs{p, x, M, to});
   NN_LAUNCHED("outer product");

@@ -196,3 +196,42 @@ class IdentityBlock:
 
     def __call__(self, q, scales, t):
         return q
+
+
+def product_of(rows, n, k, projections):
+    import ctypes
+
+    splits = ctypes.c_int32(-1)
+    return _nn.load().sdfnn_int8_product(rows, n, k, projections, ctypes.byref(splits)), splits.value
+
+
+def test_the_large_tiles_are_tested():
+    """The shapes of test_gpu_nn_tiles.py reach the 256 x 256 tiles of every product of the gated block, whole along k and split."""
+    from test_gpu_nn_tiles import TILES_16, TILES_F32, TILES_INT8, chosen
+
+    def reached(dtype, shapes):
+        return {(i, split) for s in shapes for i, (tile, split) in enumerate(chosen(dtype, s)) if tile == 256}
+
+    assert reached(0, TILES_F32) == {(i, split) for i in range(6) for split in (False, True)}
+    for dtype in (1, 2):
+        got = reached(dtype, TILES_16)
+        assert {i for i, _ in got} == set(range(6)) and {i for i, split in got if split} >= {1, 3, 4, 5}
+    assert {(s[3], product_of(*s)[1] > 1) for s in TILES_INT8 if product_of(*s)[0] == 256} == {(p, split) for p in (1, 2) for split in (False, True)}
+
+
+def test_the_kernel_is_chosen_by_rows_and_size():
+    """Few rows stream the weights: up to 32 (fp32: 64, both passes); beyond, tiles, also for the backward pass of few 16-bit rows.  Long products take
+    large tiles, narrow ones small tiles, and k is split where tiles are few."""
+    from test_gpu_nn_tiles import chosen
+
+    for rows, few in ((1, True), (32, True), (33, False)):
+        assert (product_of(rows, 4096, 4096, 2)[0] == 0) == few
+        for dtype in (1, 2):
+            assert [t == 0 for t, _ in chosen(dtype, (rows, 512, 1024, 512))] == [few, few, False, False, False, False]
+    for rows, few in ((1, True), (64, True), (65, False)):
+        assert [t == 0 for t, _ in chosen(0, (rows, 512, 1024, 512))] == [few] * 6
+    assert product_of(16384, 8192, 4096, 1) == (256, 1) and product_of(524288, 512, 256, 2) == (128, 1)
+    assert product_of(200, 64, 131072, 1)[1] > 1
+    lib = _nn.load()
+    assert lib.sdfnn_int8_product(1, 1, 0, 1, None) == -1 and lib.sdfnn_gated_product(1, 1, 64, 64, 64, 0, 2, None) == -1
+    assert lib.sdfnn_gated_product(0, 100, 64, 64, 64, 1, 3, None) in (128, 256) and lib.sdfnn_gated_product(5, 1, 64, 64, 64, 0, 0, None) == -1
