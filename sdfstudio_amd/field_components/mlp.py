@@ -79,9 +79,10 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     forward pass keeps twice the type's bits."""
     what = "gated_mlp"
     act = _nn.activation_code(activation, what)
-    if x.dim() < 1 or w_gate.dim() != 2 or w_down.dim() != 2 or w_gate.shape != w_up.shape:
+    sx, sg, sd = x.shape, w_gate.shape, w_down.shape
+    if not sx or len(sg) != 2 or len(sd) != 2 or sg != w_up.shape:
         raise ValueError(f"{what}: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}, w_down {tuple(w_down.shape)}")
-    if w_gate.shape[1] != x.shape[-1] or w_down.shape[1] != w_gate.shape[0] or 0 in w_gate.shape or 0 in w_down.shape:
+    if sg[1] != sx[-1] or sd[1] != sg[0] or 0 in sg or 0 in sd:
         raise ValueError(f"{what}: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_down {tuple(w_down.shape)} do not chain")
     if not (x.dtype == w_gate.dtype == w_up.dtype == w_down.dtype):
         raise TypeError(f"{what}: x {x.dtype}, weights {w_gate.dtype}, {w_up.dtype}, {w_down.dtype}: one type")

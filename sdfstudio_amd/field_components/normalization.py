@@ -13,11 +13,12 @@ from sdfstudio_amd import _nn
 
 
 def _check(what: str, x: torch.Tensor, weight: Optional[torch.Tensor], residual: Optional[torch.Tensor]) -> None:
-    if x.dim() < 1 or x.shape[-1] < 1:
+    shape, dtype = x.shape, x.dtype
+    if not shape or shape[-1] < 1:
         raise ValueError(f"{what}: x {tuple(x.shape)} has no features")
-    if weight is not None and (tuple(weight.shape) != (x.shape[-1],) or weight.dtype != x.dtype):
+    if weight is not None and (weight.shape != (shape[-1],) or weight.dtype is not dtype):
         raise ValueError(f"{what}: weight {tuple(weight.shape)} {weight.dtype} for x {tuple(x.shape)} {x.dtype}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+    if residual is not None and (residual.shape != shape or residual.dtype is not dtype):
         raise ValueError(f"{what}: residual {tuple(residual.shape)} {residual.dtype} for x {tuple(x.shape)} {x.dtype}")
 
 

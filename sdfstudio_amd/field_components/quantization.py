@@ -9,6 +9,7 @@ from torch import nn
 from sdfstudio_amd import _nn
 from sdfstudio_amd.field_components.normalization import _check, _quantize
 
+_CODE, _SCALE = torch.int8, torch.float32
 MAX_K = 131072  # 127 * 127 * k stays below 2^31
 
 
@@ -21,9 +22,6 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 
 def _check_operand(what: str, name: str, q: torch.Tensor, scales: torch.Tensor, k: Optional[int] = None) -> None:
-    if q.dtype == torch.int8 and scales.dtype == torch.float32 and q.dim() == 2 and scales.dim() == 1 and scales.size(0) == q.size(0) and \
-            (k is None or q.size(1) == k):
-        return  # (as nearly always)
     if q.dtype != torch.int8 or q.dim() < 1:
         raise TypeError(f"{what}: {name} {tuple(q.shape)} {q.dtype}: int8 rows expected")
     if k is not None and (q.dim() != 2 or q.shape[1] != k):
@@ -33,10 +31,14 @@ def _check_operand(what: str, name: str, q: torch.Tensor, scales: torch.Tensor, 
 
 
 def _prepare(what, q, scales, weights, out_dtype):
-    _check_operand(what, "q", q, scales)
-    k = q.shape[-1]
-    for name, (w, s) in weights.items():
-        _check_operand(what, name, w, s, k)
+    shape = q.shape
+    k = shape[-1] if shape else 0
+    if not (q.dtype is _CODE and scales.dtype is _SCALE and len(shape) == 2 and scales.shape == (shape[0],)):  # (as nearly always)
+        _check_operand(what, "q", q, scales)
+    for name, w, s in weights:
+        shape = w.shape
+        if not (w.dtype is _CODE and s.dtype is _SCALE and len(shape) == 2 and shape[1] == k and s.shape == (shape[0],)):
+            _check_operand(what, name, w, s, k)
     if not 1 <= k <= MAX_K:
         raise ValueError(f"{what}: k = {k}: the 32-bit sum is exact for 1 .. {MAX_K}")
     if out_dtype not in _nn.DTYPES:
@@ -48,7 +50,7 @@ def int8_linear(q: torch.Tensor, scales: torch.Tensor, weight_q: torch.Tensor, w
     """y[..., n] = (sum_k q[..., k] weight_q[n, k]) scales[...] weight_scales[n] + bias[n] in out_dtype.  q int8 [..., k] with scales
     float32 [...], weight_q int8 [n, k] with weight_scales float32 [n], bias float32 [n].  No gradients: scales or a bias that would need one are refused."""
     what = "int8_linear"
-    _prepare(what, q, scales, {"weight_q": (weight_q, weight_scales)}, out_dtype)
+    _prepare(what, q, scales, (("weight_q", weight_q, weight_scales),), out_dtype)
     _nn.check_modes(what, scales, weight_scales, bias)
     _nn.check_no_gradient(what, scales, weight_scales, bias)
     n = weight_q.shape[0]
@@ -74,7 +76,7 @@ def int8_gated_linear(q: torch.Tensor, scales: torch.Tensor, gate_q: torch.Tenso
                       up_scales: torch.Tensor, activation: str = "silu", out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """activation(gate) * up of two int8_linear products of the same rows, in one kernel: neither product is written out."""
     what = "int8_gated_linear"
-    _prepare(what, q, scales, {"gate_q": (gate_q, gate_scales), "up_q": (up_q, up_scales)}, out_dtype)
+    _prepare(what, q, scales, (("gate_q", gate_q, gate_scales), ("up_q", up_q, up_scales)), out_dtype)
     _nn.check_modes(what, scales, gate_scales, up_scales)
     _nn.check_no_gradient(what, scales, gate_scales, up_scales)
     if gate_q.shape != up_q.shape:
