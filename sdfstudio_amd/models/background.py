@@ -23,6 +23,9 @@ from sdfstudio_amd.model_components.renderers import AccumulationRenderer, Depth
 
 def build_background(model, config) -> None:
     """base_surface_model.py:181-216: field_background, sampler_bg and the per-head renderers on `model`."""
+    if getattr(config, "background_feature_blocks", 0) and config.background_model != "mlp":
+        raise ValueError(f"background_feature_blocks = {config.background_feature_blocks} with background_model = {config.background_model!r}: "
+                         "the blocks are part of the 'mlp' background")
     if config.background_model == "mlp":
         model.field_background = NeRFField(
             position_encoding=NeRFEncoding(in_dim=3, num_frequencies=10, min_freq_exp=0.0, max_freq_exp=9.0, include_input=True),

@@ -235,3 +235,14 @@ def test_the_kernel_is_chosen_by_rows_and_size():
     lib = _nn.load()
     assert lib.sdfnn_int8_product(1, 1, 0, 1, None) == -1 and lib.sdfnn_gated_product(1, 1, 64, 64, 64, 0, 2, None) == -1
     assert lib.sdfnn_gated_product(0, 100, 64, 64, 64, 1, 3, None) in (128, 256) and lib.sdfnn_gated_product(5, 1, 64, 64, 64, 0, 0, None) == -1
+
+
+@pytest.mark.parametrize("background", ["grid", "none"])
+def test_blocks_of_a_background_without_them_are_refused(background):
+    """background_feature_blocks belongs to the "mlp" background; another one would train without the blocks it was asked for."""
+    from types import SimpleNamespace
+
+    from sdfstudio_amd.models.background import build_background
+
+    with pytest.raises(ValueError, match="background_feature_blocks"):
+        build_background(SimpleNamespace(), SimpleNamespace(background_model=background, background_feature_blocks=2))
