@@ -32,7 +32,8 @@ int sdfnn_version(void);
 const char* sdfnn_last_error(void);
 
 /* ---- root-mean-square norm
- * h = x + residual (residual NULL: h = x);  inv = 1 / sqrt(mean(h^2) + eps);  y = h inv weight, all in fp32 from the unrounded sum.
+ * h = x + residual (residual NULL: h = x);  inv = 1 / sqrt(mean(h^2) + eps);  y = h inv weight, all in fp32 from the unrounded sum
+ * (a row with values beyond 1e19 overflows its sum of squares, as in fp32 anywhere: inv = 0).
  * x, residual [rows, dim] with strides ldx / ldr; weight [dim]; y, h [rows, dim] contiguous (h: only with a residual, may be NULL);
  * inv [rows] fp32, what the backward reads (may be NULL). */
 int sdfnn_rms_norm_forward(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int32_t dtype, int64_t rows,
@@ -71,8 +72,9 @@ int sdfnn_int8_gated_linear(const int8_t* q, int64_t ldq, const float* sq, const
  * contiguous, y [rows, out] contiguous.  16-bit types: products of those types with fp32 sums; a is rounded to the type before the second
  * product (up to 16 rows it goes there as two numbers of the type that hold twice its bits), and so are the gradients of g
  * and u before theirs (fp16: a hidden value beyond 65504 becomes infinite - up to 16 rows of a forward pass: beyond 131008 - and gradients below 6e-8
- * vanish, as everywhere in that type: scale the loss).  fp32: every operand as three bf16 parts that hold its 24 bits, six products, fp32
- * sums (magnitudes below 2^-110 hold fewer bits).  A row with an input that is not finite gives NaN.
+ * vanish, as everywhere in that type: scale the loss).  fp32: fp32 instructions up to 64 rows; beyond, every operand as three bf16 parts that
+ * hold its 24 bits, six products, fp32 sums (magnitudes below 2^-110 hold fewer bits).  A row with an input that is not finite has no finite result:
+ * infinities or NaN as the arithmetic gives them, in fp32 beyond 64 rows NaN alone.
  * saved: sdfnn_gated_saved_size bytes, what the backward needs (act(g) and u act'(g) in fp32, a in the type; fp32 above 64 rows: a and x as
  * their three parts); NULL when none will follow. */
 int64_t sdfnn_gated_saved_size(int32_t dtype, int64_t rows, int64_t dim, int64_t hidden);

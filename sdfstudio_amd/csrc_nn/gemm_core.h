@@ -11,8 +11,8 @@
 //   * The weights' rows (n) are operand A of the instruction and the tokens' rows (m) operand B: a lane then owns ONE m and runs of 4
 //     consecutive n, which the epilogue stages through LDS in 16-byte pieces.
 //   * fp32: x = p0 + p1 + p2 with p0 = bf16(x), p1 = bf16(x - p0), p2 = bf16(x - p0 - p1) holds all 24 bits; of the nine products of two
-//     such sums the six largest are formed (the rest is below 2^-24 of |a b|), the small ones first: six passes over k that differ
-//     in the pair of parts they read.
+//     such sums the six largest are formed (the rest is below 2^-24 of |a b|): six steps for each 64 of k, the small ones first,
+//     which differ in the pair of parts they read and add to one fp32 sum, as the steps of a 16-bit product do.
 //   * Workgroups are numbered so that the ones that run at the same time on one XCD (ids equal mod 8) form a square-ish patch of tiles and
 //     share their operands in that XCD's L2.
 //   * Few tiles: k is split over workgroups; raw sums go to the workspace and a second kernel adds them in order and applies the epilogue.
@@ -32,9 +32,9 @@ struct GemmArgs {
   Operand a, b[2];  // b[1]: the second projection of a gated product, or what follows b[0] along k from step `turn` on
   int64_t M;
   int N;            // rows of one projection
-  int nk;           // steps of one pass
+  int nk;           // steps of k (fp32: each taken six times)
   int turn;
-  int per;          // steps (over all passes) of one split
+  int per;          // steps of one split (fp32: six for each of k)
   int gm, gn, splits;
   EPI epi;
 };
@@ -77,7 +77,7 @@ NN_D void load_lds(const i32x4 buffer, const unsigned offset, const unsigned to)
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(buffer), "s"(to) : "memory");
 }
 
-// the parts multiplied by pass t of an fp32 product, smallest terms first
+// the parts multiplied by term t of an fp32 product, smallest terms first
 NN_D int part_a(const int t) { return (0x001102 >> (4 * t)) & 3; }
 NN_D int part_b(const int t) { return (0x010120 >> (4 * t)) & 3; }
 

@@ -76,8 +76,8 @@ class _RMSNorm(torch.autograd.Function):
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
              eps: float = 1e-6) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
-    """y = h / sqrt(mean(h^2) + eps) * weight over the last dimension with h = x + residual, the statistic in fp32 from the unrounded sum.
-    Returns y, with a residual (y, h).  x [..., dim] in float32 / bfloat16 / float16, weight [dim] and residual of the same type; gradients
+    """y = h / sqrt(mean(h^2) + eps) * weight over the last dimension with h = x + residual, the statistic in fp32 from the unrounded sum (values
+    beyond 1e19 overflow their squares there).  Returns y, with a residual (y, h).  x [..., dim] in float32 / bfloat16 / float16, weight [dim] and residual of the same type; gradients
     for x, weight and residual (one pass; not differentiable twice)."""
     _check("rms_norm", x, weight, residual)
     _nn.check_modes("rms_norm", x, weight, residual, function=True)

@@ -4,7 +4,7 @@ Tolerances are counted in roundings as in test_gpu_nn_operators.py, whose refere
 import pytest
 import torch
 
-from test_gpu_nn_operators import ACTS, BF16, F16, close, gated_ref, half, rnd
+from test_gpu_nn_operators import ACTS, BF16, F16, F32, close, gated_ref, half, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +111,21 @@ def test_rows_of_long_strides(device, rows):
     assert torch.equal(int8_gated_linear(q, s, w, sw, w, sw), int8_gated_linear(q.contiguous(), s, w, sw, w, sw))
     few = base[:3, -1]  # as weights
     assert torch.equal(int8_linear(w, sw, few, s[:3]), int8_linear(w, sw, few.contiguous(), s[:3]))
+
+
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("rows", [5, 20, 50, 70, 3000])
+def test_rows_that_are_not_finite_have_no_finite_result(device, t, act, rows):
+    """An infinity or a NaN among a row's inputs, on every kernel: no result of that row is a number; fp32 beyond 64 rows gives NaN alone."""
+    from sdfstudio_amd.field_components.mlp import gated_mlp
+
+    x = rnd(rows, 64, t=t)
+    ws = [rnd(96, 64, t=t), rnd(96, 64, t=t), rnd(64, 96, t=t)]
+    x[0, 3], x[2, 60], x[4, 0] = float("inf"), float("-inf"), float("nan")
+    y = gated_mlp(x, *ws, activation=act)
+    bad = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    bad[[0, 2, 4]] = True
+    assert not torch.isfinite(y[bad]).any() and torch.isfinite(y[~bad]).all()
+    if t == F32 and rows > 64:
+        assert torch.isnan(y[bad]).all()
