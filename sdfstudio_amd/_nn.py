@@ -142,8 +142,8 @@ def differentiated(*tensors: Optional[torch.Tensor]) -> bool:
 
 
 # whether torch.jit.trace is recording: it keeps autograd functions as calls, nothing else of these operators
-traced = torch._C._is_tracing
-_modes = torch._C._len_torch_dispatch_stack
+traced = getattr(torch._C, "_is_tracing", None) or torch.jit.is_tracing
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", None) or (lambda: 1)
 
 
 def check_modes(what: str, *tensors: Optional[torch.Tensor], function: bool = False) -> None:

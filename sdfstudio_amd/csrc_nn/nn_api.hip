@@ -368,7 +368,7 @@ int32_t product_of(const Call& c, const int32_t index, int32_t* splits) {
 
 extern "C" {
 
-int sdfnn_version(void) { return 100; }
+int sdfnn_version(void) { return 101; }  // 101: sdfnn_int8_product, sdfnn_gated_product
 const char* sdfnn_last_error(void) { return g_err; }
 
 int sdfnn_rms_norm_forward(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int32_t dtype, int64_t rows,
